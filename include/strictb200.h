@@ -295,11 +295,51 @@ int strictb200_attn_decode(strictb200_ctx* ctx, const uint16_t* d_q, const uint1
 int strictb200_attn_decode_noalloc(strictb200_ctx* ctx, const uint16_t* d_q, const uint16_t* d_kcache, const uint16_t* d_vcache,
                                    const int32_t* d_lens, int B, int Hq, int Hkv, int D, int maxlen, float scale, uint16_t* d_out);
 
+/* ---- a paged cache (bf16, D = 64 or 128) ----
+ * Keys and values of a layer lie in pages of `page` positions (16, 32, 64, 128 or 256): d_kpages and d_vpages are [n_pages, Hkv, page, D].
+ * Position j of sequence b is slot j % page of page d_table[b * table_ld + j / page]. The new tokens of all sequences are rows of packed
+ * arrays: those of sequence b are rows d_starts[b] .. d_starts[b + 1] - 1 (B + 1 values, not falling, d_starts[0] >= 0, d_starts[B] <= T), and
+ * they are the last of its d_lens[b] tokens: row r has position d_lens[b] - d_starts[b + 1] + r. A sequence may have no new tokens. Rows in
+ * front of the first sequence and behind the last one are left as they are. The reference has no counterpart.
+ * Entries of the table outside [0, n_pages), and positions beyond table_ld pages, name no page: nothing is written there, and no
+ * row sees them. Two sequences may share a page as long as none of them writes into it. */
+
+/* Per-head RMS norm (both gains NULL: none), rotation of the pairs (i, i + D/2) by the angle position * theta^(-2i/D), queries to d_q_out
+ * [T,Hq,D], keys and values into the pages: strictb200_rope_qknorm_kvappend for a paged cache. d_qkv is [T, (Hq + 2 Hkv) * D]. Angles are reduced in
+ * 64 bits: any position an int32 holds. Rows, gains and pages 16-byte aligned. */
+int strictb200_rope_qknorm_paged(strictb200_ctx* ctx, const uint16_t* d_qkv, const int32_t* d_table, const int32_t* d_lens, const int32_t* d_starts, int B,
+                                 int64_t T, int Hq, int Hkv, int D, const float* d_qgain, const float* d_kgain, float eps, float theta, int n_pages,
+                                 int page, int table_ld, uint16_t* d_q_out, uint16_t* d_kpages, uint16_t* d_vpages);
+/* Attention of the new tokens, whose keys and values are in the pages already: a decode step (one new token per sequence), drafted tokens, chunks
+ * of prompts, or a mixture of them in one call. d_q, d_out [T,Hq,D]. The row at position p sees the keys j <= p with j > p - window (0: all of them)
+ * or j < first (the first tokens stay visible). What a row does not see does not reach it, whatever is there, and pages that no row
+ * sees are not read. A row that sees no key with a score above -inf gets zeros. max_new: no sequence has more new tokens; max_len: how long
+ * the sequences are at most, for planning (longer ones are computed too). Uses context scratch where keys are split. At most 128 query heads per
+ * key/value head. q, pages and out 16-byte aligned. */
+int strictb200_attn_paged(strictb200_ctx* ctx, const uint16_t* d_q, const uint16_t* d_kpages, const uint16_t* d_vpages, const int32_t* d_table,
+                          const int32_t* d_lens, const int32_t* d_starts, int B, int64_t T, int max_new, int max_len, int Hq, int Hkv, int D, int n_pages,
+                          int page, int table_ld, int window, int first, float scale, uint16_t* d_out);
+/* Page h_dst[i] becomes a copy of page h_src[i], i < n, in every one of n_pools device arrays of n_pages pages of page_bytes each (keys and values of
+ * all layers). The page numbers are read before the call returns. A destination is neither a source nor twice a destination (ERR_INVALID_ARG).
+ * page_bytes % 16 == 0, arrays 16-byte aligned. */
+int strictb200_pages_copy(strictb200_ctx* ctx, void* const* h_pools, int n_pools, int n_pages, int64_t page_bytes, const int32_t* h_src, const int32_t* h_dst,
+                          int n);
+
 /* ---- embedding / sampling ---- */
 int strictb200_embedding_bf16(strictb200_ctx* ctx, const uint16_t* d_table, const int32_t* d_ids, int64_t T, int64_t d, int64_t vocab,
                               uint16_t* d_out);
 /* argmax over the last dimension of fp32 [M,N]; ties go to the lowest index. */
 int strictb200_argmax(strictb200_ctx* ctx, const float* d_x, int64_t M, int64_t N, int32_t* d_out);
+/* One token per row of logits [M,N] (row stride ld; dtype 0 bf16, 1 fp32; N at most 2^20), drawn with the given random number d_u[row] in [0,1)
+ * (others are brought inside). The tokens of a row are ordered by falling logit, the lower index first. With w = exp((logit - largest) / temperature)
+ * the kept ones are the first top_k; of those the shortest beginning that holds top_p of their weight; of those the ones with w >= min_p. The token is
+ * the first by index at which the sum of the kept weights exceeds u times their sum; d_prob[row] (may be NULL) its share of that sum.
+ * d_temperature, d_top_k, d_top_p, d_min_p have a value per row and may be NULL. Temperature 0 or below (or NaN): the first of the order;
+ * NULL: 1. top_k below 1 or from N on, top_p from 1 on (or NaN), min_p 0 or below (or NaN): without. top_p 0 or below keeps one token; min_p above 1 is 1.
+ * NaN logits count as -inf, which is never drawn; a row without any other gives token -1 and share 0. Weights are held to 2^-44 of the largest and summed
+ * exactly, so that a result depends on nothing but the row's inputs. */
+int strictb200_sample(strictb200_ctx* ctx, const void* d_logits, int dtype, int64_t M, int64_t N, int64_t ld, const float* d_u, const float* d_temperature,
+                      const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, int32_t* d_out, float* d_prob);
 
 /* ---- model / KV-cache objects (new API in the style of the existing surface) ---- */
 enum strictb200_arch { STRICTB200_GPT2 = 0, STRICTB200_QWEN3 = 1, STRICTB200_STACK = 2 /* strictb200_stack_create */ };

@@ -1,0 +1,63 @@
+// What the kernels over a paged cache share: where a row of the packed new tokens belongs, and where a position lies.
+#pragma once
+#include "common.cuh"
+
+// Keys and values of a layer lie in pages [n_pages, Hkv, page, D]; row b of the table names the pages of sequence b in order. The new tokens of
+// all sequences are rows of one packed array: those of sequence b are starts[b] .. starts[b + 1] - 1, the last ones of its lens[b] tokens.
+struct PagedView {
+  const int32_t* table = nullptr;   // [B, ld]
+  const int32_t* lens = nullptr;    // [B]
+  const int32_t* starts = nullptr;  // [B + 1]
+  int B = 0, ld = 0, n_pages = 0;
+  int page = 0, shift = 0;          // slots of a page, a power of two, and its logarithm
+  int64_t T = 0;                    // rows of the packed array
+};
+
+struct PagedAttnArgs {
+  PagedView at;
+  const bf16* q = nullptr;  // [T, Hq, D]
+  const bf16* k = nullptr;  // pages
+  const bf16* v = nullptr;
+  int Hq = 0, Hkv = 0, D = 0;
+  int window = 0, first = 0;  // a row at position p sees j <= p with j > p - window (0: all) or j < first
+  int max_new = 0, max_len = 0;
+  float scale = 0.f;
+  bf16* out = nullptr;  // [T, Hq, D]
+};
+int k_attn_paged(strictb200_ctx*, const PagedAttnArgs& a);  // attention_paged.cu
+
+struct PagedRopeArgs {
+  PagedView at;
+  const bf16* qkv = nullptr;  // [T, (Hq + 2 Hkv) D]
+  const float* qgain = nullptr;  // null: no norm
+  const float* kgain = nullptr;
+  float eps = 0.f, theta = 0.f;
+  int Hq = 0, Hkv = 0, D = 0;
+  bf16* q_out = nullptr;
+  bf16* k = nullptr;
+  bf16* v = nullptr;
+};
+int k_rope_paged(strictb200_ctx*, const PagedRopeArgs& a);  // rope_paged.cu
+
+// Copies page src[i] of every pool over page dst[i]; no page is named twice but as a source. pages.cu
+int k_pages_copy(strictb200_ctx*, void* const* pools, int n_pools, int64_t page_bytes, const int32_t* src, const int32_t* dst, int n);
+
+#ifdef __CUDACC__
+// Sequence of packed row t (0 <= t < T): the first b with t < starts[b + 1]; B where the row is in front of the first or behind the last
+// sequence. All lanes of a warp call it with the same t.
+__device__ __forceinline__ int paged_seq(const PagedView& v, int64_t t) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < v.B; b0 += 32) {
+    const int b = b0 + lane;
+    const unsigned past = __ballot_sync(0xffffffffu, b < v.B && t < v.starts[min(b, v.B - 1) + 1]);
+    if (past) return t >= v.starts[0] ? b0 + __ffs(past) - 1 : v.B;
+  }
+  return v.B;
+}
+// Page of slot group `n` of sequence b, or -1 where the table names none.
+__device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
+  if (n >= v.ld) return -1;
+  const int p = v.table[(int64_t)b * v.ld + n];
+  return p >= 0 && p < v.n_pages ? p : -1;
+}
+#endif

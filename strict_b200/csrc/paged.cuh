@@ -60,4 +60,23 @@ __device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
   const int p = v.table[(int64_t)b * v.ld + n];
   return p >= 0 && p < v.n_pages ? p : -1;
 }
+// The key tiles (of `kt` positions) that rows at positions lo_pos .. hi_pos walk over: those of the first tokens, then those from the window on.
+struct PagedWalk {
+  int first = 0;   // tiles of the first tokens
+  int lo = 0;      // tile where the window begins
+  int total = 0;
+  int end = 0;     // no row sees this position or a later one
+  __device__ __forceinline__ int tile(int t) const { return t < first ? t : lo + t - first; }
+};
+__device__ __forceinline__ PagedWalk paged_walk(const PagedView& v, int len, int lo_pos, int hi_pos, int window, int first, int kt) {
+  PagedWalk w;
+  const int64_t room = (int64_t)v.ld << v.shift;
+  w.end = (int)(room < len ? room : len);
+  w.end = max(0, min(w.end, hi_pos + 1));
+  const int tiles = (w.end + kt - 1) / kt;
+  w.lo = window ? min(max(0, lo_pos - window + 1) / kt, tiles) : 0;
+  w.first = min((min(first, w.end) + kt - 1) / kt, w.lo);
+  w.total = w.first + tiles - w.lo;
+  return w;
+}
 #endif

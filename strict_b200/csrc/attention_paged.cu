@@ -1,58 +1,16 @@
 // Softmax attention of new tokens over a paged cache, grouped heads of 64 or 128 dims, bf16.
 //
-// One new token per sequence and at most 16 query heads per key/value head: attn_paged_decode_kernel. Otherwise one block per row and head.
+// One new token per sequence and at most 16 query heads per key/value head: the kernel here. Otherwise attention_paged_tc.cu.
 #include <algorithm>
 
 #include "mma_tiles.cuh"
-#include "paged.cuh"
+#include "attention_paged.cuh"
 
 using namespace mt;
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-
-// One block per row and head; tiles of 128 keys, a thread per key for the scores and a thread per dim for the values. Keys that the row does not
-// see are never read.
-__global__ void __launch_bounds__(128) attn_paged_rows_kernel(PagedAttnArgs a) {
-  __shared__ float q_s[128], p_s[128], red[32];
-  __shared__ int page_s[128];
-  const int64_t t = blockIdx.x;
-  const int h = blockIdx.y, i = threadIdx.x, D = a.D;
-  const int b = paged_seq(a.at, t);
-  if (b >= a.at.B) return;
-  const int len = a.at.lens[b], pos = len - a.at.starts[b + 1] + (int)t;
-  const int64_t head = h / (a.Hq / a.Hkv);
-  if (i < D) q_s[i] = __bfloat162float(a.q[(t * a.Hq + h) * D + i]) * a.scale;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int64_t j0 = 0; j0 <= pos && j0 < ((int64_t)a.at.ld << a.at.shift); j0 += 128) {
-    __syncthreads();
-    const int64_t j = j0 + i;
-    const bool seen = j <= pos && (!a.window || j > (int64_t)pos - a.window || j < a.first);
-    const int page = seen ? paged_page(a.at, b, (int)(j >> a.at.shift)) : -1;
-    page_s[i] = page;
-    float s = -INFINITY;
-    if (page >= 0) {
-      const bf16* k = a.k + ((page * (int64_t)a.Hkv + head) * a.at.page + (j & (a.at.page - 1))) * D;
-      s = 0.f;
-      for (int d = 0; d < D; d++) s += q_s[d] * __bfloat162float(k[d]);
-    }
-    const float top = fmaxf(m, block_max(s, red));
-    const float c = m == -INFINITY ? 0.f : expf(m - top);
-    const float p = page >= 0 && top != -INFINITY ? expf(s - top) : 0.f;
-    p_s[i] = p;
-    l = l * c + block_sum(p, red);
-    __syncthreads();
-    if (i < D) {
-      o *= c;
-      for (int n = 0; n < 128; n++)
-        if (page_s[n] >= 0)
-          o += p_s[n] * __bfloat162float(a.v[((page_s[n] * (int64_t)a.Hkv + head) * a.at.page + ((j0 + n) & (a.at.page - 1))) * D + i]);
-    }
-    m = top;
-  }
-  if (i < D) a.out[(t * a.Hq + h) * D + i] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
-}
 
 // ------------------------------------------------------------------ one new token per sequence
 // Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its key tiles; the G query heads of
@@ -68,16 +26,10 @@ constexpr int STAGES = 2;
 enum { JOIN_NONE = 0, JOIN_SCRATCH = 1, JOIN_CLUSTER = 2 };
 constexpr int CLUSTER_MAX = 8;
 
-struct JoinBuf {
-  float* o;    // [T, Hq, parts, D]
-  float2* ml;  // [T, Hq, parts]: maximum (log2) and sum
-  int parts;
-};
-
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
 
 template <int HD, int JOIN>
-__global__ void __launch_bounds__(128) attn_paged_decode_kernel(PagedAttnArgs a, JoinBuf join, int ct) {
+__global__ void __launch_bounds__(128) attn_paged_decode_kernel(PagedAttnArgs a, PagedJoin join, int ct) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int page_s[CT * 4];
   pdl_wait();
@@ -291,7 +243,7 @@ __global__ void __launch_bounds__(128) attn_paged_decode_kernel(PagedAttnArgs a,
 
 // A warp per row and head: out = sum_i w_i o_i / sum_i w_i l_i over the parts, w_i = 2^(m_i - max).
 template <int HD>
-__global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, JoinBuf join) {
+__global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, PagedJoin join) {
   constexpr int E = HD / 32;
   pdl_wait();
   pdl_trigger();
@@ -321,27 +273,6 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, J
 }
 
 template <int HD>
-int join_parts(strictb200_ctx* ctx, const PagedAttnArgs& a, const JoinBuf& join) {
-  SB_CUDA(sb_launch(ctx, attn_paged_join_kernel<HD>, dim3((unsigned)((a.at.T * a.Hq + 7) / 8)), dim3(256), 0, a, join));
-  ctx->launches++;
-  return STRICTB200_OK;
-}
-
-int join_scratch(strictb200_ctx* ctx, const PagedAttnArgs& a, int parts, JoinBuf* join) {
-  const size_t rows = (size_t)a.at.T * a.Hq * parts;
-  void* ws;
-  SB_TRY(sb_ws(ctx, rows * (a.D * sizeof(float) + sizeof(float2)), &ws));
-  *join = JoinBuf{(float*)ws, (float2*)((float*)ws + rows * a.D), parts};
-  return STRICTB200_OK;
-}
-
-int64_t walk_tiles(const PagedAttnArgs& a, int kt) {  // of a sequence of max_len tokens
-  const int64_t len = std::min<int64_t>(a.max_len, (int64_t)a.at.ld << a.at.shift), tiles = (len + kt - 1) / kt;
-  if (!a.window) return tiles;
-  return std::min<int64_t>(tiles, ((int64_t)a.window + a.max_new) / kt + 2 + ((int64_t)a.first + kt - 1) / kt);
-}
-
-template <int HD>
 int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   const size_t tiles_bytes = (size_t)2 * STAGES * KT * 2 * HD, join_bytes = (size_t)(5 * 16 * HD) * 4 + 5 * 16 * 8;
   const size_t smem = std::max(tiles_bytes, join_bytes);
@@ -353,7 +284,7 @@ int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
     }
     return cudaSuccess;
   }));
-  const int64_t tiles = std::max<int64_t>(1, walk_tiles(a, KT)), units = (int64_t)a.at.B * a.Hkv, slots = (int64_t)ctx->sm_count * 3;
+  const int64_t tiles = std::max<int64_t>(1, paged_walk_tiles(a, KT)), units = (int64_t)a.at.B * a.Hkv, slots = (int64_t)ctx->sm_count * 3;
   // One wave: as many parts as there are places, in a cluster of at most eight where that leaves a block few tiles. Several waves: pieces of at least
   // eight tiles, four waves of them if the sequences are as long as they may be, so that uneven lengths even out.
   int64_t parts = std::min(tiles, slots / units);
@@ -372,21 +303,40 @@ int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   if (parts <= 1) join = JOIN_NONE, parts = 1;
   const int ct = (int)std::min<int64_t>(CT, (tiles + parts - 1) / parts);
   const dim3 grid((unsigned)parts, (unsigned)a.Hkv, (unsigned)a.at.B);
-  JoinBuf buf{};
+  PagedJoin buf{};
   buf.parts = (int)parts;
-  if (join == JOIN_SCRATCH) SB_TRY(join_scratch(ctx, a, (int)parts, &buf));
+  if (join == JOIN_SCRATCH) SB_TRY(paged_join_scratch(ctx, a, (int)parts, &buf));
   if (join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, JOIN_NONE>, grid, dim3(128), smem, a, buf, ct));
   else if (join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, JOIN_SCRATCH>, grid, dim3(128), smem, a, buf, ct));
   else SB_CUDA(sb_launch_cluster(ctx, attn_paged_decode_kernel<HD, JOIN_CLUSTER>, grid, dim3(128), smem, dim3((unsigned)parts), a, buf, ct));
   ctx->launches++;
-  return join == JOIN_SCRATCH ? join_parts<HD>(ctx, a, buf) : STRICTB200_OK;
+  return join == JOIN_SCRATCH ? paged_join(ctx, a, buf) : STRICTB200_OK;
 }
 
 }  // namespace
 
-int k_attn_paged(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  if (a.max_new <= 1 && a.Hq / a.Hkv <= 16 && a.at.B <= 65535) return a.D == 128 ? decode<128>(ctx, a) : decode<64>(ctx, a);
-  attn_paged_rows_kernel<<<dim3((unsigned)a.at.T, (unsigned)a.Hq), 128, 0, ctx->stream>>>(a);
-  SB_LAUNCHED(ctx);
+int paged_join_scratch(strictb200_ctx* ctx, const PagedAttnArgs& a, int parts, PagedJoin* join) {
+  const size_t rows = (size_t)a.at.T * a.Hq * parts;
+  void* ws;
+  SB_TRY(sb_ws(ctx, rows * (a.D * sizeof(float) + sizeof(float2)), &ws));
+  join->o = (float*)ws;
+  join->ml = (float2*)((float*)ws + rows * a.D);
+  join->parts = parts;
   return STRICTB200_OK;
+}
+int paged_join(strictb200_ctx* ctx, const PagedAttnArgs& a, const PagedJoin& join) {
+  const dim3 grid((unsigned)((a.at.T * a.Hq + 7) / 8));
+  SB_CUDA(sb_launch(ctx, a.D == 128 ? attn_paged_join_kernel<128> : attn_paged_join_kernel<64>, grid, dim3(256), 0, a, join));
+  ctx->launches++;
+  return STRICTB200_OK;
+}
+int64_t paged_walk_tiles(const PagedAttnArgs& a, int kt) {
+  const int64_t len = std::min<int64_t>(a.max_len, (int64_t)a.at.ld << a.at.shift), tiles = (len + kt - 1) / kt;
+  if (!a.window) return tiles;
+  return std::min<int64_t>(tiles, ((int64_t)a.window + a.max_new) / kt + 2 + ((int64_t)a.first + kt - 1) / kt);
+}
+
+int k_attn_paged(strictb200_ctx* ctx, const PagedAttnArgs& a) {
+  if (a.max_new > 1 || a.Hq / a.Hkv > 16 || a.at.B > 65535) return k_attn_paged_tiles(ctx, a);
+  return a.D == 128 ? decode<128>(ctx, a) : decode<64>(ctx, a);
 }

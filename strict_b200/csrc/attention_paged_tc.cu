@@ -1,0 +1,584 @@
+// Softmax attention of new tokens over a paged cache on the tcgen05 tensor cores: drafted tokens, chunks and whole prompts.
+//
+// A row of the products is one query head of one new token: the G heads that share a key/value head are packed behind one another, 128 / G tokens to a
+// tile of 128 rows (one TMA box: 64 dims x G heads x tokens), so keys and values are fetched once for all of them and a tile spans few positions. Rows
+// are lanes of tensor memory. Per tile of 128 keys, as in the attention over contiguous caches:
+//   S = Q K^T      operands in shared memory, fp32 sums in tensor memory
+//   softmax        two threads per row (64 columns each), running maximum followed lazily (a row of O is rescaled when its maximum grew by more
+//                  than 2^8), weights back to tensor memory as two bf16 terms (hi + lo by truncation: 2^-16)
+//   O += P V       weights from tensor memory, values from shared memory; O stays in tensor memory
+// Roles: warps 0..15 softmax, 16 issues products, 17 copies, 18 and 19 look over values. A block works on two things in turn, so that the tensor
+// pipe runs one while the softmax warps are at the other:
+//   two tiles (ONE = false)   A and B, 2 * (128 / G) consecutive tokens, sharing every key tile
+//   one tile (ONE = true)     few rows: the even and the odd key tiles of the same queries, each with a softmax of its own; joined later
+// Keys may be split further over `parts` blocks. Whatever is split leaves (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel.
+//
+// Pages: a tile of 128 keys is 128 / page boxes (or part of a page); the lanes of the copying warp look up one page each, one tile ahead. A page that
+// the table does not name, or that begins behind the last position any row sees, is not fetched, and its keys are hidden by a bit mask.
+// What lies at hidden positions must not count: scores are replaced by index, but a weight of zero times a value that is not finite is not zero, and
+// places that were not fetched hold anything. So in tiles where some row does not see some key, two warps put zeros over values that no row sees, and over those
+// that are not finite; if there were any of the latter (`poison`), the rows that do see them add them at the end.
+#include <algorithm>
+
+#include "attention_paged.cuh"
+#include "tcgen05.cuh"
+
+using namespace tc;
+
+namespace {
+
+constexpr int BQ = 128, BKV = 128;
+constexpr int THREADS = 640;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct TilesArgs {
+  PagedAttnArgs a;
+  PagedJoin join;  // parts of the output: ONE: 2 * parts, otherwise parts
+  int parts, ct;   // blocks that share the keys, tiles of a piece
+  int G, tw;       // heads per key/value head, tokens of a tile of 128 rows
+  int64_t tiles;   // tiles of tokens in the grid
+  int* status;
+};
+
+// What a block works on, the same in all of its threads.
+struct Work {
+  int b, hk, part;
+  int64_t row0;          // first row in q and out
+  int n;                 // tokens
+  int lo_pos;            // position of the first token
+  int lo_key;            // first key in the window of the first token
+  PagedWalk w;
+  int nt;                // key tiles of this block
+};
+
+// i-th key tile of a block whose share is every parts-th piece of ct tiles
+__device__ __forceinline__ int share_tile(int i, int part, int parts, int ct) { return parts == 1 ? i : (i / ct * parts + part) * ct + i % ct; }
+__device__ __forceinline__ int share_count(int total, int part, int parts, int ct) {
+  if (parts == 1) return total;
+  const int rounds = total / (parts * ct), rest = total - rounds * parts * ct;
+  return rounds * ct + min(max(rest - part * ct, 0), ct);
+}
+
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+
+// Whether the keys [k0, k0 + 128) are all seen by the rows at positions lo .. hi.
+__device__ __forceinline__ bool sees_all(const PagedAttnArgs& a, int end, int k0, int lo, int hi) {
+  return k0 + BKV <= end && k0 + BKV - 1 <= lo && (!a.window || k0 > hi - a.window || k0 + BKV <= a.first);
+}
+
+// The values that are not finite, of the keys that the row at `pos` sees, in dims [d0, d0 + 32): of the tiles that had theirs replaced.
+__device__ __noinline__ void add_poison(const TilesArgs& t, const Work& k, int pos, int first_i, int step_i, int n_i, int d0, uint32_t* r) {
+  const PagedAttnArgs& a = t.a;
+  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  for (int s = 0; s < n_i; s++) {
+    const int k0 = k.w.tile(share_tile(first_i + s * step_i, k.part, t.parts, t.ct)) * BKV;
+    for (int j = k0; j < min(k0 + BKV, min(k.w.end, pos + 1)); j++) {
+      if (j < lo && j >= a.first) continue;
+      const int page = paged_page(a.at, k.b, j >> a.at.shift);
+      if (page < 0) continue;
+      const bf16* v = a.v + ((page * (int64_t)a.Hkv + k.hk) * a.at.page + (j & (a.at.page - 1))) * a.D + d0;
+      for (int i = 0; i < 32; i++) {
+        const float x = __bfloat162float(v[i]);
+        if (!isfinite(x)) r[i] = __float_as_uint(__uint_as_float(r[i]) + x);
+      }
+    }
+  }
+}
+
+template <int QA, bool ONE>
+constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 4) * QA * HALF_BYTES + 1024; }
+
+template <int QA, bool ONE>
+__global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TilesArgs t) {
+  constexpr int TILE = QA * HALF_BYTES, NQ = ONE ? 1 : 2, D = 64 * QA;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t bar_q, k_full[2], k_empty[2], v_full[2], v_ready[2], v_empty[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ float x_max[2][2][BQ], x_sum[2][BQ];  // [stream][column half][row]
+  __shared__ uint32_t page_bits[4];                // pages of a key tile that are there
+  __shared__ int poison;
+  const PagedAttnArgs& a = t.a;
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  Work k;
+  {
+    const int per = a.Hkv * t.parts;
+    const int64_t x = t.tiles - 1 - blockIdx.x / per;  // the last tokens of a prompt see the most keys: they go first
+    k.part = blockIdx.x % per / a.Hkv;
+    k.hk = blockIdx.x % a.Hkv;
+    // tiles of sequence b begin at (starts[b] - starts[0]) / tokens of a block + b: room for all of them, found without a list
+    const int tb = NQ * t.tw, s0 = a.at.starts[0];
+    int before = 0;
+    for (int b0 = 0; b0 < a.at.B; b0 += 32) {
+      const int b = b0 + lane;
+      const unsigned m = __ballot_sync(0xffffffffu, b < a.at.B && (int64_t)(a.at.starts[min(b, a.at.B - 1)] - s0) / tb + b <= x);
+      before += __popc(m);
+      if (m != 0xffffffffu) break;
+    }
+    k.b = before - 1;
+    if (k.b < 0) return;
+    const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb;
+    const int64_t q0 = (x - ((int64_t)(sb - s0) / tb + k.b)) * tb;
+    if (q0 < 0 || q0 >= n_new || sb < 0 || (int64_t)sb + n_new > a.at.T) return;
+    k.row0 = sb + q0;
+    k.n = (int)min((int64_t)tb, n_new - q0);
+    const int len = a.at.lens[k.b];
+    k.lo_pos = len - n_new + (int)q0;
+    k.lo_key = a.window ? max(0, k.lo_pos - a.window + 1) : 0;
+    k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
+    k.nt = share_count(k.w.total, k.part, t.parts, t.ct);
+  }
+  // key tiles of each stream: ONE: every other one; otherwise tile A ends where its last token does
+  int nt[2];
+  if (ONE) {
+    nt[0] = (k.nt + 1) / 2;
+    nt[1] = k.nt / 2;
+  } else {
+    const int end_a = max(0, min(k.w.end, k.lo_pos + min(k.n, t.tw)));
+    nt[0] = min(k.nt, share_count(k.w.first + max(0, (end_a + BKV - 1) / BKV - k.w.lo), k.part, t.parts, t.ct));
+    nt[1] = k.n > t.tw ? k.nt : 0;
+    k.nt = max(nt[0], nt[1]);
+  }
+  auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, t.ct)) * BKV; };  // first key of the block's i-th tile
+
+  const uint32_t sQ = smem_u32(smem), sK = sQ + NQ * TILE, sV = sK + 2 * TILE;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar_q), 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&k_full[i]), 1); mbar_init(smem_u32(&k_empty[i]), 1);
+      mbar_init(smem_u32(&v_full[i]), 1); mbar_init(smem_u32(&v_ready[i]), 64); mbar_init(smem_u32(&v_empty[i]), 1);
+      mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i]), 2 * BQ); mbar_init(smem_u32(&bar_o[i]), 1);
+    }
+    poison = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 16) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem = tmem_base_slot;
+  constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  const int box = min(a.at.page, BKV), boxes = BKV / box;  // keys of a box; boxes of a tile
+
+  if (warp == 17) {
+    // ---- copies. Lane i looks up the i-th box of a tile, one tile ahead.
+    if (lane == 0 && k.nt > 0) {
+      const uint32_t bytes = (uint32_t)(t.G * t.tw * 128 * QA);
+      const int nq = !ONE && nt[1] ? 2 : 1;
+      mbar_expect_tx(smem_u32(&bar_q), nq * bytes);
+      for (int w = 0; w < nq; w++)
+        for (int i = 0; i < QA; i++) tma_load_3d(sQ + w * TILE + i * HALF_BYTES, &map_q, i * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&bar_q));
+    }
+    auto look_up = [&](int i) {
+      if (i >= k.nt || lane >= boxes) return -1;
+      const int j = tile_key(i) + lane * box;
+      return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
+    };
+    int page = look_up(0), got = 0;
+    bool good = true;
+    for (int i = 0; i < k.nt; i++) {
+      const int next = look_up(i + 1), st = i & 1;
+      const uint32_t ph = (uint32_t)((i >> 1) & 1) ^ 1;
+      const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+      const uint32_t bytes = (uint32_t)(__popc(there) * box * 128 * QA);
+      const int row = page < 0 ? 0 : (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
+      if (i >= 2) good = mbar_wait(smem_u32(&k_empty[st]), ph);
+      if (!__all_sync(0xffffffffu, good)) { if (lane == 0) set_status(t.status, 41); good = false; break; }
+      if (lane == 0) {
+        page_bits[i & 3] = there;
+        mbar_expect_tx(smem_u32(&k_full[st]), bytes);
+      }
+      __syncwarp();
+      if (page >= 0)
+        for (int x = 0; x < QA; x++) tma_load_2d(sK + st * TILE + x * HALF_BYTES + lane * box * 128, &map_k, x * 64, row, smem_u32(&k_full[st]));
+      if (i >= 2) good = mbar_wait(smem_u32(&v_empty[st]), ph);
+      if (!__all_sync(0xffffffffu, good)) { if (lane == 0) { set_status(t.status, 42); mbar_wait(smem_u32(&k_full[st]), ph ^ 1); } good = false; break; }
+      if (lane == 0) mbar_expect_tx(smem_u32(&v_full[st]), bytes);
+      __syncwarp();
+      if (page >= 0)
+        for (int x = 0; x < QA; x++) tma_load_2d(sV + st * TILE + x * HALF_BYTES + lane * box * 128, &map_v, x * 64, row, smem_u32(&v_full[st]));
+      page = next;
+      got = i + 1;
+    }
+    // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
+    if (lane == 0 && k.nt > 0) {
+      mbar_wait(smem_u32(&bar_q), 0);
+      for (int i = max(0, got - 2); i < got; i++) {
+        mbar_wait(smem_u32(&k_full[i & 1]), (uint32_t)((i >> 1) & 1));
+        mbar_wait(smem_u32(&v_full[i & 1]), (uint32_t)((i >> 1) & 1));
+      }
+    }
+    __syncwarp();
+  } else if (warp == 16) {
+    // ---- products
+    if (lane == 0 && k.nt > 0) {
+      auto issue_s = [&](int w, int st) {
+        const uint32_t tS = tmem + (uint32_t)(w * 256);
+#pragma unroll
+        for (int s = 0; s < 4 * QA; s++) {
+          const uint32_t off = (uint32_t)((s >> 2) * HALF_BYTES + (s & 3) * 32);
+          tc_mma_ss(tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
+        }
+        tc_commit(smem_u32(&bar_s[w]));
+      };
+      auto issue_pv = [&](int w, int st, bool first) {
+        const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+          const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
+          const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
+          tc_mma_ts(tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
+          tc_mma_ts(tO, tS + pcol + 16, dv, idesc_pv, 1u);
+        }
+        tc_commit(smem_u32(&bar_o[w]));
+      };
+      bool good = mbar_wait(smem_u32(&bar_q), 0);
+      if (ONE) {
+        for (int w = 0; w < 2 && good; w++) {
+          if (nt[w] == 0) break;
+          good = mbar_wait(smem_u32(&k_full[w]), 0);
+          if (!good) break;
+          tc_fence_after();
+          issue_s(w, w);
+          tc_commit(smem_u32(&k_empty[w]));
+        }
+        for (int s = 0; s < nt[0] && good; s++) {
+          for (int w = 0; w < 2 && good; w++) {
+            if (s >= nt[w]) break;
+            good = mbar_wait(smem_u32(&v_ready[w]), (uint32_t)(s & 1)) && mbar_wait(smem_u32(&bar_p[w]), (uint32_t)(s & 1));
+            if (!good) break;
+            tc_fence_after();
+            issue_pv(w, w, s == 0);
+            tc_commit(smem_u32(&v_empty[w]));
+            if (s + 1 < nt[w]) {
+              good = mbar_wait(smem_u32(&k_full[w]), (uint32_t)((s + 1) & 1));
+              if (!good) break;
+              tc_fence_after();
+              issue_s(w, w);
+              tc_commit(smem_u32(&k_empty[w]));
+            }
+          }
+        }
+      } else {
+        good = good && mbar_wait(smem_u32(&k_full[0]), 0);
+        if (good) {
+          tc_fence_after();
+          for (int w = 0; w < 2; w++)
+            if (nt[w] > 0) issue_s(w, 0);
+          tc_commit(smem_u32(&k_empty[0]));
+        }
+        for (int i = 0; i < k.nt && good; i++) {
+          const int st = i & 1;
+          good = mbar_wait(smem_u32(&v_ready[st]), (uint32_t)((i >> 1) & 1));
+          bool k_next = false;
+          for (int w = 0; w < 2 && good; w++) {
+            if (i < nt[w]) {
+              good = mbar_wait(smem_u32(&bar_p[w]), (uint32_t)(i & 1));
+              if (!good) break;
+              tc_fence_after();
+              issue_pv(w, st, i == 0);
+            }
+            if (i + 1 < nt[w]) {
+              if (!k_next) {
+                good = mbar_wait(smem_u32(&k_full[(i + 1) & 1]), (uint32_t)(((i + 1) >> 1) & 1));
+                if (!good) break;
+                tc_fence_after();
+                k_next = true;
+              }
+              issue_s(w, (i + 1) & 1);
+            }
+          }
+          if (!good) break;
+          tc_commit(smem_u32(&v_empty[st]));
+          if (i + 1 < k.nt) tc_commit(smem_u32(&k_empty[(i + 1) & 1]));
+        }
+      }
+      if (!good) set_status(t.status, 43);
+    }
+    __syncwarp();
+  } else if (warp >= 18) {
+    // ---- values of tiles that not every row sees whole
+    const int tid = (int)threadIdx.x - 18 * 32;
+    bool good = true;
+    for (int i = 0; i < k.nt && good; i++) {
+      const int st = i & 1, k0 = tile_key(i);
+      good = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((i >> 1) & 1));
+      if (!good) break;
+      const uint32_t bits = page_bits[i & 3];
+      if (bits != (1u << boxes) - 1 || !sees_all(a, k.w.end, k0, k.lo_pos, k.lo_pos + k.n - 1)) {
+        uint32_t found = 0;
+        uint4* v = (uint4*)(smem + (NQ + 2 + st) * TILE);
+        for (int x = tid; x < QA * BKV * 8; x += 64) {
+          const int r = (x >> 3) & (BKV - 1), j = k0 + r;
+          const bool seen = j < k.w.end && (bits >> (r / box) & 1) && (j >= k.lo_key || j < a.first);
+          if (!seen) {
+            v[x] = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          const uint4 w = v[x];
+          if (not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w)) {
+            auto clean = [](uint32_t y) {
+              const uint32_t f = not_finite(y);
+              return y & ~((f >> 15) * 0xFFFFu);
+            };
+            v[x] = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+            found = 1;
+          }
+        }
+        if (found) poison = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&v_ready[st])) : "memory");
+    }
+    if (!good && lane == 0) set_status(t.status, 44);
+  } else {
+    // ---- softmax of stream w
+    const int w = warp >> 3, half = (warp >> 2) & 1, row = (int)threadIdx.x & (BQ - 1);
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    auto wg_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); };  // the 256 threads of this stream
+    const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
+    const int tok = row / t.G + (ONE ? 0 : w * t.tw);
+    const bool live = row < t.G * t.tw && tok < k.n;
+    const bool any_live = __any_sync(0xffffffffu, live);  // a warp without rows only keeps step
+    const int pos_a = k.lo_pos + (ONE ? 0 : w * t.tw), pos_b = k.lo_pos + min(k.n, (ONE ? 1 : 1 + w) * t.tw) - 1;  // positions of the stream's tokens
+    const int pos = k.lo_pos + tok;
+    const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const float scale_log2 = a.scale * LOG2E;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;  // after a wait that gave up the steps go on without waiting, so that no one is left alone at a barrier
+    for (int s = 0; s < nt[w]; s++) {
+      const uint32_t ph = (uint32_t)(s & 1);
+      const int i = ONE ? 2 * s + w : s;
+      ok = ok && mbar_wait(smem_u32(&bar_s[w]), ph);
+      __syncwarp();  // the loads from tensor memory want the warp together
+      tc_fence_after();
+      const int k0 = tile_key(i);
+      const uint32_t bits = page_bits[i & 3];
+      const bool full = bits == (1u << boxes) - 1 && sees_all(a, k.w.end, k0, pos_a, pos_b);
+      // columns that this row sees, from this thread's 64 on
+      uint64_t see = ~0ull;
+      if (!full) {
+        see = 0;
+        const int c0 = k0 + 64 * half, hi = min(k.w.end, pos + 1) - c0, lw = lo - c0, fi = a.first - c0;
+        const uint64_t below_hi = hi >= 64 ? ~0ull : hi > 0 ? (1ull << hi) - 1 : 0;
+        const uint64_t below_lo = lw >= 64 ? ~0ull : lw > 0 ? (1ull << lw) - 1 : 0;
+        const uint64_t below_fi = fi >= 64 ? ~0ull : fi > 0 ? (1ull << fi) - 1 : 0;
+        see = below_hi & (~below_lo | below_fi);
+        for (int x = 0; x < 64; x += 16)
+          if (!(bits >> ((64 * half + x) / box) & 1)) see &= ~(0xFFFFull << x);
+      }
+      float m_tile = -INFINITY;
+      if (any_live) {
+#pragma unroll 1
+        for (int c = 0; c < 2; c++) {
+          uint32_t r[32];
+          tc_ld32(tS + lane_base + (uint32_t)((2 * half + c) * 32), r);
+          tc_wait_ld();
+          if (full) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) m_tile = fmaxf(m_tile, __uint_as_float(r[j]));
+          } else {
+            const uint32_t bm = (uint32_t)(see >> (32 * c));
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+              if (bm >> j & 1) m_tile = fmaxf(m_tile, __uint_as_float(r[j]));
+          }
+        }
+        x_max[w][half][row] = m_tile;
+      }
+      wg_sync();
+      if (any_live) {
+        m_tile = fmaxf(x_max[w][0][row], x_max[w][1][row]) * scale_log2;
+        const bool grow = m_tile > m_run + 8.0f;
+        const float m_use = grow ? m_tile : m_run;
+        const float corr = grow ? exp2f(m_run - m_use) : 1.0f;
+        m_run = m_use;
+        if (s > 0 && __any_sync(0xffffffffu, grow)) {
+          ok = ok && mbar_wait(smem_u32(&bar_o[w]), ph ^ 1);  // the product in front has finished O
+          __syncwarp();
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = QA * half; c < QA * half + QA; c++) {
+            uint32_t r[32];
+            tc_ld32(tO + lane_base + (uint32_t)(c * 32), r);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * corr);
+            tc_st32(tO + lane_base + (uint32_t)(c * 32), r);
+          }
+        }
+        const float base = m_use == -INFINITY ? 0.f : -m_use;
+        float row_sum = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < 2; c++) {
+          const uint32_t at = tS + lane_base + (uint32_t)((2 * half + c) * 32);
+          uint32_t r[32];
+          tc_ld32(at, r);
+          tc_wait_ld();
+          const uint32_t bm = (uint32_t)(see >> (32 * c));
+          uint32_t hi[16], lo16[16];
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            float p0 = ex2_approx(fmaf(__uint_as_float(r[2 * j]), scale_log2, base));
+            float p1 = ex2_approx(fmaf(__uint_as_float(r[2 * j + 1]), scale_log2, base));
+            if (!full) {
+              if (!(bm >> (2 * j) & 1)) p0 = 0.f;
+              if (!(bm >> (2 * j + 1) & 1)) p1 = 0.f;
+            }
+            row_sum += p0 + p1;
+            const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+            hi[j] = __byte_perm(b0, b1, 0x7632);
+            const uint32_t l0 = __float_as_uint(p0 - __uint_as_float(b0 & 0xFFFF0000u)), l1 = __float_as_uint(p1 - __uint_as_float(b1 & 0xFFFF0000u));
+            lo16[j] = __byte_perm(l0, l1, 0x7632);
+          }
+          tc_st16(at, hi);
+          tc_st16(at + 16, lo16);
+        }
+        tc_wait_st();
+        l_run = l_run * corr + row_sum;
+      }
+      tc_fence_before();
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w])) : "memory");
+      wg_sync();  // x_max is rewritten in the next step
+    }
+    if (nt[w] > 0) {
+      ok = ok && mbar_wait(smem_u32(&bar_o[w]), (uint32_t)((nt[w] - 1) & 1));
+      __syncwarp();
+      tc_fence_after();
+    }
+    if (!ok && lane == 0) set_status(t.status, 45);
+    if (half) x_sum[w][row] = l_run;
+    wg_sync();
+    if (!half) x_sum[w][row] += l_run;
+    wg_sync();
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok && any_live) {
+      const float sum = x_sum[w][row];
+      const int64_t at = (k.row0 + tok) * a.Hq + k.hk * t.G + row % t.G;
+      const int np = ONE ? 2 * t.parts : t.parts, p = ONE ? 2 * k.part + w : k.part;
+      const bool split = np > 1;
+      const float inv = split ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
+      if (split && live && !half) t.join.ml[at * np + p] = make_float2(m_run, sum);
+      const bool bad = *(volatile int*)&poison;
+#pragma unroll 1
+      for (int c = QA * half; c < QA * half + QA; c++) {
+        uint32_t r[32];
+        __syncwarp();
+        if (nt[w] > 0) {
+          tc_ld32(tO + lane_base + (uint32_t)(c * 32), r);
+          tc_wait_ld();
+        }
+        if (!live || (split && sum == 0.f)) continue;
+        if (sum == 0.f) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) r[j] = 0;
+        } else if (bad) {
+          add_poison(t, k, pos, ONE ? w : 0, ONE ? 2 : 1, nt[w], c * 32, r);
+        }
+        if (split) {
+          float* dst = t.join.o + (at * np + p) * D + c * 32;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) *(uint4*)(dst + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+        } else {
+          bf16* dst = a.out + at * D + c * 32;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 v;
+            v.x = f32_to_bf16_bits(__uint_as_float(r[j]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 1]) * inv) << 16);
+            v.y = f32_to_bf16_bits(__uint_as_float(r[j + 2]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 3]) * inv) << 16);
+            v.z = f32_to_bf16_bits(__uint_as_float(r[j + 4]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 5]) * inv) << 16);
+            v.w = f32_to_bf16_bits(__uint_as_float(r[j + 6]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 7]) * inv) << 16);
+            *(uint4*)(dst + j) = v;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 16) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// rows of `cols` bf16, boxes of `box` rows x 64 columns, 128-byte swizzle
+int map_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box) {
+  EncodeFn encode;
+  SB_TRY(encode_fn(&encode));
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  cuuint32_t boxes[2] = {64u, (cuuint32_t)box};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return sb_fail(STRICTB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return STRICTB200_OK;
+}
+// [T, heads, cols], boxes of `tokens` x G heads x 64 columns
+int map_tokens(CUtensorMap* map, const void* base, int64_t T, int heads, int cols, int G, int tokens) {
+  EncodeFn encode;
+  SB_TRY(encode_fn(&encode));
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)heads, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * heads * 2};
+  cuuint32_t boxes[3] = {64u, (cuuint32_t)G, (cuuint32_t)tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return sb_fail(STRICTB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return STRICTB200_OK;
+}
+
+template <int QA, bool ONE>
+int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
+  TilesArgs t;
+  t.a = a;
+  t.G = a.Hq / a.Hkv;
+  t.tw = BQ / t.G;
+  t.status = ctx->d_status;
+  const int tb = (ONE ? 1 : 2) * t.tw;
+  t.tiles = a.at.T / tb + a.at.B;
+  // Parts: the fewest rounds of key tiles over the SMs, a block counted with three tiles more (its start and its end) and the join with four.
+  const int64_t units = std::max<int64_t>((a.at.T + tb - 1) / tb, a.at.B) * a.Hkv, keys = std::max<int64_t>(1, paged_walk_tiles(a, BKV));
+  int64_t best = INT64_MAX;
+  t.parts = 1;
+  for (int p = 1; p <= 64 && p <= keys; p++) {
+    if (p > 1 && (size_t)a.at.T * a.Hq * p * (ONE ? 2 : 1) * (64 * QA + 2) * 4 > ((size_t)256 << 20)) break;
+    const int64_t cost = (units * p + ctx->sm_count - 1) / ctx->sm_count * ((keys + p - 1) / p + 3) + (p > 1 ? 4 : 0);
+    if (cost < best) best = cost, t.parts = p;
+  }
+  t.ct = (int)((keys + t.parts - 1) / t.parts);
+  const int np = (ONE ? 2 : 1) * t.parts;
+  if (np > 1) SB_TRY(paged_join_scratch(ctx, a, np, &t.join));
+  const int64_t blocks = t.tiles * a.Hkv * t.parts;
+  if (blocks > INT32_MAX) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "attention: too many rows and heads for one call");
+  CUtensorMap mq, mk, mv;
+  const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
+  SB_TRY(map_tokens(&mq, a.q, a.at.T, a.Hq, a.D, t.G, t.tw));
+  SB_TRY(map_rows(&mk, a.k, rows, a.D, std::min(a.at.page, BKV)));
+  SB_TRY(map_rows(&mv, a.v, rows, a.D, std::min(a.at.page, BKV)));
+  constexpr size_t smem = tiles_smem<QA, ONE>();
+  static SbDeviceOnce once;  // one per instantiation
+  SB_CUDA(once.run(ctx->device, [&] { return cudaFuncSetAttribute(attn_paged_tiles_kernel<QA, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
+  SB_CUDA(sb_launch(ctx, attn_paged_tiles_kernel<QA, ONE>, dim3((unsigned)blocks), dim3(THREADS), smem, mq, mk, mv, t));
+  ctx->launches++;
+  return np > 1 ? paged_join(ctx, a, t.join) : STRICTB200_OK;
+}
+
+}  // namespace
+
+int k_attn_paged_tiles(strictb200_ctx* ctx, const PagedAttnArgs& a) {
+  if ((int64_t)a.at.n_pages * a.Hkv * a.at.page > INT32_MAX) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "attention: more than 2^31 - 1 rows of keys");
+  const bool one = (int64_t)a.max_new * (a.Hq / a.Hkv) <= BQ;  // one tile per sequence
+  if (a.D == 128) return one ? launch<2, true>(ctx, a) : launch<2, false>(ctx, a);
+  return one ? launch<1, true>(ctx, a) : launch<1, false>(ctx, a);
+}

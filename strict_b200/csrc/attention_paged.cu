@@ -13,169 +13,243 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ one new token per sequence
-// Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its key tiles; the G query heads of
-// the key/value head are the rows of the products (mma.sync m16n8k16, 16 rows), warp w owns keys 16 w .. 16 w + 15 of every tile of 64 with a softmax
-// of its own, and the four warps are joined at the end. Tiles come by cp.async into two stages; page numbers are fetched one piece of the walk (CT tiles) at
-// a time. Positions that the row does not see, or whose entry names no page, are zeros in the tiles and -inf among the scores, so nothing that lies there counts.
+// Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its tiles of 64 keys. Warp 4 copies:
+// its lanes look up a page each, one tile ahead, and request the tile by TMA (boxes of min(page, 64) keys x 64 dims, 128-byte swizzle) into a ring
+// of STAGES. Warp w < 4 owns keys 16 w .. 16 w + 15 of every tile, with a softmax of its own; the four are joined at the end.
+// Products are mma.sync m16n8k16 with keys (then dims) as the 16 rows and query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T: at most eight heads
+// waste nothing that way. (With the heads as rows, half of everything was idle: 874 instructions per warp and tile, 166 registers and 5.3 TB/s.)
+// Positions that the row does not see, or whose entry names no page, are not fetched or hidden by index: their scores become -inf and the warp that
+// owns them puts zeros over their values, so nothing that lies there counts.
 //
-// Shares: chunk c of CT tiles belongs to block c % gridDim.x, however long the sequence turns out to be. JOIN: 0 there is one block, 1 the
+// Shares: piece c of ct tiles belongs to block c % gridDim.x, however long the sequence turns out to be. JOIN: 0 there is one block, 1 the
 // blocks leave (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel, 2 they are one cluster and join through distributed shared memory.
 constexpr int KT = 64;
-constexpr int CT = 64;  // tiles of a piece at most: 1 KB of page numbers
 constexpr int STAGES = 2;
+constexpr int DEC_THREADS = 160;
 enum { JOIN_NONE = 0, JOIN_SCRATCH = 1, JOIN_CLUSTER = 2 };
 constexpr int CLUSTER_MAX = 8;
 
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-template <int HD, int JOIN>
-__global__ void __launch_bounds__(128) attn_paged_decode_kernel(PagedAttnArgs a, PagedJoin join, int ct) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int page_s[CT * 4];
-  pdl_wait();
-  pdl_trigger();
+constexpr size_t dec_tile_bytes(int HD) { return (size_t)KT * 2 * HD; }
+constexpr size_t dec_smem(int HD) {
+  const size_t ring = 2 * STAGES * dec_tile_bytes(HD), join = (size_t)(4 * 16 * (HD + 4) + 16 * HD) * 4 + 5 * 16 * 8;
+  return (ring > join ? ring : join) + 1024;
+}
+
+// NB: blocks of eight query heads
+template <int HD, int NB, int JOIN>
+__global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                        const __grid_constant__ PagedAttnArgs a, PagedJoin join, int ct, int* status) {
+  constexpr int ATOM = KT * 128, TILE = ATOM * (HD / 64);  // bytes of 64 keys x 64 dims, and of a tile
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint32_t page_bits[STAGES];
   const int part = blockIdx.x, parts = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = a.Hq / a.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3, mi = lane >> 3, r8 = lane & 7;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; i++) {
+      tc::mbar_init(smem_u32(&full[i]), 1);
+      tc::mbar_init(smem_u32(&empty[i]), 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
   const int64_t t0 = a.at.starts[b];
-  const bool real = t0 >= 0 && t0 < a.at.T && a.at.starts[b + 1] > t0;  // the same for every block of a cluster
-  if (!real) return;
-  const int len = a.at.lens[b], pos = len - a.at.starts[b + 1] + (int)t0;
+  const int last = a.at.starts[b + 1], len = a.at.lens[b];
+  if (t0 < 0 || t0 >= a.at.T || last <= t0) return;  // the same for every block of a cluster
+  const int pos = len - last + (int)t0;
   const PagedWalk w = paged_walk(a.at, len, pos, pos, a.window, a.first, KT);
   const int lo = a.window ? max(0, pos - a.window + 1) : 0;
-  const uint32_t sK = smem_u32(smem), sV = sK + STAGES * KT * 2 * HD;
-  const int gp = a.at.page < KT ? KT / a.at.page : 1, gshift = a.at.page < KT ? a.at.shift : 6;  // pages of a tile; slots of a tile in one page
+  const int n = share_count(w.total, part, parts, ct);
+  const uint32_t sK = smem_u32(smem), sV = sK + STAGES * TILE;
+  const int box = min(a.at.page, KT), boxes = KT / box;
 
-  uint32_t qf[HD / 16][4];
-  {
+  float o[HD / 16][NB][4], m_run[NB][2], l_run[NB][2];
+  if (warp == 4) {
+    auto look_up = [&](int i) {
+      if (i >= n || lane >= boxes) return -1;
+      const int j = w.tile(share_tile(i, part, parts, ct)) * KT + lane * box;
+      return j < w.end ? paged_page(a.at, b, j >> a.at.shift) : -1;
+    };
+    int page = look_up(0), got = 0;
+    bool good = true;
+    for (int i = 0; i < n; i++) {
+      const int next = look_up(i + 1), st = i % STAGES;
+      const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+      const int j = w.tile(share_tile(i, part, parts, ct)) * KT + lane * box;
+      const int row = page < 0 ? 0 : (int)((page * (int64_t)a.Hkv + hk) * a.at.page) + (j & (a.at.page - 1));
+      if (i >= STAGES) good = tc::mbar_wait(smem_u32(&empty[st]), (uint32_t)((i / STAGES) & 1) ^ 1);
+      if (!__all_sync(0xffffffffu, good)) {
+        if (lane == 0) tc::set_status(status, 47);
+        break;
+      }
+      if (lane == 0) {
+        page_bits[st] = there;
+        tc::mbar_expect_tx(smem_u32(&full[st]), (uint32_t)(__popc(there) * box * 2 * 2 * HD));
+      }
+      __syncwarp();
+      if (page >= 0)
+#pragma unroll
+        for (int x = 0; x < HD / 64; x++) {
+          tc::tma_load_2d(sK + st * TILE + x * ATOM + lane * box * 128, &map_k, x * 64, row, smem_u32(&full[st]));
+          tc::tma_load_2d(sV + st * TILE + x * ATOM + lane * box * 128, &map_v, x * 64, row, smem_u32(&full[st]));
+        }
+      page = next;
+      got = i + 1;
+    }
+    // copies in flight have landed before this block's memory is somebody else's; only needed where a wait gave up
+    for (int i = max(0, got - STAGES); i < got; i++) tc::mbar_wait(smem_u32(&full[i % STAGES]), (uint32_t)((i / STAGES) & 1));
+    __syncwarp();
+  } else {
+    // queries as columns: head 8 nb + g, dims 16 ks + 2 tig ..
+    uint32_t qf[HD / 16][NB][2];
     const bf16* q0 = a.q + (t0 * a.Hq + hk * G) * HD;
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ks++) {
-      const int d0 = ks * 16 + 2 * tig;
-      qf[ks][0] = g < G ? *(const uint32_t*)(q0 + g * HD + d0) : 0u;
-      qf[ks][1] = g + 8 < G ? *(const uint32_t*)(q0 + (g + 8) * HD + d0) : 0u;
-      qf[ks][2] = g < G ? *(const uint32_t*)(q0 + g * HD + d0 + 8) : 0u;
-      qf[ks][3] = g + 8 < G ? *(const uint32_t*)(q0 + (g + 8) * HD + d0 + 8) : 0u;
-    }
-  }
-  float o[HD / 8][4];
+    for (int ks = 0; ks < HD / 16; ks++)
 #pragma unroll
-  for (int j = 0; j < HD / 8; j++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[j][i] = 0.f;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-
-  const float scale_log2 = a.scale * LOG2E;
-  auto seen = [&](int j) { return j < w.end && (j >= lo || j < a.first); };
-
-  for (int c0 = part * ct; c0 < w.total; c0 += parts * ct) {
-    const int n = min(ct, w.total - c0);
-    for (int i = threadIdx.x; i < n * gp; i += 128) page_s[i] = paged_page(a.at, b, (w.tile(c0 + i / gp) * KT + ((i % gp) << gshift)) >> a.at.shift);
-    __syncthreads();
-    auto load = [&](int t) {
-      const int j0 = w.tile(c0 + t) * KT;
-      constexpr int CH = HD / 8, RS = 128 / CH;  // 16-byte chunks of a row; rows that the block fetches at a time
-      const int cc = threadIdx.x % CH, r0 = threadIdx.x / CH;
-      const uint32_t st = (uint32_t)((t % STAGES) * KT * 2 * HD);
-#pragma unroll
-      for (int i = 0; i < KT / RS; i++) {
-        const int r = r0 + i * RS, p = page_s[t * gp + (r >> gshift)];
-        const bool ok = p >= 0 && seen(j0 + r);
-        const int64_t at = ok ? ((p * (int64_t)a.Hkv + hk) * a.at.page + ((j0 + r) & (a.at.page - 1))) * HD + cc * 8 : 0;
-        cp_async16(sK + st + tile_off<HD>(r, cc), a.k + at, ok);
-        cp_async16(sV + st + tile_off<HD>(r, cc), a.v + at, ok);
+      for (int nb = 0; nb < NB; nb++) {
+        const bf16* q = q0 + (8 * nb + g) * HD + ks * 16 + 2 * tig;
+        qf[ks][nb][0] = 8 * nb + g < G ? *(const uint32_t*)q : 0u;
+        qf[ks][nb][1] = 8 * nb + g < G ? *(const uint32_t*)(q + 8) : 0u;
       }
-    };
-    load(0);
-    cp_async_commit();
-    for (int t = 0; t < n; t++) {
-      if (t + 1 < n) load(t + 1);
-      cp_async_commit();
-      cp_async_wait<1>();
-      __syncthreads();
-      const uint32_t tK = sK + (t % STAGES) * KT * 2 * HD, tV = sV + (t % STAGES) * KT * 2 * HD;
-      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+      for (int j = 0; j < HD / 16; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[j][nb][i] = 0.f;
+      m_run[nb][0] = m_run[nb][1] = -INFINITY;
+      l_run[nb][0] = l_run[nb][1] = 0.f;
+    }
+    const float scale_log2 = a.scale * LOG2E;
+    const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
+    bool ok = true;
+    for (int i = 0; i < n; i++) {
+      const int st = i % STAGES, j0 = w.tile(share_tile(i, part, parts, ct)) * KT + warp * 16;
+      ok = ok && tc::mbar_wait(smem_u32(&full[st]), (uint32_t)((i / STAGES) & 1));
+      __syncwarp();
+      const uint32_t tK = sK + st * TILE + warp * 16 * 128, tV = sV + st * TILE + warp * 16 * 128;
+      const bool there = page_bits[st] >> (warp * 16 / box) & 1;
+      const bool whole = there && j0 + 16 <= w.end && (j0 >= lo || j0 + 16 <= a.first);
+      // scores: keys g and g + 8, heads 2 tig and 2 tig + 1
+      float s[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[nb][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++) {
-        uint32_t kb[4];
-        ldsm_x4(tK + tile_off<HD>(warp * 16 + (mi >> 1) * 8 + r8, 2 * ks + (mi & 1)), kb);
-        mma_bf16(s[0], qf[ks], kb[0], kb[1]);
-        mma_bf16(s[1], qf[ks], kb[2], kb[3]);
+        uint32_t kf[4];
+        ldsm_x4(tK + (ks >> 2) * ATOM + ((mi & 1) * 8 + r8) * 128 + ((((ks & 3) * 2 + (mi >> 1)) << 4) ^ sw), kf);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) mma_bf16(s[nb], kf, qf[ks][nb][0], qf[ks][nb][1]);
       }
-      const int r0 = warp * 16 + 2 * tig, j0 = w.tile(c0 + t) * KT;
-      float mx[2] = {-INFINITY, -INFINITY};
+      if (!whole) {
+        auto seen = [&](int r) { return there && j0 + r < w.end && (j0 + r >= lo || j0 + r < a.first); };
+        const bool s0 = seen(g), s1 = seen(g + 8);
 #pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int r = r0 + 8 * j + (i & 1);
-          const float v = seen(j0 + r) && page_s[t * gp + (r >> gshift)] >= 0 ? s[j][i] * scale_log2 : -INFINITY;
-          s[j][i] = v;
-          mx[i >> 1] = fmaxf(mx[i >> 1], v);
+        for (int nb = 0; nb < NB; nb++) {
+          if (!s0) s[nb][0] = s[nb][1] = -INFINITY;
+          if (!s1) s[nb][2] = s[nb][3] = -INFINITY;
         }
-      float corr[2], m_use[2];
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        const float m_new = fmaxf(m_run[r], mx[r]);
-        m_use[r] = m_new == -INFINITY ? 0.f : m_new;
-        corr[r] = exp2f(m_run[r] - m_use[r]);
-        m_run[r] = m_new;
-      }
-      uint32_t pf[4], pl[4];
-      {
-        float p[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          p[j][0] = exp2f(s[j][0] - m_use[0]); p[j][1] = exp2f(s[j][1] - m_use[0]);
-          p[j][2] = exp2f(s[j][2] - m_use[1]); p[j][3] = exp2f(s[j][3] - m_use[1]);
+        for (int x = lane; x < 16 * (HD / 8); x += 32) {
+          const int r = x / (HD / 8), c = x % (HD / 8);
+          if (!seen(r)) *(uint4*)(smem + (tV - sK) + (c >> 3) * ATOM + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
-        l_run[0] = l_run[0] * corr[0] + (p[0][0] + p[0][1] + p[1][0] + p[1][1]);
-        l_run[1] = l_run[1] * corr[1] + (p[0][2] + p[0][3] + p[1][2] + p[1][3]);
-        split_bf16(p[0][0], p[0][1], pf[0], pl[0]); split_bf16(p[0][2], p[0][3], pf[1], pl[1]);
-        split_bf16(p[1][0], p[1][1], pf[2], pl[2]); split_bf16(p[1][2], p[1][3], pf[3], pl[3]);
+        __syncwarp();
+      }
+      uint32_t pf[NB][2], pl[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) {
+        float mx[2] = {fmaxf(s[nb][0], s[nb][2]), fmaxf(s[nb][1], s[nb][3])}, corr[2], base[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
+          const float m_new = fmaxf(m_run[nb][h], mx[h] * scale_log2);
+          base[h] = m_new == -INFINITY ? 0.f : -m_new;
+          corr[h] = tc::ex2_approx(m_run[nb][h] + base[h]);
+          m_run[nb][h] = m_new;
+        }
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) p[e] = tc::ex2_approx(fmaf(s[nb][e], scale_log2, base[e & 1]));
+        l_run[nb][0] = l_run[nb][0] * corr[0] + (p[0] + p[2]);
+        l_run[nb][1] = l_run[nb][1] * corr[1] + (p[1] + p[3]);
+        split_bf16(p[0], p[1], pf[nb][0], pl[nb][0]);
+        split_bf16(p[2], p[3], pf[nb][1], pl[nb][1]);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          pf[nb][x] = transposed(pf[nb][x]);
+          pl[nb][x] = transposed(pl[nb][x]);
+        }
+        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+          for (int j = 0; j < HD / 16; j++) {
+            o[j][nb][0] *= corr[0]; o[j][nb][1] *= corr[1];
+            o[j][nb][2] *= corr[0]; o[j][nb][3] *= corr[1];
+          }
+        }
       }
 #pragma unroll
-      for (int j = 0; j < HD / 8; j++) {
-        o[j][0] *= corr[0]; o[j][1] *= corr[0];
-        o[j][2] *= corr[1]; o[j][3] *= corr[1];
-      }
+      for (int j = 0; j < HD / 16; j++) {
+        uint32_t vf[4];  // dims 16 j .. as rows, keys as columns
+        ldsm_x4_t(tV + (j >> 2) * ATOM + ((mi >> 1) * 8 + r8) * 128 + ((((j & 3) * 2 + (mi & 1)) << 4) ^ sw), vf);
 #pragma unroll
-      for (int jj = 0; jj < HD / 16; jj++) {
-        uint32_t vb[4];
-        ldsm_x4_t(tV + tile_off<HD>(warp * 16 + (mi & 1) * 8 + r8, 2 * jj + (mi >> 1)), vb);
-        mma_bf16(o[2 * jj], pf, vb[0], vb[1]);
-        mma_bf16(o[2 * jj + 1], pf, vb[2], vb[3]);
-        mma_bf16(o[2 * jj], pl, vb[0], vb[1]);
-        mma_bf16(o[2 * jj + 1], pl, vb[2], vb[3]);
+        for (int nb = 0; nb < NB; nb++) {
+          mma_bf16(o[j][nb], vf, pf[nb][0], pf[nb][1]);
+          mma_bf16(o[j][nb], vf, pl[nb][0], pl[nb][1]);
+        }
       }
-      __syncthreads();
+      if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros stay in front of the next copy into this place
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[st])) : "memory");
     }
-    cp_async_wait<0>();
+    if (!__all_sync(0xffffffffu, ok) && lane == 0) tc::set_status(status, 48);
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l_run[nb][h] += __shfl_xor_sync(0xffffffffu, l_run[nb][h], x);
   }
+  __syncthreads();  // every copy has been waited for, and nobody reads a tile any more
+  // the four warps joined through shared memory
+  constexpr int LD = HD + 4;
+  float* so = (float*)smem;                    // [4 warps][16 heads][LD]
+  float* jo = so + 4 * 16 * LD;                // [G][HD] joined
+  float2* sml = (float2*)(jo + 16 * HD);       // [4 warps][16 heads]
+  float2* jml = sml + 4 * 16;                  // [G]
+  if (warp < 4) {
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-  }
-  // the four warps joined through shared memory (the tiles are free after the last barrier)
-  float* so = (float*)smem;                    // [4 warps][16 rows][HD]
-  float2* sml = (float2*)(so + 4 * 16 * HD);   // [4 warps][16 rows]
-  float* jo = (float*)(sml + 4 * 16);          // [G][HD] joined
-  float2* jml = (float2*)(jo + 16 * HD);       // [G]
+    for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    const int row = g + 8 * r;
-    if (row < G) {
+      for (int h = 0; h < 2; h++) {
+        const int head = 8 * nb + 2 * tig + h;
+        if (head < G) {
 #pragma unroll
-      for (int j = 0; j < HD / 8; j++) *(float2*)(so + (warp * 16 + row) * HD + 8 * j + 2 * tig) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-      if (tig == 0) sml[warp * 16 + row] = make_float2(m_run[r], l_run[r]);
-    }
+          for (int j = 0; j < HD / 16; j++) {
+            so[(warp * 16 + head) * LD + 16 * j + g] = o[j][nb][h];
+            so[(warp * 16 + head) * LD + 16 * j + g + 8] = o[j][nb][2 + h];
+          }
+          if (g == 0) sml[warp * 16 + head] = make_float2(m_run[nb][h], l_run[nb][h]);
+        }
+      }
   }
   __syncthreads();
   bf16* out = a.out + (t0 * a.Hq + hk * G) * HD;
-  for (int e = threadIdx.x; e < G * (HD / 4); e += 128) {
+  for (int e = threadIdx.x; e < G * (HD / 4); e += DEC_THREADS) {
     const int row = e / (HD / 4), d = e % (HD / 4) * 4;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -184,7 +258,7 @@ __global__ void __launch_bounds__(128) attn_paged_decode_kernel(PagedAttnArgs a,
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const float f = weight_of(sml[i * 16 + row].x, M);
-      const float4 p = *(const float4*)(so + (i * 16 + row) * HD + d);
+      const float4 p = *(const float4*)(so + (i * 16 + row) * LD + d);
       L += sml[i * 16 + row].y * f;
       O.x += p.x * f; O.y += p.y * f; O.z += p.z * f; O.w += p.w * f;
     }
@@ -208,7 +282,7 @@ __global__ void __launch_bounds__(128) attn_paged_decode_kernel(PagedAttnArgs a,
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"(local), "r"(rank));
       return x;
     };
-    for (int e = part * 128 + threadIdx.x; e < G * (HD / 4); e += parts * 128) {
+    for (int e = part * DEC_THREADS + threadIdx.x; e < G * (HD / 4); e += parts * DEC_THREADS) {
       const int row = e / (HD / 4), d = e % (HD / 4) * 4;
       float2 ml[CLUSTER_MAX];
       float4 p[CLUSTER_MAX];
@@ -272,13 +346,12 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, P
   for (int e = 0; e < E; e += 2) *(uint32_t*)(a.out + at * HD + lane * E + e) = pack_bf16(O[e] * inv, O[e + 1] * inv);
 }
 
-template <int HD>
+template <int HD, int NB>
 int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  const size_t tiles_bytes = (size_t)2 * STAGES * KT * 2 * HD, join_bytes = (size_t)(5 * 16 * HD) * 4 + 5 * 16 * 8;
-  const size_t smem = std::max(tiles_bytes, join_bytes);
+  constexpr size_t smem = dec_smem(HD);
   static SbDeviceOnce once;
   SB_CUDA(once.run(ctx->device, [&] {
-    for (auto f : {attn_paged_decode_kernel<HD, JOIN_NONE>, attn_paged_decode_kernel<HD, JOIN_SCRATCH>, attn_paged_decode_kernel<HD, JOIN_CLUSTER>}) {
+    for (auto f : {attn_paged_decode_kernel<HD, NB, JOIN_NONE>, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>}) {
       cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       if (e != cudaSuccess) return e;
     }
@@ -301,14 +374,18 @@ int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   }
   parts = std::min<int64_t>(parts, 256);
   if (parts <= 1) join = JOIN_NONE, parts = 1;
-  const int ct = (int)std::min<int64_t>(CT, (tiles + parts - 1) / parts);
+  const int ct = (int)((tiles + parts - 1) / parts);
   const dim3 grid((unsigned)parts, (unsigned)a.Hkv, (unsigned)a.at.B);
-  PagedJoin buf{};
-  buf.parts = (int)parts;
+  PagedJoin buf;
   if (join == JOIN_SCRATCH) SB_TRY(paged_join_scratch(ctx, a, (int)parts, &buf));
-  if (join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, JOIN_NONE>, grid, dim3(128), smem, a, buf, ct));
-  else if (join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, JOIN_SCRATCH>, grid, dim3(128), smem, a, buf, ct));
-  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_decode_kernel<HD, JOIN_CLUSTER>, grid, dim3(128), smem, dim3((unsigned)parts), a, buf, ct));
+  CUtensorMap mk, mv;
+  const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
+  SB_TRY(paged_map_rows(&mk, a.k, rows, HD, std::min(a.at.page, KT)));
+  SB_TRY(paged_map_rows(&mv, a.v, rows, HD, std::min(a.at.page, KT)));
+  const dim3 block(DEC_THREADS);
+  if (join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, ctx->d_status));
+  else if (join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, ctx->d_status));
+  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, ctx->d_status));
   ctx->launches++;
   return join == JOIN_SCRATCH ? paged_join(ctx, a, buf) : STRICTB200_OK;
 }
@@ -338,5 +415,6 @@ int64_t paged_walk_tiles(const PagedAttnArgs& a, int kt) {
 
 int k_attn_paged(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   if (a.max_new > 1 || a.Hq / a.Hkv > 16 || a.at.B > 65535) return k_attn_paged_tiles(ctx, a);
-  return a.D == 128 ? decode<128>(ctx, a) : decode<64>(ctx, a);
+  if (a.Hq / a.Hkv > 8) return a.D == 128 ? decode<128, 2>(ctx, a) : decode<64, 2>(ctx, a);
+  return a.D == 128 ? decode<128, 1>(ctx, a) : decode<64, 1>(ctx, a);
 }

@@ -1,6 +1,7 @@
 // What the kernels of the attention over a paged cache share: the join of their parts.
 #pragma once
 #include "paged.cuh"
+#include "tcgen05.cuh"
 
 // Unnormalised outputs of rows whose keys were split, [T, Hq, parts]; an output is read only where its sum is not zero.
 struct PagedJoin {
@@ -12,3 +13,28 @@ int paged_join_scratch(strictb200_ctx*, const PagedAttnArgs& a, int parts, Paged
 int paged_join(strictb200_ctx*, const PagedAttnArgs& a, const PagedJoin& join);
 int64_t paged_walk_tiles(const PagedAttnArgs& a, int kt);  // tiles of kt keys that the rows of a sequence of max_len tokens walk over
 int k_attn_paged_tiles(strictb200_ctx*, const PagedAttnArgs& a);  // attention_paged_tc.cu
+
+#ifdef __CUDACC__
+// i-th key tile of a block whose share is every parts-th piece of ct tiles
+__device__ __forceinline__ int share_tile(int i, int part, int parts, int ct) { return parts == 1 ? i : (i / ct * parts + part) * ct + i % ct; }
+__device__ __forceinline__ int share_count(int total, int part, int parts, int ct) {
+  if (parts == 1) return total;
+  const int rounds = total / (parts * ct), rest = total - rounds * parts * ct;
+  return rounds * ct + min(max(rest - part * ct, 0), ct);
+}
+
+
+// Tensor map of rows of `cols` bf16, boxes of `box` rows x 64 columns, 128-byte swizzle
+inline int paged_map_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box) {
+  tc::EncodeFn encode;
+  SB_TRY(tc::encode_fn(&encode));
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  cuuint32_t boxes[2] = {64u, (cuuint32_t)box};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return sb_fail(STRICTB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return STRICTB200_OK;
+}
+#endif

@@ -21,7 +21,6 @@
 #include <algorithm>
 
 #include "attention_paged.cuh"
-#include "tcgen05.cuh"
 
 using namespace tc;
 
@@ -50,14 +49,6 @@ struct Work {
   PagedWalk w;
   int nt;                // key tiles of this block
 };
-
-// i-th key tile of a block whose share is every parts-th piece of ct tiles
-__device__ __forceinline__ int share_tile(int i, int part, int parts, int ct) { return parts == 1 ? i : (i / ct * parts + part) * ct + i % ct; }
-__device__ __forceinline__ int share_count(int total, int part, int parts, int ct) {
-  if (parts == 1) return total;
-  const int rounds = total / (parts * ct), rest = total - rounds * parts * ct;
-  return rounds * ct + min(max(rest - part * ct, 0), ct);
-}
 
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
@@ -511,19 +502,6 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   }
 }
 
-// rows of `cols` bf16, boxes of `box` rows x 64 columns, 128-byte swizzle
-int map_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box) {
-  EncodeFn encode;
-  SB_TRY(encode_fn(&encode));
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t boxes[2] = {64u, (cuuint32_t)box};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return sb_fail(STRICTB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
-  return STRICTB200_OK;
-}
 // [T, heads, cols], boxes of `tokens` x G heads x 64 columns
 int map_tokens(CUtensorMap* map, const void* base, int64_t T, int heads, int cols, int G, int tokens) {
   EncodeFn encode;
@@ -564,8 +542,8 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   CUtensorMap mq, mk, mv;
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(map_tokens(&mq, a.q, a.at.T, a.Hq, a.D, t.G, t.tw));
-  SB_TRY(map_rows(&mk, a.k, rows, a.D, std::min(a.at.page, BKV)));
-  SB_TRY(map_rows(&mv, a.v, rows, a.D, std::min(a.at.page, BKV)));
+  SB_TRY(paged_map_rows(&mk, a.k, rows, a.D, std::min(a.at.page, BKV)));
+  SB_TRY(paged_map_rows(&mv, a.v, rows, a.D, std::min(a.at.page, BKV)));
   constexpr size_t smem = tiles_smem<QA, ONE>();
   static SbDeviceOnce once;  // one per instantiation
   SB_CUDA(once.run(ctx->device, [&] { return cudaFuncSetAttribute(attn_paged_tiles_kernel<QA, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
@@ -577,7 +555,6 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
 }  // namespace
 
 int k_attn_paged_tiles(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  if ((int64_t)a.at.n_pages * a.Hkv * a.at.page > INT32_MAX) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "attention: more than 2^31 - 1 rows of keys");
   const bool one = (int64_t)a.max_new * (a.Hq / a.Hkv) <= BQ;  // one tile per sequence
   if (a.D == 128) return one ? launch<2, true>(ctx, a) : launch<2, false>(ctx, a);
   return one ? launch<1, true>(ctx, a) : launch<1, false>(ctx, a);

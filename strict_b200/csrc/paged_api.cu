@@ -25,10 +25,12 @@ int paged_view(PagedView* v, const int32_t* table, const int32_t* lens, const in
   *v = PagedView{table, lens, starts, B, table_ld, n_pages, page, shift, T};
   return STRICTB200_OK;
 }
-int paged_heads(int Hq, int Hkv, int D, int n_pages) {
+int paged_heads(int Hq, int Hkv, int D, int n_pages, int page) {
   if (D != 64 && D != 128) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
   SB_REQUIRE(Hq > 0 && Hkv > 0, "bad shape: no heads");
-  if (Hq > 65535 || (int64_t)n_pages * Hkv > INT32_MAX) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "more than 65535 heads, or than 2^31 - 1 pages of all heads");
+  // positions of all pages and heads are rows of one matrix, with 32-bit coordinates
+  if (Hq > 65535 || Hkv > 65535 || (int64_t)n_pages * Hkv * page > INT32_MAX)
+    return sb_fail(STRICTB200_ERR_UNSUPPORTED, "more than 65535 heads, or than 2^31 - 1 positions of all pages and heads");
   return STRICTB200_OK;
 }
 
@@ -41,7 +43,7 @@ int strictb200_attn_paged(strictb200_ctx* ctx, const uint16_t* q, const uint16_t
                           int window, int first, float scale, uint16_t* out) {
   PAGED_CONTEXT(ctx);
   PagedAttnArgs a;
-  SB_TRY(paged_heads(Hq, Hkv, D, n_pages > 0 ? n_pages : 0));
+  SB_TRY(paged_heads(Hq, Hkv, D, n_pages, page));
   SB_REQUIRE(Hq % Hkv == 0, "Hq must be a multiple of Hkv");
   if (Hq / Hkv > 128) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "at most 128 query heads per key/value head");
   SB_REQUIRE(max_new >= 0 && max_len >= 0 && window >= 0 && first >= 0, "max_new, max_len, window and first must not be negative");
@@ -61,7 +63,7 @@ int strictb200_rope_qknorm_paged(strictb200_ctx* ctx, const uint16_t* qkv, const
                                  uint16_t* q_out, uint16_t* kpages, uint16_t* vpages) {
   PAGED_CONTEXT(ctx);
   PagedRopeArgs a;
-  SB_TRY(paged_heads(Hq, Hkv, D, n_pages > 0 ? n_pages : 0));
+  SB_TRY(paged_heads(Hq, Hkv, D, n_pages, page));
   SB_REQUIRE(theta > 0.f && std::isfinite(theta) && eps >= 0.f, "theta must be positive and finite, eps not negative");
   SB_TRY(paged_view(&a.at, table, lens, starts, B, T, n_pages, page, table_ld));
   if (!B || !T) return STRICTB200_OK;

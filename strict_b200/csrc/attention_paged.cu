@@ -2,6 +2,7 @@
 //
 // One new token per sequence and at most 16 query heads per key/value head: the kernel here. Otherwise attention_paged_tc.cu.
 #include <algorithm>
+#include <cmath>
 
 #include "mma_tiles.cuh"
 #include "attention_paged.cuh"
@@ -14,8 +15,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ one new token per sequence
 // Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its tiles of 64 keys. Warp 4 copies:
-// its lanes look up a page each, one tile ahead, and request the tile by TMA (boxes of min(page, 64) keys x 64 dims, 128-byte swizzle) into a ring
-// of STAGES. Warp w < 4 owns keys 16 w .. 16 w + 15 of every tile, with a softmax of its own; the four are joined at the end.
+// its lanes look the pages up, well ahead, and request the tile by TMA (boxes of min(page, 64) keys x 64 dims, 128-byte swizzle) into a ring
+// of `stages`. Warp w < 4 owns keys 16 w .. 16 w + 15 of every tile, with a softmax of its own; the four are joined at the end.
 // Products are mma.sync m16n8k16 with keys (then dims) as the 16 rows and query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T: at most eight heads
 // waste nothing that way. (With the heads as rows, half of everything was idle: 874 instructions per warp and tile, 166 registers and 5.3 TB/s.)
 // Positions that the row does not see, or whose entry names no page, are not fetched or hidden by index: their scores become -inf and the warp that
@@ -24,7 +25,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Shares: piece c of ct tiles belongs to block c % gridDim.x, however long the sequence turns out to be. JOIN: 0 there is one block, 1 the
 // blocks leave (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel, 2 they are one cluster and join through distributed shared memory.
 constexpr int KT = 64;
-constexpr int STAGES = 2;
+constexpr int MAX_STAGES = 6;
 constexpr int DEC_THREADS = 160;
 enum { JOIN_NONE = 0, JOIN_SCRATCH = 1, JOIN_CLUSTER = 2 };
 constexpr int CLUSTER_MAX = 8;
@@ -37,25 +38,25 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 
 constexpr size_t dec_tile_bytes(int HD) { return (size_t)KT * 2 * HD; }
-constexpr size_t dec_smem(int HD) {
-  const size_t ring = 2 * STAGES * dec_tile_bytes(HD), join = (size_t)(4 * 16 * (HD + 4) + 16 * HD) * 4 + 5 * 16 * 8;
+constexpr size_t dec_smem(int HD, int stages) {
+  const size_t ring = 2 * stages * dec_tile_bytes(HD), join = (size_t)(4 * 16 * (HD + 4) + 16 * HD) * 4 + 5 * 16 * 8;
   return (ring > join ? ring : join) + 1024;
 }
 
 // NB: blocks of eight query heads
 template <int HD, int NB, int JOIN>
 __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                        const __grid_constant__ PagedAttnArgs a, PagedJoin join, int ct, int* status) {
+                                                                        const __grid_constant__ PagedAttnArgs a, PagedJoin join, int ct, int stages, int* status) {
   constexpr int ATOM = KT * 128, TILE = ATOM * (HD / 64);  // bytes of 64 keys x 64 dims, and of a tile
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
-  __shared__ uint32_t page_bits[STAGES];
+  __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  __shared__ uint32_t page_bits[MAX_STAGES];
   const int part = blockIdx.x, parts = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = a.Hq / a.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3, mi = lane >> 3, r8 = lane & 7;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; i++) {
+    for (int i = 0; i < stages; i++) {
       tc::mbar_init(smem_u32(&full[i]), 1);
       tc::mbar_init(smem_u32(&empty[i]), 4);
     }
@@ -64,6 +65,7 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
   __syncthreads();
   pdl_wait();
   pdl_trigger();
+  const int box = min(a.at.page, KT), boxes = KT / box;
   const int64_t t0 = a.at.starts[b];
   const int last = a.at.starts[b + 1], len = a.at.lens[b];
   if (t0 < 0 || t0 >= a.at.T || last <= t0) return;  // the same for every block of a cluster
@@ -71,24 +73,26 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
   const PagedWalk w = paged_walk(a.at, len, pos, pos, a.window, a.first, KT);
   const int lo = a.window ? max(0, pos - a.window + 1) : 0;
   const int n = share_count(w.total, part, parts, ct);
-  const uint32_t sK = smem_u32(smem), sV = sK + STAGES * TILE;
-  const int box = min(a.at.page, KT), boxes = KT / box;
+  const uint32_t sK = smem_u32(smem), sV = sK + stages * TILE;
 
   float o[HD / 16][NB][4], m_run[NB][2], l_run[NB][2];
   if (warp == 4) {
-    auto look_up = [&](int i) {
-      if (i >= n || lane >= boxes) return -1;
-      const int j = w.tile(share_tile(i, part, parts, ct)) * KT + lane * box;
+    auto page_of = [&](int i, int x) {
+      const int j = i < n ? w.tile(share_tile(i, part, parts, ct)) * KT + x * box : w.end;
       return j < w.end ? paged_page(a.at, b, j >> a.at.shift) : -1;
     };
-    int page = look_up(0), got = 0;
+    PageNames names;
+    names.begin(boxes, lane, page_of);
+    int got = 0;
     bool good = true;
+    int st = 0;
+    uint32_t ph = 1;  // of the round in front
     for (int i = 0; i < n; i++) {
-      const int next = look_up(i + 1), st = i % STAGES;
+      const int page = names.of(i, boxes, lane, page_of);
       const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
       const int j = w.tile(share_tile(i, part, parts, ct)) * KT + lane * box;
       const int row = page < 0 ? 0 : (int)((page * (int64_t)a.Hkv + hk) * a.at.page) + (j & (a.at.page - 1));
-      if (i >= STAGES) good = tc::mbar_wait(smem_u32(&empty[st]), (uint32_t)((i / STAGES) & 1) ^ 1);
+      if (i >= stages) good = tc::mbar_wait(smem_u32(&empty[st]), ph);
       if (!__all_sync(0xffffffffu, good)) {
         if (lane == 0) tc::set_status(status, 47);
         break;
@@ -104,11 +108,11 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
           tc::tma_load_2d(sK + st * TILE + x * ATOM + lane * box * 128, &map_k, x * 64, row, smem_u32(&full[st]));
           tc::tma_load_2d(sV + st * TILE + x * ATOM + lane * box * 128, &map_v, x * 64, row, smem_u32(&full[st]));
         }
-      page = next;
       got = i + 1;
+      if (++st == stages) st = 0, ph ^= 1;
     }
     // copies in flight have landed before this block's memory is somebody else's; only needed where a wait gave up
-    for (int i = max(0, got - STAGES); i < got; i++) tc::mbar_wait(smem_u32(&full[i % STAGES]), (uint32_t)((i / STAGES) & 1));
+    for (int i = max(0, got - stages); i < got; i++) tc::mbar_wait(smem_u32(&full[i % stages]), (uint32_t)((i / stages) & 1));
     __syncwarp();
   } else {
     // queries as columns: head 8 nb + g, dims 16 ks + 2 tig ..
@@ -134,26 +138,33 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
     const float scale_log2 = a.scale * LOG2E;
     const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
     bool ok = true;
+    int st = 0, step = part * ct, left = ct;  // place in the walk, tiles of the piece
+    uint32_t ph = 0;
     for (int i = 0; i < n; i++) {
-      const int st = i % STAGES, j0 = w.tile(share_tile(i, part, parts, ct)) * KT + warp * 16;
-      ok = ok && tc::mbar_wait(smem_u32(&full[st]), (uint32_t)((i / STAGES) & 1));
+      const int j0 = w.tile(step++) * KT + warp * 16;
+      if (--left == 0) left = ct, step += (parts - 1) * ct;
+      ok = ok && tc::mbar_wait(smem_u32(&full[st]), ph);
       __syncwarp();
       const uint32_t tK = sK + st * TILE + warp * 16 * 128, tV = sV + st * TILE + warp * 16 * 128;
       const bool there = page_bits[st] >> (warp * 16 / box) & 1;
       const bool whole = there && j0 + 16 <= w.end && (j0 >= lo || j0 + 16 <= a.first);
       // scores: keys g and g + 8, heads 2 tig and 2 tig + 1
-      float s[NB][4];
+      float s[NB][4], s2[NB][4];  // two sums, so that half as many products wait for one another
 #pragma unroll
       for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[nb][e] = 0.f;
+        for (int e = 0; e < 4; e++) s[nb][e] = s2[nb][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++) {
         uint32_t kf[4];
         ldsm_x4(tK + (ks >> 2) * ATOM + ((mi & 1) * 8 + r8) * 128 + ((((ks & 3) * 2 + (mi >> 1)) << 4) ^ sw), kf);
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) mma_bf16(s[nb], kf, qf[ks][nb][0], qf[ks][nb][1]);
+        for (int nb = 0; nb < NB; nb++) mma_bf16(ks & 1 ? s2[nb] : s[nb], kf, qf[ks][nb][0], qf[ks][nb][1]);
       }
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[nb][e] += s2[nb][e];
       if (!whole) {
         auto seen = [&](int r) { return there && j0 + r < w.end && (j0 + r >= lo || j0 + r < a.first); };
         const bool s0 = seen(g), s1 = seen(g + 8);
@@ -203,18 +214,23 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
         }
       }
 #pragma unroll
-      for (int j = 0; j < HD / 16; j++) {
-        uint32_t vf[4];  // dims 16 j .. as rows, keys as columns
-        ldsm_x4_t(tV + (j >> 2) * ATOM + ((mi >> 1) * 8 + r8) * 128 + ((((j & 3) * 2 + (mi & 1)) << 4) ^ sw), vf);
+      for (int j0 = 0; j0 < HD / 16; j0 += 4) {
+        uint32_t vf[4][4];  // dims 16 j .. as rows, keys as columns; four products between the two that add to one sum
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-          mma_bf16(o[j][nb], vf, pf[nb][0], pf[nb][1]);
-          mma_bf16(o[j][nb], vf, pl[nb][0], pl[nb][1]);
+        for (int j = 0; j < 4; j++) {
+          ldsm_x4_t(tV + (j0 >> 2) * ATOM + ((mi >> 1) * 8 + r8) * 128 + (((j * 2 + (mi & 1)) << 4) ^ sw), vf[j]);
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) mma_bf16(o[j0 + j][nb], vf[j], pf[nb][0], pf[nb][1]);
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) mma_bf16(o[j0 + j][nb], vf[j], pl[nb][0], pl[nb][1]);
       }
       if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros stay in front of the next copy into this place
       __syncwarp();
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[st])) : "memory");
+      if (++st == stages) st = 0, ph ^= 1;
     }
     if (!__all_sync(0xffffffffu, ok) && lane == 0) tc::set_status(status, 48);
 #pragma unroll
@@ -327,67 +343,102 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, P
   const int64_t t = at / a.Hq;
   if (t < a.at.starts[0] || t >= a.at.starts[a.at.B]) return;
   const float2* ml = join.ml + at * join.parts;
+  const float* o = join.o + at * join.parts * HD + lane * E;
   float M = -INFINITY, L = 0.f, O[E];
   for (int i = lane; i < join.parts; i += 32) M = fmaxf(M, ml[i].x);
   M = warp_max(M);
 #pragma unroll
   for (int e = 0; e < E; e++) O[e] = 0.f;
-  for (int i = 0; i < join.parts; i++) {
-    const float2 v = ml[i];
-    if (v.y == 0.f) continue;
+  for (int i0 = 0; i0 < join.parts; i0 += 32) {  // a lane has the weight of a part; the outputs of eight parts are requested together
+    const float2 v = i0 + lane < join.parts ? ml[i0 + lane] : make_float2(-INFINITY, 0.f);
     const float f = weight_of(v.x, M);
     L += v.y * f;
-    const float* o = join.o + (at * join.parts + i) * HD + lane * E;
+    const unsigned there = __ballot_sync(0xffffffffu, v.y != 0.f);
+    for (int i = 0; i < min(32, join.parts - i0); i += 8) {
+      float x[8][E];
 #pragma unroll
-    for (int e = 0; e < E; e++) O[e] += o[e] * f;
+      for (int n = 0; n < 8; n++)
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 y = there >> (i + n) & 1 ? *(const float2*)(o + (int64_t)(i0 + i + n) * HD + e) : make_float2(0.f, 0.f);
+          x[n][e] = y.x;
+          x[n][e + 1] = y.y;
+        }
+#pragma unroll
+      for (int n = 0; n < 8; n++) {
+        const float fn = __shfl_sync(0xffffffffu, f, i + n);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (there >> (i + n) & 1) O[e] += x[n][e] * fn;
+      }
+    }
   }
+  L = warp_sum(L);
   const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
   for (int e = 0; e < E; e += 2) *(uint32_t*)(a.out + at * HD + lane * E + e) = pack_bf16(O[e] * inv, O[e + 1] * inv);
 }
 
+struct DecodePlan {
+  int parts = 1, stages = 2, join = JOIN_NONE;
+};
+// How a decode step is cut, from its sizes, by a model in microseconds: a block starts after 3 and has a tile every 1.3 / stages at best (the latency of a copy) and
+// every `chain` (its products and its softmax one after the other); an SM takes 46 GB/s; blocks beyond those that fit run in further rounds, with half a round of unevenness; the join in a cluster takes 1.5, the one through scratch 4 and its bytes.
+// Ring: what shared memory leaves the blocks that share an SM. Clusters need all their blocks at once: one wave only, counted with 7/8 of the SMs, and
+// with shared memory for two blocks on each, or those that find no eight empty SMs wait for a second wave.
+DecodePlan plan_decode(const strictb200_ctx* ctx, int HD, int64_t units, int64_t tiles, int64_t out_floats) {
+  const double stage = 2.0 * dec_tile_bytes(HD), tile_us = stage / 46e3, sms = ctx->sm_count;
+  const double chain = HD == 128 ? 0.8 : 0.6;
+  const int fit = HD == 128 ? 3 : 5;  // blocks per SM with two stages: shared memory (128 dims), registers (64 dims)
+  DecodePlan best;
+  double best_us = 1e30;
+  for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 128); parts += parts < 16 ? 1 : parts / 8) {
+    const double ct = (double)((tiles + parts - 1) / parts), blocks = (double)(units * parts);
+    const int resident = (int)std::min<double>(fit, std::ceil(blocks / sms));
+    DecodePlan p;
+    p.parts = (int)parts;
+    const bool one_wave = blocks <= (parts > 1 ? 0.875 : 1) * fit * sms;
+    const int share = one_wave && parts > 1 && parts <= CLUSTER_MAX ? std::max(2, resident) : resident;
+    p.stages = std::max(2, std::min<int>({MAX_STAGES, (int)ct, (int)((double)(220 << 10) / share / stage - 0.1)}));
+    double us = 3 + ct * std::max({tile_us * resident, chain, 1.3 / p.stages});
+    if (!one_wave) us = 3 + ct * tile_us * fit * (blocks / (fit * sms) + 0.5);
+    if (parts > 1) {
+      p.join = one_wave && parts <= CLUSTER_MAX ? JOIN_CLUSTER : JOIN_SCRATCH;
+      us += p.join == JOIN_CLUSTER ? 1.5 : 4 + out_floats * parts * 8 / 6e6;
+    }
+    if (us < best_us * 0.99) best_us = us, best = p;
+    if (parts > 1 && out_floats * (parts + 1) * 4 > (double)(512 << 20)) break;  // scratch
+  }
+  return best;
+}
+
 template <int HD, int NB>
 int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  constexpr size_t smem = dec_smem(HD);
   static SbDeviceOnce once;
   SB_CUDA(once.run(ctx->device, [&] {
     for (auto f : {attn_paged_decode_kernel<HD, NB, JOIN_NONE>, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>}) {
-      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec_smem(HD, MAX_STAGES));
       if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
   }));
-  const int64_t tiles = std::max<int64_t>(1, paged_walk_tiles(a, KT)), units = (int64_t)a.at.B * a.Hkv, slots = (int64_t)ctx->sm_count * 3;
-  // One wave: as many parts as there are places, in a cluster of at most eight where that leaves a block few tiles. Several waves: pieces of at least
-  // eight tiles, four waves of them if the sequences are as long as they may be, so that uneven lengths even out.
-  int64_t parts = std::min(tiles, slots / units);
-  int join = JOIN_CLUSTER;
-  if (units * 2 > slots) {
-    parts = std::max<int64_t>(1, std::min(tiles / 8, (4 * slots + units - 1) / units));
-    join = JOIN_SCRATCH;
-  } else if (parts > CLUSTER_MAX) {
-    if (tiles <= CLUSTER_MAX * 4) parts = CLUSTER_MAX;
-    else {
-      parts = std::min<int64_t>(parts, (tiles + 1) / 2);
-      join = JOIN_SCRATCH;
-    }
-  }
-  parts = std::min<int64_t>(parts, 256);
-  if (parts <= 1) join = JOIN_NONE, parts = 1;
-  const int ct = (int)((tiles + parts - 1) / parts);
+  const int64_t tiles = std::max<int64_t>(1, paged_walk_tiles(a, KT));
+  const DecodePlan plan = plan_decode(ctx, HD, (int64_t)a.at.B * a.Hkv, tiles, (double)a.at.T * a.Hq * HD);
+  const int parts = plan.parts, ct = (int)((tiles + parts - 1) / parts), stages = plan.stages;
+  const size_t smem = dec_smem(HD, stages);
   const dim3 grid((unsigned)parts, (unsigned)a.Hkv, (unsigned)a.at.B);
   PagedJoin buf;
-  if (join == JOIN_SCRATCH) SB_TRY(paged_join_scratch(ctx, a, (int)parts, &buf));
+  if (plan.join == JOIN_SCRATCH) SB_TRY(paged_join_scratch(ctx, a, parts, &buf));
   CUtensorMap mk, mv;
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(paged_map_rows(&mk, a.k, rows, HD, std::min(a.at.page, KT)));
   SB_TRY(paged_map_rows(&mv, a.v, rows, HD, std::min(a.at.page, KT)));
   const dim3 block(DEC_THREADS);
-  if (join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, ctx->d_status));
-  else if (join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, ctx->d_status));
-  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, ctx->d_status));
+  if (plan.join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
+  else if (plan.join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
+  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, stages, ctx->d_status));
   ctx->launches++;
-  return join == JOIN_SCRATCH ? paged_join(ctx, a, buf) : STRICTB200_OK;
+  return plan.join == JOIN_SCRATCH ? paged_join(ctx, a, buf) : STRICTB200_OK;
 }
 
 }  // namespace

@@ -15,6 +15,28 @@ int64_t paged_walk_tiles(const PagedAttnArgs& a, int kt);  // tiles of kt keys t
 int k_attn_paged_tiles(strictb200_ctx*, const PagedAttnArgs& a);  // attention_paged_tc.cu
 
 #ifdef __CUDACC__
+// Page numbers of a block's key tiles, fetched by one warp for 32 boxes at a time, the next 32 while the present ones are in use (a look-up per tile
+// held a block to a tile per trip to L2). Box i of a tile is in lane i.
+struct PageNames {
+  int now, next, per;  // tiles of a fetch
+  template <typename F>
+  __device__ __forceinline__ void begin(int boxes, int lane, F&& page_of) {
+    per = 32 / boxes;
+    now = page_of(lane / boxes, lane % boxes);
+    next = page_of(per + lane / boxes, lane % boxes);
+  }
+  // of tile i, asked for in order
+  template <typename F>
+  __device__ __forceinline__ int of(int i, int boxes, int lane, F&& page_of) {
+    const int k = i % per;
+    if (i && !k) {
+      now = next;
+      next = page_of(i + per + lane / boxes, lane % boxes);
+    }
+    const int p = __shfl_sync(0xffffffffu, now, (k * boxes + lane) & 31);
+    return lane < boxes ? p : -1;
+  }
+};
 // i-th key tile of a block whose share is every parts-th piece of ct tiles
 __device__ __forceinline__ int share_tile(int i, int part, int parts, int ct) { return parts == 1 ? i : (i / ct * parts + part) * ct + i % ct; }
 __device__ __forceinline__ int share_count(int total, int part, int parts, int ct) {

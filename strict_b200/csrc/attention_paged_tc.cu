@@ -13,7 +13,7 @@
 //   one tile (ONE = true)     few rows: the even and the odd key tiles of the same queries, each with a softmax of its own; joined later
 // Keys may be split further over `parts` blocks. Whatever is split leaves (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel.
 //
-// Pages: a tile of 128 keys is 128 / page boxes (or part of a page); the lanes of the copying warp look up one page each, one tile ahead. A page that
+// Pages: a tile of 128 keys is 128 / page boxes (or part of a page); the lanes of the copying warp look the pages up, well ahead. A page that
 // the table does not name, or that begins behind the last position any row sees, is not fetched, and its keys are hidden by a bit mask.
 // What lies at hidden positions must not count: scores are replaced by index, but a weight of zero times a value that is not finite is not zero, and
 // places that were not fetched hold anything. So in tiles where some row does not see some key, two warps put zeros over values that no row sees, and over those
@@ -169,15 +169,16 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
       for (int w = 0; w < nq; w++)
         for (int i = 0; i < QA; i++) tma_load_3d(sQ + w * TILE + i * HALF_BYTES, &map_q, i * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&bar_q));
     }
-    auto look_up = [&](int i) {
-      if (i >= k.nt || lane >= boxes) return -1;
-      const int j = tile_key(i) + lane * box;
+    auto page_of = [&](int i, int x) {
+      const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
       return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
     };
-    int page = look_up(0), got = 0;
+    PageNames names;
+    names.begin(boxes, lane, page_of);
+    int got = 0;
     bool good = true;
     for (int i = 0; i < k.nt; i++) {
-      const int next = look_up(i + 1), st = i & 1;
+      const int page = names.of(i, boxes, lane, page_of), st = i & 1;
       const uint32_t ph = (uint32_t)((i >> 1) & 1) ^ 1;
       const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
       const uint32_t bytes = (uint32_t)(__popc(there) * box * 128 * QA);
@@ -197,7 +198,6 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
       __syncwarp();
       if (page >= 0)
         for (int x = 0; x < QA; x++) tma_load_2d(sV + st * TILE + x * HALF_BYTES + lane * box * 128, &map_v, x * 64, row, smem_u32(&v_full[st]));
-      page = next;
       got = i + 1;
     }
     // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up

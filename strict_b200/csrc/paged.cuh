@@ -56,7 +56,7 @@ __device__ __forceinline__ int paged_seq(const PagedView& v, int64_t t) {
 }
 // Page of slot group `n` of sequence b, or -1 where the table names none.
 __device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
-  if (n >= v.ld) return -1;
+  if ((unsigned)n >= (unsigned)v.ld) return -1;
   const int p = v.table[(int64_t)b * v.ld + n];
   return p >= 0 && p < v.n_pages ? p : -1;
 }

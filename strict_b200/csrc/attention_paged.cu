@@ -1,6 +1,6 @@
 // Softmax attention of new tokens over a paged cache, grouped heads of 64 or 128 dims, bf16.
 //
-// One new token per sequence and at most 16 query heads per key/value head: the kernel here. Otherwise attention_paged_tc.cu.
+// Few rows, where a row is one query head of one new token: at most 32 per sequence and key/value head. More: attention_paged_tc.cu.
 #include <algorithm>
 #include <cmath>
 
@@ -13,20 +13,21 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// ------------------------------------------------------------------ one new token per sequence
-// Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its tiles of 64 keys. Warp 4 copies:
+// Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its tiles of 64 keys. The last warp copies:
 // its lanes look the pages up, well ahead, and request the tile by TMA (boxes of min(page, 64) keys x 64 dims, 128-byte swizzle) into a ring
-// of `stages`. Warp w < 4 owns keys 16 w .. 16 w + 15 of every tile, with a softmax of its own; the four are joined at the end.
-// Products are mma.sync m16n8k16 with keys (then dims) as the 16 rows and query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T: at most eight heads
-// waste nothing that way. (With the heads as rows, half of everything was idle: 874 instructions per warp and tile, 166 registers and 5.3 TB/s.)
-// Positions that the row does not see, or whose entry names no page, are not fetched or hidden by index: their scores become -inf and the warp that
-// owns them puts zeros over their values, so nothing that lies there counts.
+// of `stages`. The others have 16 keys of every tile and 8 NB rows each (RG groups of them), with a softmax of their own; the four shares of the keys are
+// joined at the end.
+// Products are mma.sync m16n8k16 with keys (then dims) as the 16 rows and attention rows as the 8 columns, S^T = K Q^T and O^T = V^T P^T: at most eight
+// rows waste nothing that way. (With the rows as rows, half of everything was idle: 874 instructions per warp and tile, 166 registers and 5.3 TB/s.)
+// Positions that a row does not see, or whose entry names no page, are not fetched or hidden by index: their scores become -inf, and where some row
+// does not see some of the 16 keys, values that are not finite are replaced by zeros on their way into the product (add_poison has the rest), so nothing
+// that lies there counts.
 //
 // Shares: piece c of ct tiles belongs to block c % gridDim.x, however long the sequence turns out to be. JOIN: 0 there is one block, 1 the
 // blocks leave (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel, 2 they are one cluster and join through distributed shared memory.
 constexpr int KT = 64;
 constexpr int MAX_STAGES = 6;
-constexpr int DEC_THREADS = 160;
+constexpr int FEW_ROWS = 32;
 enum { JOIN_NONE = 0, JOIN_SCRATCH = 1, JOIN_CLUSTER = 2 };
 constexpr int CLUSTER_MAX = 8;
 
@@ -37,29 +38,31 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
-constexpr size_t dec_tile_bytes(int HD) { return (size_t)KT * 2 * HD; }
-constexpr size_t dec_smem(int HD, int stages) {
-  const size_t ring = 2 * stages * dec_tile_bytes(HD), join = (size_t)(4 * 16 * (HD + 4) + 16 * HD) * 4 + 5 * 16 * 8;
+constexpr size_t few_tile_bytes(int HD) { return (size_t)KT * 2 * HD; }
+constexpr size_t few_smem(int HD, int rows, int stages) {
+  const size_t ring = 2 * stages * few_tile_bytes(HD), join = (size_t)rows * ((4 * (HD + 4) + HD) * 4 + 5 * 8);
   return (ring > join ? ring : join) + 1024;
 }
 
-// NB: blocks of eight query heads
-template <int HD, int NB, int JOIN>
-__global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                        const __grid_constant__ PagedAttnArgs a, PagedJoin join, int ct, int stages, int* status) {
+template <int HD, int NB, int RG, int JOIN>
+__global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                       const __grid_constant__ PagedAttnArgs a, PagedJoin join, int ct, int stages, int* status) {
   constexpr int ATOM = KT * 128, TILE = ATOM * (HD / 64);  // bytes of 64 keys x 64 dims, and of a tile
+  constexpr int WARPS = 4 * RG, ROWS = 8 * NB * RG, BLOCK = 32 * (WARPS + 1);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES];
   __shared__ uint32_t page_bits[MAX_STAGES];
+  __shared__ int poison;
   const int part = blockIdx.x, parts = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = a.Hq / a.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3, mi = lane >> 3, r8 = lane & 7;
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; i++) {
       tc::mbar_init(smem_u32(&full[i]), 1);
-      tc::mbar_init(smem_u32(&empty[i]), 4);
+      tc::mbar_init(smem_u32(&empty[i]), WARPS);
     }
+    poison = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -68,15 +71,16 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
   const int box = min(a.at.page, KT), boxes = KT / box;
   const int64_t t0 = a.at.starts[b];
   const int last = a.at.starts[b + 1], len = a.at.lens[b];
-  if (t0 < 0 || t0 >= a.at.T || last <= t0) return;  // the same for every block of a cluster
-  const int pos = len - last + (int)t0;
-  const PagedWalk w = paged_walk(a.at, len, pos, pos, a.window, a.first, KT);
-  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  if (t0 < 0 || last > a.at.T || last <= t0) return;  // the same for every block of a cluster
+  const int R = (int)min((int64_t)ROWS / G, last - t0) * G, lo_pos = len - last + (int)t0, hi_pos = lo_pos + R / G - 1;
+  const PagedWalk w = paged_walk(a.at, len, lo_pos, hi_pos, a.window, a.first, KT);
   const int n = share_count(w.total, part, parts, ct);
   const uint32_t sK = smem_u32(smem), sV = sK + stages * TILE;
+  auto row_head = [&](int row) { return (t0 + row / G) * a.Hq + hk * G + row % G; };  // place among all rows and heads
 
   float o[HD / 16][NB][4], m_run[NB][2], l_run[NB][2];
-  if (warp == 4) {
+  const int kg = warp & 3, row0 = (warp >> 2) * 8 * NB;  // keys 16 kg .. of a tile, rows row0 .. of this warp
+  if (warp == WARPS) {
     auto page_of = [&](int i, int x) {
       const int j = i < n ? w.tile(share_tile(i, part, parts, ct)) * KT + x * box : w.end;
       return j < w.end ? paged_page(a.at, b, j >> a.at.shift) : -1;
@@ -115,40 +119,47 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
     for (int i = max(0, got - stages); i < got; i++) tc::mbar_wait(smem_u32(&full[i % stages]), (uint32_t)((i / stages) & 1));
     __syncwarp();
   } else {
-    // queries as columns: head 8 nb + g, dims 16 ks + 2 tig ..
+    // queries as columns: row row0 + 8 nb + g, dims 16 ks + 2 tig ..
     uint32_t qf[HD / 16][NB][2];
-    const bf16* q0 = a.q + (t0 * a.Hq + hk * G) * HD;
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ks++)
+    for (int nb = 0; nb < NB; nb++) {
+      const int row = row0 + 8 * nb + g;
+      const bf16* q = a.q + (row < R ? row_head(row) * HD : 0) + 2 * tig;
 #pragma unroll
-      for (int nb = 0; nb < NB; nb++) {
-        const bf16* q = q0 + (8 * nb + g) * HD + ks * 16 + 2 * tig;
-        qf[ks][nb][0] = 8 * nb + g < G ? *(const uint32_t*)q : 0u;
-        qf[ks][nb][1] = 8 * nb + g < G ? *(const uint32_t*)(q + 8) : 0u;
+      for (int ks = 0; ks < HD / 16; ks++) {
+        qf[ks][nb][0] = row < R ? *(const uint32_t*)(q + ks * 16) : 0u;
+        qf[ks][nb][1] = row < R ? *(const uint32_t*)(q + ks * 16 + 8) : 0u;
       }
+    }
+    int pos[NB][2];  // of the columns that this thread has scores of
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
       for (int j = 0; j < HD / 16; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) o[j][nb][i] = 0.f;
-      m_run[nb][0] = m_run[nb][1] = -INFINITY;
-      l_run[nb][0] = l_run[nb][1] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        m_run[nb][h] = -INFINITY;
+        l_run[nb][h] = 0.f;
+        pos[nb][h] = lo_pos + (row0 + 8 * nb + 2 * tig + h) / G;
+      }
     }
     const float scale_log2 = a.scale * LOG2E;
     const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
+    uint32_t found = 0;
     bool ok = true;
     int st = 0, step = part * ct, left = ct;  // place in the walk, tiles of the piece
     uint32_t ph = 0;
     for (int i = 0; i < n; i++) {
-      const int j0 = w.tile(step++) * KT + warp * 16;
+      const int j0 = w.tile(step++) * KT + kg * 16;
       if (--left == 0) left = ct, step += (parts - 1) * ct;
       ok = ok && tc::mbar_wait(smem_u32(&full[st]), ph);
       __syncwarp();
-      const uint32_t tK = sK + st * TILE + warp * 16 * 128, tV = sV + st * TILE + warp * 16 * 128;
-      const bool there = page_bits[st] >> (warp * 16 / box) & 1;
-      const bool whole = there && j0 + 16 <= w.end && (j0 >= lo || j0 + 16 <= a.first);
-      // scores: keys g and g + 8, heads 2 tig and 2 tig + 1
+      const uint32_t tK = sK + st * TILE + kg * 16 * 128, tV = sV + st * TILE + kg * 16 * 128;
+      const bool there = page_bits[st] >> (kg * 16 / box) & 1;
+      const bool whole = there && sees_all(a, w.end, j0, 16, lo_pos, hi_pos);
+      // scores: keys g and g + 8, rows 2 tig and 2 tig + 1
       float s[NB][4], s2[NB][4];  // two sums, so that half as many products wait for one another
 #pragma unroll
       for (int nb = 0; nb < NB; nb++)
@@ -166,18 +177,13 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
 #pragma unroll
         for (int e = 0; e < 4; e++) s[nb][e] += s2[nb][e];
       if (!whole) {
-        auto seen = [&](int r) { return there && j0 + r < w.end && (j0 + r >= lo || j0 + r < a.first); };
-        const bool s0 = seen(g), s1 = seen(g + 8);
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-          if (!s0) s[nb][0] = s[nb][1] = -INFINITY;
-          if (!s1) s[nb][2] = s[nb][3] = -INFINITY;
-        }
-        for (int x = lane; x < 16 * (HD / 8); x += 32) {
-          const int r = x / (HD / 8), c = x % (HD / 8);
-          if (!seen(r)) *(uint4*)(smem + (tV - sK) + (c >> 3) * ATOM + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        __syncwarp();
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int j = j0 + g + (e & 2) * 4, p = pos[nb][e & 1];
+            if (!(there && j <= p && j < w.end && (!a.window || j > p - a.window || j < a.first))) s[nb][e] = -INFINITY;
+          }
       }
       uint32_t pf[NB][2], pl[NB][2];
 #pragma unroll
@@ -214,25 +220,34 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
         }
       }
 #pragma unroll
-      for (int j0 = 0; j0 < HD / 16; j0 += 4) {
+      for (int j4 = 0; j4 < HD / 16; j4 += 4) {
         uint32_t vf[4][4];  // dims 16 j .. as rows, keys as columns; four products between the two that add to one sum
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          ldsm_x4_t(tV + (j0 >> 2) * ATOM + ((mi >> 1) * 8 + r8) * 128 + (((j * 2 + (mi & 1)) << 4) ^ sw), vf[j]);
+        for (int j = 0; j < 4; j++) ldsm_x4_t(tV + (j4 >> 2) * ATOM + ((mi >> 1) * 8 + r8) * 128 + (((j * 2 + (mi & 1)) << 4) ^ sw), vf[j]);
+        if (!whole) {
 #pragma unroll
-          for (int nb = 0; nb < NB; nb++) mma_bf16(o[j0 + j][nb], vf[j], pf[nb][0], pf[nb][1]);
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+              found |= not_finite(vf[j][x]);
+              vf[j][x] = only_finite(vf[j][x]);
+            }
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-          for (int nb = 0; nb < NB; nb++) mma_bf16(o[j0 + j][nb], vf[j], pl[nb][0], pl[nb][1]);
+          for (int nb = 0; nb < NB; nb++) mma_bf16(o[j4 + j][nb], vf[j], pf[nb][0], pf[nb][1]);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++) mma_bf16(o[j4 + j][nb], vf[j], pl[nb][0], pl[nb][1]);
       }
-      if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros stay in front of the next copy into this place
       __syncwarp();
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[st])) : "memory");
       if (++st == stages) st = 0, ph ^= 1;
     }
     if (!__all_sync(0xffffffffu, ok) && lane == 0) tc::set_status(status, 48);
+    if (found) poison = 1;
 #pragma unroll
     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -241,48 +256,53 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
         for (int x = 4; x < 32; x <<= 1) l_run[nb][h] += __shfl_xor_sync(0xffffffffu, l_run[nb][h], x);
   }
   __syncthreads();  // every copy has been waited for, and nobody reads a tile any more
-  // the four warps joined through shared memory
+  // the four shares of the keys joined through shared memory
   constexpr int LD = HD + 4;
-  float* so = (float*)smem;                    // [4 warps][16 heads][LD]
-  float* jo = so + 4 * 16 * LD;                // [G][HD] joined
-  float2* sml = (float2*)(jo + 16 * HD);       // [4 warps][16 heads]
-  float2* jml = sml + 4 * 16;                  // [G]
-  if (warp < 4) {
+  float* so = (float*)smem;                    // [4][ROWS][LD]
+  float* jo = so + 4 * ROWS * LD;              // [ROWS][HD] joined
+  float2* sml = (float2*)(jo + ROWS * HD);     // [4][ROWS]
+  float2* jml = sml + 4 * ROWS;                // [ROWS]
+  if (warp < WARPS) {
 #pragma unroll
     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int head = 8 * nb + 2 * tig + h;
-        if (head < G) {
+        const int row = row0 + 8 * nb + 2 * tig + h;
+        if (row < R) {
 #pragma unroll
           for (int j = 0; j < HD / 16; j++) {
-            so[(warp * 16 + head) * LD + 16 * j + g] = o[j][nb][h];
-            so[(warp * 16 + head) * LD + 16 * j + g + 8] = o[j][nb][2 + h];
+            so[(kg * ROWS + row) * LD + 16 * j + g] = o[j][nb][h];
+            so[(kg * ROWS + row) * LD + 16 * j + g + 8] = o[j][nb][2 + h];
           }
-          if (g == 0) sml[warp * 16 + head] = make_float2(m_run[nb][h], l_run[nb][h]);
+          if (g == 0) sml[kg * ROWS + row] = make_float2(m_run[nb][h], l_run[nb][h]);
         }
       }
   }
   __syncthreads();
-  bf16* out = a.out + (t0 * a.Hq + hk * G) * HD;
-  for (int e = threadIdx.x; e < G * (HD / 4); e += DEC_THREADS) {
+  const bool bad = poison;
+  for (int e = threadIdx.x; e < R * (HD / 4); e += BLOCK) {
     const int row = e / (HD / 4), d = e % (HD / 4) * 4;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) M = fmaxf(M, sml[i * 16 + row].x);
+    for (int i = 0; i < 4; i++) M = fmaxf(M, sml[i * ROWS + row].x);
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float f = weight_of(sml[i * 16 + row].x, M);
-      const float4 p = *(const float4*)(so + (i * 16 + row) * LD + d);
-      L += sml[i * 16 + row].y * f;
+      const float f = weight_of(sml[i * ROWS + row].x, M);
+      const float4 p = *(const float4*)(so + (i * ROWS + row) * LD + d);
+      L += sml[i * ROWS + row].y * f;
       O.x += p.x * f; O.y += p.y * f; O.z += p.z * f; O.w += p.w * f;
+    }
+    if (bad && L != 0.f) {
+      float r[4] = {O.x, O.y, O.z, O.w};
+      add_poison(a, w, b, hk, part, parts, ct, KT, 0, 1, n, lo_pos + row / G, d, 4, r);
+      O = make_float4(r[0], r[1], r[2], r[3]);
     }
     if (JOIN == JOIN_NONE) {
       const float inv = L == 0.f ? 0.f : 1.0f / L;
-      *(uint2*)(out + row * HD + d) = make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
+      *(uint2*)(a.out + row_head(row) * HD + d) = make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
     } else if (JOIN == JOIN_SCRATCH) {
-      const int64_t at = (t0 * a.Hq + hk * G + row) * parts + part;
+      const int64_t at = row_head(row) * parts + part;
       if (L != 0.f) *(float4*)(join.o + at * HD + d) = O;  // read only where the sum is not zero
       if (d == 0) join.ml[at] = make_float2(M, L);
     } else {
@@ -298,7 +318,7 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"(local), "r"(rank));
       return x;
     };
-    for (int e = part * DEC_THREADS + threadIdx.x; e < G * (HD / 4); e += parts * DEC_THREADS) {
+    for (int e = part * BLOCK + threadIdx.x; e < R * (HD / 4); e += parts * BLOCK) {
       const int row = e / (HD / 4), d = e % (HD / 4) * 4;
       float2 ml[CLUSTER_MAX];
       float4 p[CLUSTER_MAX];
@@ -324,7 +344,7 @@ __global__ void __launch_bounds__(DEC_THREADS) attn_paged_decode_kernel(const __
           O.x += p[i].x * f; O.y += p[i].y * f; O.z += p[i].z * f; O.w += p[i].w * f;
         }
       const float inv = L == 0.f ? 0.f : 1.0f / L;
-      *(uint2*)(out + row * HD + d) = make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
+      *(uint2*)(a.out + row_head(row) * HD + d) = make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
     }
     __syncthreads();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody leaves while its memory is read
@@ -379,23 +399,24 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, P
   for (int e = 0; e < E; e += 2) *(uint32_t*)(a.out + at * HD + lane * E + e) = pack_bf16(O[e] * inv, O[e + 1] * inv);
 }
 
-struct DecodePlan {
+struct FewPlan {
   int parts = 1, stages = 2, join = JOIN_NONE;
 };
-// How a decode step is cut, from its sizes, by a model in microseconds: a block starts after 3 and has a tile every 1.3 / stages at best (the latency of a copy) and
+// How the keys are cut, from the sizes, by a model in microseconds: a block starts after 3 and has a tile every 1.3 / stages at best (the latency of a copy) and
 // every `chain` (its products and its softmax one after the other); an SM takes 46 GB/s; blocks beyond those that fit run in further rounds, with half a round of unevenness; the join in a cluster takes 1.5, the one through scratch 4 and its bytes.
 // Ring: what shared memory leaves the blocks that share an SM. Clusters need all their blocks at once: one wave only, counted with 7/8 of the SMs, and
 // with shared memory for two blocks on each, or those that find no eight empty SMs wait for a second wave.
-DecodePlan plan_decode(const strictb200_ctx* ctx, int HD, int64_t units, int64_t tiles, int64_t out_floats) {
-  const double stage = 2.0 * dec_tile_bytes(HD), tile_us = stage / 46e3, sms = ctx->sm_count;
-  const double chain = HD == 128 ? 0.8 : 0.6;
-  const int fit = HD == 128 ? 3 : 5;  // blocks per SM with two stages: shared memory (128 dims), registers (64 dims)
-  DecodePlan best;
+FewPlan plan_few(const strictb200_ctx* ctx, int HD, int rows, int64_t units, int64_t tiles, double out_floats) {
+  const double stage = 2.0 * few_tile_bytes(HD), tile_us = stage / 46e3, sms = ctx->sm_count;
+  const double chain = (HD == 128 ? 0.8 : 0.6) * (rows > 8 ? 1.4 : 1);
+  // blocks per SM with two stages: shared memory (8 rows of 128 dims), registers (otherwise)
+  const int fit = rows > 16 ? (HD == 128 ? 1 : 2) : rows > 8 ? (HD == 128 ? 2 : 4) : HD == 128 ? 3 : 5;
+  FewPlan best;
   double best_us = 1e30;
   for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 128); parts += parts < 16 ? 1 : parts / 8) {
     const double ct = (double)((tiles + parts - 1) / parts), blocks = (double)(units * parts);
     const int resident = (int)std::min<double>(fit, std::ceil(blocks / sms));
-    DecodePlan p;
+    FewPlan p;
     p.parts = (int)parts;
     const bool one_wave = blocks <= (parts > 1 ? 0.875 : 1) * fit * sms;
     const int share = one_wave && parts > 1 && parts <= CLUSTER_MAX ? std::max(2, resident) : resident;
@@ -412,20 +433,20 @@ DecodePlan plan_decode(const strictb200_ctx* ctx, int HD, int64_t units, int64_t
   return best;
 }
 
-template <int HD, int NB>
-int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
+template <int HD, int NB, int RG>
+int few_rows(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   static SbDeviceOnce once;
   SB_CUDA(once.run(ctx->device, [&] {
-    for (auto f : {attn_paged_decode_kernel<HD, NB, JOIN_NONE>, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>}) {
-      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dec_smem(HD, MAX_STAGES));
+    for (auto f : {attn_paged_few_kernel<HD, NB, RG, JOIN_NONE>, attn_paged_few_kernel<HD, NB, RG, JOIN_SCRATCH>, attn_paged_few_kernel<HD, NB, RG, JOIN_CLUSTER>}) {
+      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(HD, 8 * NB * RG, MAX_STAGES));
       if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
   }));
   const int64_t tiles = std::max<int64_t>(1, paged_walk_tiles(a, KT));
-  const DecodePlan plan = plan_decode(ctx, HD, (int64_t)a.at.B * a.Hkv, tiles, (double)a.at.T * a.Hq * HD);
+  const FewPlan plan = plan_few(ctx, HD, 8 * NB * RG, (int64_t)a.at.B * a.Hkv, tiles, (double)a.at.T * a.Hq * HD);
   const int parts = plan.parts, ct = (int)((tiles + parts - 1) / parts), stages = plan.stages;
-  const size_t smem = dec_smem(HD, stages);
+  const size_t smem = few_smem(HD, 8 * NB * RG, stages);
   const dim3 grid((unsigned)parts, (unsigned)a.Hkv, (unsigned)a.at.B);
   PagedJoin buf;
   if (plan.join == JOIN_SCRATCH) SB_TRY(paged_join_scratch(ctx, a, parts, &buf));
@@ -433,10 +454,10 @@ int decode(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(paged_map_rows(&mk, a.k, rows, HD, std::min(a.at.page, KT)));
   SB_TRY(paged_map_rows(&mv, a.v, rows, HD, std::min(a.at.page, KT)));
-  const dim3 block(DEC_THREADS);
-  if (plan.join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
-  else if (plan.join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_decode_kernel<HD, NB, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
-  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_decode_kernel<HD, NB, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, stages, ctx->d_status));
+  const dim3 block(128 * RG + 32);
+  if (plan.join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_few_kernel<HD, NB, RG, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
+  else if (plan.join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_few_kernel<HD, NB, RG, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
+  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_few_kernel<HD, NB, RG, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, stages, ctx->d_status));
   ctx->launches++;
   return plan.join == JOIN_SCRATCH ? paged_join(ctx, a, buf) : STRICTB200_OK;
 }
@@ -465,7 +486,9 @@ int64_t paged_walk_tiles(const PagedAttnArgs& a, int kt) {
 }
 
 int k_attn_paged(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  if (a.max_new > 1 || a.Hq / a.Hkv > 16 || a.at.B > 65535) return k_attn_paged_tiles(ctx, a);
-  if (a.Hq / a.Hkv > 8) return a.D == 128 ? decode<128, 2>(ctx, a) : decode<64, 2>(ctx, a);
-  return a.D == 128 ? decode<128, 1>(ctx, a) : decode<64, 1>(ctx, a);
+  const int64_t rows = (int64_t)std::max(1, a.max_new) * (a.Hq / a.Hkv);
+  if (rows > FEW_ROWS || a.at.B > 65535) return k_attn_paged_tiles(ctx, a);
+  if (rows > 16) return a.D == 128 ? few_rows<128, 2, 2>(ctx, a) : few_rows<64, 2, 2>(ctx, a);
+  if (rows > 8) return a.D == 128 ? few_rows<128, 2, 1>(ctx, a) : few_rows<64, 2, 1>(ctx, a);
+  return a.D == 128 ? few_rows<128, 1, 1>(ctx, a) : few_rows<64, 1, 1>(ctx, a);
 }

@@ -37,6 +37,15 @@ struct PageNames {
     return lane < boxes ? p : -1;
   }
 };
+// Which halves of a pair of bf16 are infinities or NaN: bits 15 and 31; and the pair with zeros in their place.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) { return w & ~((not_finite(w) >> 15) * 0xFFFFu); }
+
+// Whether keys [k0, k0 + kn) are all seen by the rows at positions lo_pos .. hi_pos (end: no row sees that position or a later one).
+__device__ __forceinline__ bool sees_all(const PagedAttnArgs& a, int end, int k0, int kn, int lo_pos, int hi_pos) {
+  return k0 + kn <= end && k0 + kn - 1 <= lo_pos && (!a.window || k0 > hi_pos - a.window || k0 + kn <= a.first);
+}
+
 // i-th key tile of a block whose share is every parts-th piece of ct tiles
 __device__ __forceinline__ int share_tile(int i, int part, int parts, int ct) { return parts == 1 ? i : (i / ct * parts + part) * ct + i % ct; }
 __device__ __forceinline__ int share_count(int total, int part, int parts, int ct) {
@@ -45,6 +54,27 @@ __device__ __forceinline__ int share_count(int total, int part, int parts, int c
   return rounds * ct + min(max(rest - part * ct, 0), ct);
 }
 
+
+// What a weight of zero times a value that is not finite would do to a row that does not see it is avoided by zeros in place of such values in tiles that some
+// row does not see whole. Where there were any, a row that does see them gets them here: those of the n tiles i0, i0 + step .. of a block, dims d0 .. d0 + nd - 1, added
+// to r. Seldom, so slow. (A weight is positive; that it may have been rounded to zero does not matter to the sum: it is not finite either way.)
+static __device__ __noinline__ void add_poison(const PagedAttnArgs& a, const PagedWalk& w, int b, int hk, int part, int parts, int ct, int kt, int i0, int step, int n,
+                                               int pos, int d0, int nd, float* r) {
+  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  for (int i = i0; n > 0; n--, i += step) {
+    const int k0 = w.tile(share_tile(i, part, parts, ct)) * kt;
+    for (int j = k0; j < min(k0 + kt, min(w.end, pos + 1)); j++) {
+      if (j < lo && j >= a.first) continue;
+      const int page = paged_page(a.at, b, j >> a.at.shift);
+      if (page < 0) continue;
+      const bf16* v = a.v + ((page * (int64_t)a.Hkv + hk) * a.at.page + (j & (a.at.page - 1))) * a.D + d0;
+      for (int d = 0; d < nd; d++) {
+        const float x = __bfloat162float(v[d]);
+        if (!isfinite(x)) r[d] += x;
+      }
+    }
+  }
+}
 
 // Tensor map of rows of `cols` bf16, boxes of `box` rows x 64 columns, 128-byte swizzle
 inline int paged_map_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box) {

@@ -4,10 +4,10 @@
 // tile of 128 rows (one TMA box: 64 dims x G heads x tokens), so keys and values are fetched once for all of them and a tile spans few positions. Rows
 // are lanes of tensor memory. Per tile of 128 keys, as in the attention over contiguous caches:
 //   S = Q K^T      operands in shared memory, fp32 sums in tensor memory
-//   softmax        two threads per row (64 columns each), running maximum followed lazily (a row of O is rescaled when its maximum grew by more
-//                  than 2^8), weights back to tensor memory as two bf16 terms (hi + lo by truncation: 2^-16)
+//   softmax        a thread per row, running maximum followed lazily (a row of O is rescaled when its maximum grew by more than 2^8), weights back to
+//                  tensor memory as two bf16 terms (hi + lo by truncation: 2^-16)
 //   O += P V       weights from tensor memory, values from shared memory; O stays in tensor memory
-// Roles: warps 0..15 softmax, 16 issues products, 17 copies, 18 and 19 look over values. A block works on two things in turn, so that the tensor
+// Roles: warps 0..7 softmax, 8 issues products, 9 copies, 10 and 11 look over values. A block works on two things in turn, so that the tensor
 // pipe runs one while the softmax warps are at the other:
 //   two tiles (ONE = false)   A and B, 2 * (128 / G) consecutive tokens, sharing every key tile
 //   one tile (ONE = true)     few rows: the even and the odd key tiles of the same queries, each with a softmax of its own; joined later
@@ -27,7 +27,7 @@ using namespace tc;
 namespace {
 
 constexpr int BQ = 128, BKV = 128;
-constexpr int THREADS = 640;
+constexpr int THREADS = 384;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct TilesArgs {
@@ -50,45 +50,39 @@ struct Work {
   int nt;                // key tiles of this block
 };
 
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
-
-// Whether the keys [k0, k0 + 128) are all seen by the rows at positions lo .. hi.
-__device__ __forceinline__ bool sees_all(const PagedAttnArgs& a, int end, int k0, int lo, int hi) {
-  return k0 + BKV <= end && k0 + BKV - 1 <= lo && (!a.window || k0 > hi - a.window || k0 + BKV <= a.first);
+// two fp32 operations per instruction
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
-// The values that are not finite, of the keys that the row at `pos` sees, in dims [d0, d0 + 32): of the tiles that had theirs replaced.
-__device__ __noinline__ void add_poison(const TilesArgs& t, const Work& k, int pos, int first_i, int step_i, int n_i, int d0, uint32_t* r) {
-  const PagedAttnArgs& a = t.a;
-  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
-  for (int s = 0; s < n_i; s++) {
-    const int k0 = k.w.tile(share_tile(first_i + s * step_i, k.part, t.parts, t.ct)) * BKV;
-    for (int j = k0; j < min(k0 + BKV, min(k.w.end, pos + 1)); j++) {
-      if (j < lo && j >= a.first) continue;
-      const int page = paged_page(a.at, k.b, j >> a.at.shift);
-      if (page < 0) continue;
-      const bf16* v = a.v + ((page * (int64_t)a.Hkv + k.hk) * a.at.page + (j & (a.at.page - 1))) * a.D + d0;
-      for (int i = 0; i < 32; i++) {
-        const float x = __bfloat162float(v[i]);
-        if (!isfinite(x)) r[i] = __float_as_uint(__uint_as_float(r[i]) + x);
-      }
-    }
-  }
-}
-
+// key (and value) tiles in shared memory: what 227 KB hold beside the queries
 template <int QA, bool ONE>
-constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 4) * QA * HALF_BYTES + 1024; }
+constexpr int tiles_ring() { return QA == 1 ? 4 : ONE ? 3 : 2; }
+template <int QA, bool ONE>
+constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 2 * tiles_ring<QA, ONE>()) * QA * HALF_BYTES + 1024; }
 
 template <int QA, bool ONE>
 __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TilesArgs t) {
-  constexpr int TILE = QA * HALF_BYTES, NQ = ONE ? 1 : 2, D = 64 * QA;
+  constexpr int TILE = QA * HALF_BYTES, NQ = ONE ? 1 : 2, D = 64 * QA, RING = tiles_ring<QA, ONE>();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t bar_q, k_full[2], k_empty[2], v_full[2], v_ready[2], v_empty[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ __align__(8) uint64_t bar_q, k_full[RING], k_empty[RING], v_full[RING], v_ready[RING], v_empty[RING], bar_s[2], bar_p[2][2], bar_o[2];
   __shared__ uint32_t tmem_base_slot;
-  __shared__ float x_max[2][2][BQ], x_sum[2][BQ];  // [stream][column half][row]
-  __shared__ uint32_t page_bits[4];                // pages of a key tile that are there
+  __shared__ uint32_t page_bits[8];  // pages of a key tile that are there
   __shared__ int poison;
   const PagedAttnArgs& a = t.a;
   pdl_wait();
@@ -135,18 +129,20 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   }
   auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, t.ct)) * BKV; };  // first key of the block's i-th tile
 
-  const uint32_t sQ = smem_u32(smem), sK = sQ + NQ * TILE, sV = sK + 2 * TILE;
+  const uint32_t sQ = smem_u32(smem), sK = sQ + NQ * TILE, sV = sK + RING * TILE;
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&bar_q), 1);
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < RING; i++) {
       mbar_init(smem_u32(&k_full[i]), 1); mbar_init(smem_u32(&k_empty[i]), 1);
       mbar_init(smem_u32(&v_full[i]), 1); mbar_init(smem_u32(&v_ready[i]), 64); mbar_init(smem_u32(&v_empty[i]), 1);
-      mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i]), 2 * BQ); mbar_init(smem_u32(&bar_o[i]), 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i][0]), BQ); mbar_init(smem_u32(&bar_p[i][1]), BQ); mbar_init(smem_u32(&bar_o[i]), 1);
     }
     poison = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 16) {
+  if (warp == 8) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -160,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   const int box = min(a.at.page, BKV), boxes = BKV / box;  // keys of a box; boxes of a tile
 
-  if (warp == 17) {
+  if (warp == 9) {
     // ---- copies. Lane i looks up the i-th box of a tile, one tile ahead.
     if (lane == 0 && k.nt > 0) {
       const uint32_t bytes = (uint32_t)(t.G * t.tw * 128 * QA);
@@ -178,21 +174,21 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
     int got = 0;
     bool good = true;
     for (int i = 0; i < k.nt; i++) {
-      const int page = names.of(i, boxes, lane, page_of), st = i & 1;
-      const uint32_t ph = (uint32_t)((i >> 1) & 1) ^ 1;
+      const int page = names.of(i, boxes, lane, page_of), st = i % RING;
+      const uint32_t ph = (uint32_t)(i / RING & 1) ^ 1;
       const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
       const uint32_t bytes = (uint32_t)(__popc(there) * box * 128 * QA);
       const int row = page < 0 ? 0 : (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
-      if (i >= 2) good = mbar_wait(smem_u32(&k_empty[st]), ph);
+      if (i >= RING) good = mbar_wait(smem_u32(&k_empty[st]), ph);
       if (!__all_sync(0xffffffffu, good)) { if (lane == 0) set_status(t.status, 41); good = false; break; }
       if (lane == 0) {
-        page_bits[i & 3] = there;
+        page_bits[i & 7] = there;
         mbar_expect_tx(smem_u32(&k_full[st]), bytes);
       }
       __syncwarp();
       if (page >= 0)
         for (int x = 0; x < QA; x++) tma_load_2d(sK + st * TILE + x * HALF_BYTES + lane * box * 128, &map_k, x * 64, row, smem_u32(&k_full[st]));
-      if (i >= 2) good = mbar_wait(smem_u32(&v_empty[st]), ph);
+      if (i >= RING) good = mbar_wait(smem_u32(&v_empty[st]), ph);
       if (!__all_sync(0xffffffffu, good)) { if (lane == 0) { set_status(t.status, 42); mbar_wait(smem_u32(&k_full[st]), ph ^ 1); } good = false; break; }
       if (lane == 0) mbar_expect_tx(smem_u32(&v_full[st]), bytes);
       __syncwarp();
@@ -203,13 +199,13 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
     // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
     if (lane == 0 && k.nt > 0) {
       mbar_wait(smem_u32(&bar_q), 0);
-      for (int i = max(0, got - 2); i < got; i++) {
-        mbar_wait(smem_u32(&k_full[i & 1]), (uint32_t)((i >> 1) & 1));
-        mbar_wait(smem_u32(&v_full[i & 1]), (uint32_t)((i >> 1) & 1));
+      for (int i = max(0, got - RING); i < got; i++) {
+        mbar_wait(smem_u32(&k_full[i % RING]), (uint32_t)(i / RING & 1));
+        mbar_wait(smem_u32(&v_full[i % RING]), (uint32_t)(i / RING & 1));
       }
     }
     __syncwarp();
-  } else if (warp == 16) {
+  } else if (warp == 8) {
     // ---- products
     if (lane == 0 && k.nt > 0) {
       auto issue_s = [&](int w, int st) {
@@ -221,16 +217,21 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
         }
         tc_commit(smem_u32(&bar_s[w]));
       };
-      auto issue_pv = [&](int w, int st, bool first) {
+      auto issue_pv = [&](int w, int st, bool first, uint32_t ph) {  // by halves of the keys, as their weights come
         const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
 #pragma unroll
         for (int s = 0; s < 8; s++) {
+          if ((s & 3) == 0) {
+            if (!mbar_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
+            tc_fence_after();
+          }
           const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
           const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
           tc_mma_ts(tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
           tc_mma_ts(tO, tS + pcol + 16, dv, idesc_pv, 1u);
         }
         tc_commit(smem_u32(&bar_o[w]));
+        return true;
       };
       bool good = mbar_wait(smem_u32(&bar_q), 0);
       if (ONE) {
@@ -245,17 +246,17 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
         for (int s = 0; s < nt[0] && good; s++) {
           for (int w = 0; w < 2 && good; w++) {
             if (s >= nt[w]) break;
-            good = mbar_wait(smem_u32(&v_ready[w]), (uint32_t)(s & 1)) && mbar_wait(smem_u32(&bar_p[w]), (uint32_t)(s & 1));
+            const int i = 2 * s + w;
+            good = mbar_wait(smem_u32(&v_ready[i % RING]), (uint32_t)(i / RING & 1)) && issue_pv(w, i % RING, s == 0, (uint32_t)(s & 1));
             if (!good) break;
-            tc_fence_after();
-            issue_pv(w, w, s == 0);
-            tc_commit(smem_u32(&v_empty[w]));
+            tc_commit(smem_u32(&v_empty[i % RING]));
             if (s + 1 < nt[w]) {
-              good = mbar_wait(smem_u32(&k_full[w]), (uint32_t)((s + 1) & 1));
+              const int in = i + 2;
+              good = mbar_wait(smem_u32(&k_full[in % RING]), (uint32_t)(in / RING & 1));
               if (!good) break;
               tc_fence_after();
-              issue_s(w, w);
-              tc_commit(smem_u32(&k_empty[w]));
+              issue_s(w, in % RING);
+              tc_commit(smem_u32(&k_empty[in % RING]));
             }
           }
         }
@@ -268,46 +269,48 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
           tc_commit(smem_u32(&k_empty[0]));
         }
         for (int i = 0; i < k.nt && good; i++) {
-          const int st = i & 1;
-          good = mbar_wait(smem_u32(&v_ready[st]), (uint32_t)((i >> 1) & 1));
+          const int st = i % RING, in = (i + 1) % RING;
+          good = mbar_wait(smem_u32(&v_ready[st]), (uint32_t)(i / RING & 1));
           bool k_next = false;
           for (int w = 0; w < 2 && good; w++) {
             if (i < nt[w]) {
-              good = mbar_wait(smem_u32(&bar_p[w]), (uint32_t)(i & 1));
+              good = issue_pv(w, st, i == 0, (uint32_t)(i & 1));
               if (!good) break;
-              tc_fence_after();
-              issue_pv(w, st, i == 0);
             }
             if (i + 1 < nt[w]) {
               if (!k_next) {
-                good = mbar_wait(smem_u32(&k_full[(i + 1) & 1]), (uint32_t)(((i + 1) >> 1) & 1));
+                good = mbar_wait(smem_u32(&k_full[in]), (uint32_t)((i + 1) / RING & 1));
                 if (!good) break;
                 tc_fence_after();
                 k_next = true;
               }
-              issue_s(w, (i + 1) & 1);
+              issue_s(w, in);
             }
           }
           if (!good) break;
           tc_commit(smem_u32(&v_empty[st]));
-          if (i + 1 < k.nt) tc_commit(smem_u32(&k_empty[(i + 1) & 1]));
+          if (i + 1 < k.nt) tc_commit(smem_u32(&k_empty[in]));
         }
       }
-      if (!good) set_status(t.status, 43);
+      if (!good) {  // what was issued has ended before the tiles are somebody else's
+        set_status(t.status, 43);
+        tc_commit(smem_u32(&bar_q));
+        mbar_wait(smem_u32(&bar_q), 1);
+      }
     }
     __syncwarp();
-  } else if (warp >= 18) {
+  } else if (warp >= 10) {
     // ---- values of tiles that not every row sees whole
-    const int tid = (int)threadIdx.x - 18 * 32;
+    const int tid = (int)threadIdx.x - 10 * 32;
     bool good = true;
     for (int i = 0; i < k.nt && good; i++) {
-      const int st = i & 1, k0 = tile_key(i);
-      good = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((i >> 1) & 1));
+      const int st = i % RING, k0 = tile_key(i);
+      good = mbar_wait(smem_u32(&v_full[st]), (uint32_t)(i / RING & 1));
       if (!good) break;
-      const uint32_t bits = page_bits[i & 3];
-      if (bits != (1u << boxes) - 1 || !sees_all(a, k.w.end, k0, k.lo_pos, k.lo_pos + k.n - 1)) {
+      const uint32_t bits = page_bits[i & 7];
+      if (bits != (1u << boxes) - 1 || !sees_all(a, k.w.end, k0, BKV, k.lo_pos, k.lo_pos + k.n - 1)) {
         uint32_t found = 0;
-        uint4* v = (uint4*)(smem + (NQ + 2 + st) * TILE);
+        uint4* v = (uint4*)(smem + (NQ + RING + st) * TILE);
         for (int x = tid; x < QA * BKV * 8; x += 64) {
           const int r = (x >> 3) & (BKV - 1), j = k0 + r;
           const bool seen = j < k.w.end && (bits >> (r / box) & 1) && (j >= k.lo_key || j < a.first);
@@ -317,11 +320,7 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
           }
           const uint4 w = v[x];
           if (not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w)) {
-            auto clean = [](uint32_t y) {
-              const uint32_t f = not_finite(y);
-              return y & ~((f >> 15) * 0xFFFFu);
-            };
-            v[x] = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+            v[x] = make_uint4(only_finite(w.x), only_finite(w.y), only_finite(w.z), only_finite(w.w));
             found = 1;
           }
         }
@@ -332,10 +331,9 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
     }
     if (!good && lane == 0) set_status(t.status, 44);
   } else {
-    // ---- softmax of stream w
-    const int w = warp >> 3, half = (warp >> 2) & 1, row = (int)threadIdx.x & (BQ - 1);
+    // ---- softmax of stream w, a thread per row: its 128 scores stay in registers between the maximum and the exponentials
+    const int w = warp >> 2, row = (int)threadIdx.x & (BQ - 1);
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    auto wg_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); };  // the 256 threads of this stream
     const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
     const int tok = row / t.G + (ONE ? 0 : w * t.tw);
     const bool live = row < t.G * t.tw && tok < k.n;
@@ -345,135 +343,121 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
     const int lo = a.window ? max(0, pos - a.window + 1) : 0;
     const float scale_log2 = a.scale * LOG2E;
     float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;  // after a wait that gave up the steps go on without waiting, so that no one is left alone at a barrier
+    bool ok = true;  // after a wait that gave up the steps go on without waiting
     for (int s = 0; s < nt[w]; s++) {
       const uint32_t ph = (uint32_t)(s & 1);
       const int i = ONE ? 2 * s + w : s;
       ok = ok && mbar_wait(smem_u32(&bar_s[w]), ph);
       __syncwarp();  // the loads from tensor memory want the warp together
       tc_fence_after();
-      const int k0 = tile_key(i);
-      const uint32_t bits = page_bits[i & 3];
-      const bool full = bits == (1u << boxes) - 1 && sees_all(a, k.w.end, k0, pos_a, pos_b);
-      // columns that this row sees, from this thread's 64 on
-      uint64_t see = ~0ull;
-      if (!full) {
-        see = 0;
-        const int c0 = k0 + 64 * half, hi = min(k.w.end, pos + 1) - c0, lw = lo - c0, fi = a.first - c0;
-        const uint64_t below_hi = hi >= 64 ? ~0ull : hi > 0 ? (1ull << hi) - 1 : 0;
-        const uint64_t below_lo = lw >= 64 ? ~0ull : lw > 0 ? (1ull << lw) - 1 : 0;
-        const uint64_t below_fi = fi >= 64 ? ~0ull : fi > 0 ? (1ull << fi) - 1 : 0;
-        see = below_hi & (~below_lo | below_fi);
-        for (int x = 0; x < 64; x += 16)
-          if (!(bits >> ((64 * half + x) / box) & 1)) see &= ~(0xFFFFull << x);
-      }
-      float m_tile = -INFINITY;
       if (any_live) {
-#pragma unroll 1
-        for (int c = 0; c < 2; c++) {
-          uint32_t r[32];
-          tc_ld32(tS + lane_base + (uint32_t)((2 * half + c) * 32), r);
-          tc_wait_ld();
-          if (full) {
+        uint32_t r[BKV];
 #pragma unroll
-            for (int j = 0; j < 32; j++) m_tile = fmaxf(m_tile, __uint_as_float(r[j]));
-          } else {
-            const uint32_t bm = (uint32_t)(see >> (32 * c));
+        for (int c = 0; c < 4; c++) tc_ld32(tS + lane_base + (uint32_t)(c * 32), r + c * 32);
+        const int k0 = tile_key(i);
+        const uint32_t bits = page_bits[i & 7];
+        const bool full = bits == (1u << boxes) - 1 && sees_all(a, k.w.end, k0, BKV, pos_a, pos_b);
+        tc_wait_ld();
+        if (!full) {
+          // keys [0, hi) of the tile without [first, lo) and without pages that are not there
+          const int hi = min(k.w.end, pos + 1) - k0, lw = lo - k0, fi = a.first - k0;
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            auto below = [&](int x) { return x - c * 32 >= 32 ? ~0u : x - c * 32 > 0 ? (1u << (x - c * 32)) - 1 : 0u; };
+            uint32_t see = below(hi) & (~below(lw) | below(fi));
+            if (!(bits >> (c * 32 / box) & 1)) see &= 0xFFFF0000u;
+            if (!(bits >> ((c * 32 + 16) / box) & 1)) see &= 0x0000FFFFu;
 #pragma unroll
             for (int j = 0; j < 32; j++)
-              if (bm >> j & 1) m_tile = fmaxf(m_tile, __uint_as_float(r[j]));
+              if (!(see >> j & 1)) r[c * 32 + j] = 0xFF800000u;  // -inf
           }
         }
-        x_max[w][half][row] = m_tile;
-      }
-      wg_sync();
-      if (any_live) {
-        m_tile = fmaxf(x_max[w][0][row], x_max[w][1][row]) * scale_log2;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < BKV; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+        const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale_log2;
         const bool grow = m_tile > m_run + 8.0f;
         const float m_use = grow ? m_tile : m_run;
         const float corr = grow ? exp2f(m_run - m_use) : 1.0f;
         m_run = m_use;
+        const float base = m_use == -INFINITY ? 0.f : -m_use;
         if (s > 0 && __any_sync(0xffffffffu, grow)) {
           ok = ok && mbar_wait(smem_u32(&bar_o[w]), ph ^ 1);  // the product in front has finished O
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (int c = QA * half; c < QA * half + QA; c++) {
-            uint32_t r[32];
-            tc_ld32(tO + lane_base + (uint32_t)(c * 32), r);
+          for (int c = 0; c < 4 * QA; c++) {
+            uint32_t x[16];
+            tc_ld16(tO + lane_base + (uint32_t)(c * 16), x);
             tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * corr);
-            tc_st32(tO + lane_base + (uint32_t)(c * 32), r);
+            for (int j = 0; j < 16; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * corr);
+            tc_st16(tO + lane_base + (uint32_t)(c * 16), x);
           }
         }
-        const float base = m_use == -INFINITY ? 0.f : -m_use;
-        float row_sum = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < 2; c++) {
-          const uint32_t at = tS + lane_base + (uint32_t)((2 * half + c) * 32);
-          uint32_t r[32];
-          tc_ld32(at, r);
-          tc_wait_ld();
-          const uint32_t bm = (uint32_t)(see >> (32 * c));
+        const uint64_t scale2 = pack2(__float_as_uint(scale_log2), __float_as_uint(scale_log2)), base2 = pack2(__float_as_uint(base), __float_as_uint(base));
+        const uint64_t minus = pack2(0xBF800000u, 0xBF800000u);  // -1, -1
+        uint64_t sum = 0;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
           uint32_t hi[16], lo16[16];
 #pragma unroll
           for (int j = 0; j < 16; j++) {
-            float p0 = ex2_approx(fmaf(__uint_as_float(r[2 * j]), scale_log2, base));
-            float p1 = ex2_approx(fmaf(__uint_as_float(r[2 * j + 1]), scale_log2, base));
-            if (!full) {
-              if (!(bm >> (2 * j) & 1)) p0 = 0.f;
-              if (!(bm >> (2 * j + 1) & 1)) p1 = 0.f;
-            }
-            row_sum += p0 + p1;
-            const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+            const uint64_t e = fma2(pack2(r[c * 32 + 2 * j], r[c * 32 + 2 * j + 1]), scale2, base2);
+            const uint32_t b0 = __float_as_uint(ex2_approx(__uint_as_float((uint32_t)e))), b1 = __float_as_uint(ex2_approx(__uint_as_float((uint32_t)(e >> 32))));
+            const uint64_t p = pack2(b0, b1);
+            sum = add2(sum, p);
             hi[j] = __byte_perm(b0, b1, 0x7632);
-            const uint32_t l0 = __float_as_uint(p0 - __uint_as_float(b0 & 0xFFFF0000u)), l1 = __float_as_uint(p1 - __uint_as_float(b1 & 0xFFFF0000u));
-            lo16[j] = __byte_perm(l0, l1, 0x7632);
+            const uint64_t rest = fma2(pack2(b0 & 0xFFFF0000u, b1 & 0xFFFF0000u), minus, p);
+            lo16[j] = __byte_perm((uint32_t)rest, (uint32_t)(rest >> 32), 0x7632);
           }
-          tc_st16(at, hi);
-          tc_st16(at + 16, lo16);
+          tc_st16(tS + lane_base + (uint32_t)(c * 32), hi);
+          tc_st16(tS + lane_base + (uint32_t)(c * 32 + 16), lo16);
+          if (c == 1) {  // the product of the first 64 keys may begin
+            tc_wait_st();
+            tc_fence_before();
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][0])) : "memory");
+          }
         }
+        l_run = l_run * corr + (__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)));
         tc_wait_st();
-        l_run = l_run * corr + row_sum;
+      } else {
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][0])) : "memory");
       }
       tc_fence_before();
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w])) : "memory");
-      wg_sync();  // x_max is rewritten in the next step
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][1])) : "memory");
     }
     if (nt[w] > 0) {
       ok = ok && mbar_wait(smem_u32(&bar_o[w]), (uint32_t)((nt[w] - 1) & 1));
       __syncwarp();
       tc_fence_after();
     }
-    if (!ok && lane == 0) set_status(t.status, 45);
-    if (half) x_sum[w][row] = l_run;
-    wg_sync();
-    if (!half) x_sum[w][row] += l_run;
-    wg_sync();
     ok = __all_sync(0xffffffffu, ok);
+    if (!ok && lane == 0) set_status(t.status, 45);
     if (ok && any_live) {
-      const float sum = x_sum[w][row];
       const int64_t at = (k.row0 + tok) * a.Hq + k.hk * t.G + row % t.G;
       const int np = ONE ? 2 * t.parts : t.parts, p = ONE ? 2 * k.part + w : k.part;
       const bool split = np > 1;
-      const float inv = split ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
-      if (split && live && !half) t.join.ml[at * np + p] = make_float2(m_run, sum);
+      const float inv = split ? 1.f : l_run == 0.f ? 0.f : 1.0f / l_run;
+      if (split && live) t.join.ml[at * np + p] = make_float2(m_run, l_run);
       const bool bad = *(volatile int*)&poison;
 #pragma unroll 1
-      for (int c = QA * half; c < QA * half + QA; c++) {
+      for (int c = 0; c < 2 * QA; c++) {
         uint32_t r[32];
         __syncwarp();
         if (nt[w] > 0) {
           tc_ld32(tO + lane_base + (uint32_t)(c * 32), r);
           tc_wait_ld();
         }
-        if (!live || (split && sum == 0.f)) continue;
-        if (sum == 0.f) {
+        if (!live || (split && l_run == 0.f)) continue;
+        if (l_run == 0.f) {
 #pragma unroll
           for (int j = 0; j < 32; j++) r[j] = 0;
         } else if (bad) {
-          add_poison(t, k, pos, ONE ? w : 0, ONE ? 2 : 1, nt[w], c * 32, r);
+          float f[32];
+          for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
+          add_poison(a, k.w, k.b, k.hk, k.part, t.parts, t.ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt[w], pos, c * 32, 32, f);
+          for (int j = 0; j < 32; j++) r[j] = __float_as_uint(f[j]);
         }
         if (split) {
           float* dst = t.join.o + (at * np + p) * D + c * 32;
@@ -496,7 +480,7 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }

@@ -50,6 +50,43 @@ struct Work {
   int nt;                // key tiles of this block
 };
 
+// What the issuing warp executes as a whole, one lane of it acting: operands that the compiler knows to be the same in all lanes need not be moved to
+// uniform registers one by one in front of every instruction (a lane on its own took 85 to 120 cycles per product, more than the product).
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < WAIT_LIMIT; i++) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    if (__all_sync(0xffffffffu, done)) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void warp_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void warp_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void warp_commit(uint32_t lead, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead)
+      : "memory");
+}
+
 // two fp32 operations per instruction
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
@@ -86,7 +123,7 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   __shared__ int poison;
   const PagedAttnArgs& a = t.a;
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   Work k;
   {
@@ -207,79 +244,81 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
     __syncwarp();
   } else if (warp == 8) {
     // ---- products
-    if (lane == 0 && k.nt > 0) {
+    const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0), n_all = __shfl_sync(0xffffffffu, k.nt, 0);
+    if (n_all > 0) {
+      const uint32_t lead = elected();
       auto issue_s = [&](int w, int st) {
         const uint32_t tS = tmem + (uint32_t)(w * 256);
 #pragma unroll
         for (int s = 0; s < 4 * QA; s++) {
           const uint32_t off = (uint32_t)((s >> 2) * HALF_BYTES + (s & 3) * 32);
-          tc_mma_ss(tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
+          warp_mma_ss(lead, tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
         }
-        tc_commit(smem_u32(&bar_s[w]));
+        warp_commit(lead, smem_u32(&bar_s[w]));
       };
       auto issue_pv = [&](int w, int st, bool first, uint32_t ph) {  // by halves of the keys, as their weights come
         const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
 #pragma unroll
         for (int s = 0; s < 8; s++) {
           if ((s & 3) == 0) {
-            if (!mbar_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
+            if (!warp_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
             tc_fence_after();
           }
           const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
           const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
-          tc_mma_ts(tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
-          tc_mma_ts(tO, tS + pcol + 16, dv, idesc_pv, 1u);
+          warp_mma_ts(lead, tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
+          warp_mma_ts(lead, tO, tS + pcol + 16, dv, idesc_pv, 1u);
         }
-        tc_commit(smem_u32(&bar_o[w]));
+        warp_commit(lead, smem_u32(&bar_o[w]));
         return true;
       };
-      bool good = mbar_wait(smem_u32(&bar_q), 0);
+      bool good = warp_wait(smem_u32(&bar_q), 0);
       if (ONE) {
         for (int w = 0; w < 2 && good; w++) {
-          if (nt[w] == 0) break;
-          good = mbar_wait(smem_u32(&k_full[w]), 0);
+          if ((w ? n1 : n0) == 0) break;
+          good = warp_wait(smem_u32(&k_full[w]), 0);
           if (!good) break;
           tc_fence_after();
           issue_s(w, w);
-          tc_commit(smem_u32(&k_empty[w]));
+          warp_commit(lead, smem_u32(&k_empty[w]));
         }
-        for (int s = 0; s < nt[0] && good; s++) {
+        for (int s = 0; s < n0 && good; s++) {
           for (int w = 0; w < 2 && good; w++) {
-            if (s >= nt[w]) break;
+            if (s >= (w ? n1 : n0)) break;
             const int i = 2 * s + w;
-            good = mbar_wait(smem_u32(&v_ready[i % RING]), (uint32_t)(i / RING & 1)) && issue_pv(w, i % RING, s == 0, (uint32_t)(s & 1));
+            good = warp_wait(smem_u32(&v_ready[i % RING]), (uint32_t)(i / RING & 1)) && issue_pv(w, i % RING, s == 0, (uint32_t)(s & 1));
             if (!good) break;
-            tc_commit(smem_u32(&v_empty[i % RING]));
-            if (s + 1 < nt[w]) {
+            warp_commit(lead, smem_u32(&v_empty[i % RING]));
+            if (s + 1 < (w ? n1 : n0)) {
               const int in = i + 2;
-              good = mbar_wait(smem_u32(&k_full[in % RING]), (uint32_t)(in / RING & 1));
+              good = warp_wait(smem_u32(&k_full[in % RING]), (uint32_t)(in / RING & 1));
               if (!good) break;
               tc_fence_after();
               issue_s(w, in % RING);
-              tc_commit(smem_u32(&k_empty[in % RING]));
+              warp_commit(lead, smem_u32(&k_empty[in % RING]));
             }
           }
         }
       } else {
-        good = good && mbar_wait(smem_u32(&k_full[0]), 0);
+        good = good && warp_wait(smem_u32(&k_full[0]), 0);
         if (good) {
           tc_fence_after();
           for (int w = 0; w < 2; w++)
-            if (nt[w] > 0) issue_s(w, 0);
-          tc_commit(smem_u32(&k_empty[0]));
+            if ((w ? n1 : n0) > 0) issue_s(w, 0);
+          warp_commit(lead, smem_u32(&k_empty[0]));
         }
-        for (int i = 0; i < k.nt && good; i++) {
+        for (int i = 0; i < n_all && good; i++) {
           const int st = i % RING, in = (i + 1) % RING;
-          good = mbar_wait(smem_u32(&v_ready[st]), (uint32_t)(i / RING & 1));
+          good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)(i / RING & 1));
           bool k_next = false;
           for (int w = 0; w < 2 && good; w++) {
-            if (i < nt[w]) {
+            if (i < (w ? n1 : n0)) {
               good = issue_pv(w, st, i == 0, (uint32_t)(i & 1));
               if (!good) break;
             }
-            if (i + 1 < nt[w]) {
+            if (i + 1 < (w ? n1 : n0)) {
               if (!k_next) {
-                good = mbar_wait(smem_u32(&k_full[in]), (uint32_t)((i + 1) / RING & 1));
+                good = warp_wait(smem_u32(&k_full[in]), (uint32_t)((i + 1) / RING & 1));
                 if (!good) break;
                 tc_fence_after();
                 k_next = true;
@@ -288,14 +327,14 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
             }
           }
           if (!good) break;
-          tc_commit(smem_u32(&v_empty[st]));
-          if (i + 1 < k.nt) tc_commit(smem_u32(&k_empty[in]));
+          warp_commit(lead, smem_u32(&v_empty[st]));
+          if (i + 1 < n_all) warp_commit(lead, smem_u32(&k_empty[in]));
         }
       }
       if (!good) {  // what was issued has ended before the tiles are somebody else's
-        set_status(t.status, 43);
-        tc_commit(smem_u32(&bar_q));
-        mbar_wait(smem_u32(&bar_q), 1);
+        if (lane == 0) set_status(t.status, 43);
+        warp_commit(lead, smem_u32(&bar_q));
+        warp_wait(smem_u32(&bar_q), 1);
       }
     }
     __syncwarp();

@@ -35,7 +35,7 @@ struct TilesArgs {
   PagedJoin join;  // parts of the output: ONE: 2 * parts, otherwise parts
   int parts, ct;   // blocks that share the keys, tiles of a piece
   int G, tw;       // heads per key/value head, tokens of a tile of 128 rows
-  int64_t tiles;   // tiles of tokens in the grid
+  double inv_tb;   // 1 / tokens of a block
   int* status;
 };
 
@@ -111,6 +111,77 @@ constexpr int tiles_ring() { return QA == 1 ? 4 : ONE ? 3 : 2; }
 template <int QA, bool ONE>
 constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 2 * tiles_ring<QA, ONE>()) * QA * HALF_BYTES + 1024; }
 
+// The x-th unit of work, a tile of tb tokens of a sequence, in the order of falling positions (of the last token, by 128): the blocks with the most keys
+// start first, those of all sequences, and the short ones fill the SMs at the end. (Sequence by sequence, 4 prompts of 683 to 2048 tokens took 174 us
+// instead of TIME_LPT.) Nobody lists the units: how many of them end at position X or later is a sum over the sequences, so the level of the x-th is searched
+// for, and its sequence found in that level. False behind the last unit. A warp calls it together.
+struct UnitSeq {
+  int past, n, units;  // of sequence lane + 32 i: tokens before the new ones, new ones, tiles
+};
+__device__ __forceinline__ int units_from(const UnitSeq& u, int X, double inv_tb) {  // its units that end at X or later
+  if (X <= 0) return u.units;
+  if (u.past + u.n < X) return 0;
+  return u.units - (X > u.past ? (int)((X - u.past - 1 + 0.5) * inv_tb) : 0);  // (X - past - 1) / tb units end before
+}
+__device__ bool find_unit(const PagedView& v, int tb, double inv_tb, int x, int lane, int* b_out, int* tile_out) {
+  constexpr int KEEP = 4;  // sequences of a lane that stay in registers; more are read again each time
+  auto seq = [&](int b) {
+    UnitSeq u{0, 0, 0};
+    if (b < v.B) {
+      u.n = max(0, v.starts[b + 1] - v.starts[b]);
+      u.past = v.lens[b] - u.n;
+      u.units = (int)((u.n + tb - 1 + 0.5) * inv_tb);
+    }
+    return u;
+  };
+  UnitSeq kept[KEEP];
+#pragma unroll
+  for (int i = 0; i < KEEP; i++) kept[i] = seq(lane + 32 * i);
+  int top = 0;
+#pragma unroll
+  for (int i = 0; i < KEEP; i++)
+    if (kept[i].n) top = max(top, kept[i].past + kept[i].n);
+  for (int b = lane + 32 * KEEP; b < v.B; b += 32) {
+    const UnitSeq u = seq(b);
+    if (u.n) top = max(top, u.past + u.n);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  auto from = [&](int X) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) c += units_from(kept[i], X, inv_tb);
+    for (int b = lane + 32 * KEEP; b < v.B; b += 32) c += units_from(seq(b), X, inv_tb);
+    return __reduce_add_sync(0xffffffffu, c);
+  };
+  if (x >= from(0)) return false;
+  int lo = 0, hi = top / BKV + 1, below = 0;  // from(128 lo) > x >= from(128 hi) = below
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2, c = from(mid * BKV);
+    if (c > x) lo = mid;
+    else hi = mid, below = c;
+  }
+  int rest = x - below;
+  for (int b0 = 0; b0 < v.B; b0 += 32) {
+    const UnitSeq u = seq(b0 + lane);
+    const int first = u.units - units_from(u, lo * BKV, inv_tb), c = u.units - first - units_from(u, hi * BKV, inv_tb);
+    int sum = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const unsigned there = __ballot_sync(0xffffffffu, sum > rest);
+    if (there) {
+      const int src = __ffs(there) - 1;
+      *b_out = b0 + src;
+      *tile_out = __shfl_sync(0xffffffffu, first + rest - (sum - c), src);
+      return true;
+    }
+    rest -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
 template <int QA, bool ONE>
 __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TilesArgs t) {
@@ -128,27 +199,15 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   Work k;
   {
     const int per = a.Hkv * t.parts;
-    const int64_t x = t.tiles - 1 - blockIdx.x / per;  // the last tokens of a prompt see the most keys: they go first
     k.part = blockIdx.x % per / a.Hkv;
     k.hk = blockIdx.x % a.Hkv;
-    // tiles of sequence b begin at (starts[b] - starts[0]) / tokens of a block + b: room for all of them, found without a list
-    const int tb = NQ * t.tw, s0 = a.at.starts[0];
-    int before = 0;
-    for (int b0 = 0; b0 < a.at.B; b0 += 32) {
-      const int b = b0 + lane;
-      const unsigned m = __ballot_sync(0xffffffffu, b < a.at.B && (int64_t)(a.at.starts[min(b, a.at.B - 1)] - s0) / tb + b <= x);
-      before += __popc(m);
-      if (m != 0xffffffffu) break;
-    }
-    k.b = before - 1;
-    if (k.b < 0) return;
-    const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb;
-    const int64_t q0 = (x - ((int64_t)(sb - s0) / tb + k.b)) * tb;
-    if (q0 < 0 || q0 >= n_new || sb < 0 || (int64_t)sb + n_new > a.at.T) return;
+    int tile;
+    if (!find_unit(a.at, NQ * t.tw, t.inv_tb, blockIdx.x / per, lane, &k.b, &tile)) return;
+    const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb, len = a.at.lens[k.b], q0 = tile * NQ * t.tw;
+    if (sb < 0 || (int64_t)sb + n_new > a.at.T || q0 < 0 || q0 >= n_new) return;  // starts or lengths that are none
     k.row0 = sb + q0;
-    k.n = (int)min((int64_t)tb, n_new - q0);
-    const int len = a.at.lens[k.b];
-    k.lo_pos = len - n_new + (int)q0;
+    k.n = min(NQ * t.tw, n_new - q0);
+    k.lo_pos = len - n_new + q0;
     k.lo_key = a.window ? max(0, k.lo_pos - a.window + 1) : 0;
     k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
     k.nt = share_count(k.w.total, k.part, t.parts, t.ct);
@@ -167,17 +226,57 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, t.ct)) * BKV; };  // first key of the block's i-th tile
 
   const uint32_t sQ = smem_u32(smem), sK = sQ + NQ * TILE, sV = sK + RING * TILE;
-  if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&bar_q), 1);
-    for (int i = 0; i < RING; i++) {
-      mbar_init(smem_u32(&k_full[i]), 1); mbar_init(smem_u32(&k_empty[i]), 1);
-      mbar_init(smem_u32(&v_full[i]), 1); mbar_init(smem_u32(&v_ready[i]), 64); mbar_init(smem_u32(&v_empty[i]), 1);
+  // The copying warp sets up the barriers, requests what has room and meets the others at the barrier below.
+  const int box = min(a.at.page, BKV), boxes = BKV / box;  // keys of a box; boxes of a tile
+  int ready = 0;  // key and value tiles requested
+  auto page_of = [&](int i, int x) {
+    const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
+    return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
+  };
+  PageNames names;
+  unsigned there = 0;
+  auto copy_box = [&](const CUtensorMap* map, uint32_t tile, int i, int page, uint32_t bar) {
+    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(there) * box * 128 * QA));
+    __syncwarp();
+    if (page >= 0) {
+      const int row = (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
+      for (int x = 0; x < QA; x++) tma_load_2d(tile + x * HALF_BYTES + lane * box * 128, map, x * 64, row, bar);
     }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i][0]), BQ); mbar_init(smem_u32(&bar_p[i][1]), BQ); mbar_init(smem_u32(&bar_o[i]), 1);
+  };
+  auto copy_k = [&](int i) {
+    const int page = names.of(i, boxes, lane, page_of), st = i % RING;
+    there = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane == 0) page_bits[i & 7] = there;
+    copy_box(&map_k, sK + st * TILE, i, page, smem_u32(&k_full[st]));
+    return page;
+  };
+  auto copy_v = [&](int i, int page) { copy_box(&map_v, sV + i % RING * TILE, i, page, smem_u32(&v_full[i % RING])); };
+  if (warp == 9) {
+    if (lane == 0) {
+      mbar_init(smem_u32(&bar_q), 1);
+      for (int i = 0; i < RING; i++) {
+        mbar_init(smem_u32(&k_full[i]), 1); mbar_init(smem_u32(&k_empty[i]), 1);
+        mbar_init(smem_u32(&v_full[i]), 1); mbar_init(smem_u32(&v_ready[i]), 64); mbar_init(smem_u32(&v_empty[i]), 1);
+      }
+      for (int i = 0; i < 2; i++) {
+        mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i][0]), BQ); mbar_init(smem_u32(&bar_p[i][1]), BQ); mbar_init(smem_u32(&bar_o[i]), 1);
+      }
+      poison = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
     }
-    poison = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    if (k.nt > 0) {
+      names.begin(boxes, lane, page_of);
+      if (lane == 0) {
+        const uint32_t bytes = (uint32_t)(t.G * t.tw * 128 * QA);
+        const int nq = !ONE && nt[1] ? 2 : 1;
+        mbar_expect_tx(smem_u32(&bar_q), nq * bytes);
+        for (int w = 0; w < nq; w++)
+          for (int i = 0; i < QA; i++) tma_load_3d(sQ + w * TILE + i * HALF_BYTES, &map_q, i * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&bar_q));
+      }
+      __syncwarp();
+      for (; ready < min(k.nt, RING); ready++) copy_v(ready, copy_k(ready));
+    }
   }
   if (warp == 8) {
     __syncwarp();
@@ -191,52 +290,25 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   const uint32_t tmem = tmem_base_slot;
   constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-  const int box = min(a.at.page, BKV), boxes = BKV / box;  // keys of a box; boxes of a tile
 
   if (warp == 9) {
-    // ---- copies. Lane i looks up the i-th box of a tile, one tile ahead.
-    if (lane == 0 && k.nt > 0) {
-      const uint32_t bytes = (uint32_t)(t.G * t.tw * 128 * QA);
-      const int nq = !ONE && nt[1] ? 2 : 1;
-      mbar_expect_tx(smem_u32(&bar_q), nq * bytes);
-      for (int w = 0; w < nq; w++)
-        for (int i = 0; i < QA; i++) tma_load_3d(sQ + w * TILE + i * HALF_BYTES, &map_q, i * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&bar_q));
-    }
-    auto page_of = [&](int i, int x) {
-      const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
-      return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
-    };
-    PageNames names;
-    names.begin(boxes, lane, page_of);
-    int got = 0;
+    // ---- copies, the first of them requested already
     bool good = true;
-    for (int i = 0; i < k.nt; i++) {
-      const int page = names.of(i, boxes, lane, page_of), st = i % RING;
+    for (int i = ready; i < k.nt; i++) {
+      const int st = i % RING;
       const uint32_t ph = (uint32_t)(i / RING & 1) ^ 1;
-      const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-      const uint32_t bytes = (uint32_t)(__popc(there) * box * 128 * QA);
-      const int row = page < 0 ? 0 : (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
-      if (i >= RING) good = mbar_wait(smem_u32(&k_empty[st]), ph);
-      if (!__all_sync(0xffffffffu, good)) { if (lane == 0) set_status(t.status, 41); good = false; break; }
-      if (lane == 0) {
-        page_bits[i & 7] = there;
-        mbar_expect_tx(smem_u32(&k_full[st]), bytes);
-      }
-      __syncwarp();
-      if (page >= 0)
-        for (int x = 0; x < QA; x++) tma_load_2d(sK + st * TILE + x * HALF_BYTES + lane * box * 128, &map_k, x * 64, row, smem_u32(&k_full[st]));
-      if (i >= RING) good = mbar_wait(smem_u32(&v_empty[st]), ph);
-      if (!__all_sync(0xffffffffu, good)) { if (lane == 0) { set_status(t.status, 42); mbar_wait(smem_u32(&k_full[st]), ph ^ 1); } good = false; break; }
-      if (lane == 0) mbar_expect_tx(smem_u32(&v_full[st]), bytes);
-      __syncwarp();
-      if (page >= 0)
-        for (int x = 0; x < QA; x++) tma_load_2d(sV + st * TILE + x * HALF_BYTES + lane * box * 128, &map_v, x * 64, row, smem_u32(&v_full[st]));
-      got = i + 1;
+      good = warp_wait(smem_u32(&k_empty[st]), ph);
+      if (!good) { if (lane == 0) set_status(t.status, 41); break; }
+      const int page = copy_k(i);
+      good = warp_wait(smem_u32(&v_empty[st]), ph);
+      if (!good) { if (lane == 0) { set_status(t.status, 42); mbar_wait(smem_u32(&k_full[st]), ph ^ 1); } break; }
+      copy_v(i, page);
+      ready = i + 1;
     }
     // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
     if (lane == 0 && k.nt > 0) {
       mbar_wait(smem_u32(&bar_q), 0);
-      for (int i = max(0, got - RING); i < got; i++) {
+      for (int i = max(0, ready - RING); i < ready; i++) {
         mbar_wait(smem_u32(&k_full[i % RING]), (uint32_t)(i / RING & 1));
         mbar_wait(smem_u32(&v_full[i % RING]), (uint32_t)(i / RING & 1));
       }
@@ -391,11 +463,19 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
       tc_fence_after();
       if (any_live) {
         uint32_t r[BKV];
-#pragma unroll
-        for (int c = 0; c < 4; c++) tc_ld32(tS + lane_base + (uint32_t)(c * 32), r + c * 32);
+        tc_ld32(tS + lane_base, r);
+        tc_ld32(tS + lane_base + 32, r + 32);
         const int k0 = tile_key(i);
         const uint32_t bits = page_bits[i & 7];
         const bool full = bits == (1u << boxes) - 1 && sees_all(a, k.w.end, k0, BKV, pos_a, pos_b);
+        tc_wait_ld();
+        tc_ld32(tS + lane_base + 64, r + 64);  // on their way while the maximum of the first half is taken
+        tc_ld32(tS + lane_base + 96, r + 96);
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (full) {
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+        }
         tc_wait_ld();
         if (!full) {
           // keys [0, hi) of the tile without [first, lo) and without pages that are not there
@@ -410,10 +490,11 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
             for (int j = 0; j < 32; j++)
               if (!(see >> j & 1)) r[c * 32 + j] = 0xFF800000u;  // -inf
           }
-        }
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < BKV; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+          for (int j = 0; j < 64; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+        }
+#pragma unroll
+        for (int j = 64; j < BKV; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
         const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale_log2;
         const bool grow = m_tile > m_run + 8.0f;
         const float m_use = grow ? m_tile : m_run;
@@ -480,6 +561,10 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
       const float inv = split ? 1.f : l_run == 0.f ? 0.f : 1.0f / l_run;
       if (split && live) t.join.ml[at * np + p] = make_float2(m_run, l_run);
       const bool bad = *(volatile int*)&poison;
+      // Finished rows go through the queries' place in shared memory, which nobody reads any more, so that a warp's stores are whole rows (a thread per row
+      // and store is 32 lines for 512 bytes: 4700 cycles of a block).
+      uint4* stage = (uint4*)(smem + (ONE ? 0 : w * TILE)) + (row & ~31) * (D / 8);  // 32 rows of this warp, chunk c of row r at c ^ (r & 7)
+      if (!split && nt[w] == 0 && k.nt > 0) mbar_wait(smem_u32(&bar_q), 0);  // the queries have come there
 #pragma unroll 1
       for (int c = 0; c < 2 * QA; c++) {
         uint32_t r[32];
@@ -488,22 +573,22 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
           tc_ld32(tO + lane_base + (uint32_t)(c * 32), r);
           tc_wait_ld();
         }
-        if (!live || (split && l_run == 0.f)) continue;
         if (l_run == 0.f) {
 #pragma unroll
           for (int j = 0; j < 32; j++) r[j] = 0;
-        } else if (bad) {
+        } else if (bad && live) {
           float f[32];
           for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
           add_poison(a, k.w, k.b, k.hk, k.part, t.parts, t.ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt[w], pos, c * 32, 32, f);
           for (int j = 0; j < 32; j++) r[j] = __float_as_uint(f[j]);
         }
         if (split) {
-          float* dst = t.join.o + (at * np + p) * D + c * 32;
+          if (live && l_run != 0.f) {
+            float* dst = t.join.o + (at * np + p) * D + c * 32;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *(uint4*)(dst + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            for (int j = 0; j < 32; j += 4) *(uint4*)(dst + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+          }
         } else {
-          bf16* dst = a.out + at * D + c * 32;
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 v;
@@ -511,8 +596,20 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
             v.y = f32_to_bf16_bits(__uint_as_float(r[j + 2]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 3]) * inv) << 16);
             v.z = f32_to_bf16_bits(__uint_as_float(r[j + 4]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 5]) * inv) << 16);
             v.w = f32_to_bf16_bits(__uint_as_float(r[j + 6]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 7]) * inv) << 16);
-            *(uint4*)(dst + j) = v;
+            stage[lane * (D / 8) + ((c * 4 + j / 8) ^ (lane & 7))] = v;
           }
+        }
+      }
+      if (!split) {
+        __syncwarp();
+        constexpr int LANES = D / 8, PASS = 32 / LANES;  // lanes of a row, rows of a pass
+#pragma unroll 4
+        for (int x = 0; x < 32; x += PASS) {
+          const int rr = x + lane / LANES, cc = lane % LANES;
+          const int64_t to = __shfl_sync(0xffffffffu, at, rr);
+          const bool on = __shfl_sync(0xffffffffu, (int)live, rr);
+          const uint4 v = stage[rr * LANES + (cc ^ (rr & 7))];
+          if (on) *(uint4*)(a.out + to * D + cc * 8) = v;
         }
       }
     }
@@ -547,7 +644,8 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   t.tw = BQ / t.G;
   t.status = ctx->d_status;
   const int tb = (ONE ? 1 : 2) * t.tw;
-  t.tiles = a.at.T / tb + a.at.B;
+  t.inv_tb = 1.0 / tb;
+  const int64_t tiles = a.at.T / tb + a.at.B;  // room for the tiles of all sequences
   // Parts: the fewest rounds of key tiles over the SMs, a block counted with three tiles more (its start and its end) and the join with four.
   const int64_t units = std::max<int64_t>((a.at.T + tb - 1) / tb, a.at.B) * a.Hkv, keys = std::max<int64_t>(1, paged_walk_tiles(a, BKV));
   int64_t best = INT64_MAX;
@@ -560,7 +658,7 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   t.ct = (int)((keys + t.parts - 1) / t.parts);
   const int np = (ONE ? 2 : 1) * t.parts;
   if (np > 1) SB_TRY(paged_join_scratch(ctx, a, np, &t.join));
-  const int64_t blocks = t.tiles * a.Hkv * t.parts;
+  const int64_t blocks = tiles * a.Hkv * t.parts;
   if (blocks > INT32_MAX) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "attention: too many rows and heads for one call");
   CUtensorMap mq, mk, mv;
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;

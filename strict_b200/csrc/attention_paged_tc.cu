@@ -7,8 +7,10 @@
 //   softmax        a thread per row, running maximum followed lazily (a row of O is rescaled when its maximum grew by more than 2^8), weights back to
 //                  tensor memory as two bf16 terms (hi + lo by truncation: 2^-16)
 //   O += P V       weights from tensor memory, values from shared memory; O stays in tensor memory
-// Roles: warps 0..7 softmax, 8 issues products, 9 copies, 10 and 11 look over values. A block works on two things in turn, so that the tensor
-// pipe runs one while the softmax warps are at the other:
+// Blocks stay (one per SM) and take one unit after the other: a tile of tokens, a key/value head and a share of the keys. Roles: warps 0..7 softmax, 8 issues
+// products, 9 finds units, announces them (two ahead of the slowest) and copies, 10 and 11 look over values. They meet at mbarriers only, so the copies and
+// first products of a unit run while the last one's rows are being written. (A block per unit cost 13 us a unit beside 2.5 us a key tile.) A block
+// works on two things in turn, so that the tensor pipe runs one while the softmax warps are at the other:
 //   two tiles (ONE = false)   A and B, 2 * (128 / G) consecutive tokens, sharing every key tile
 //   one tile (ONE = true)     few rows: the even and the odd key tiles of the same queries, each with a softmax of its own; joined later
 // Keys may be split further over `parts` blocks. Whatever is split leaves (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel.
@@ -35,19 +37,20 @@ struct TilesArgs {
   PagedJoin join;  // parts of the output: ONE: 2 * parts, otherwise parts
   int parts, ct;   // blocks that share the keys, tiles of a piece
   int G, tw;       // heads per key/value head, tokens of a tile of 128 rows
-  double inv_tb;   // 1 / tokens of a block
+  double inv_tb;   // 1 / tokens of a unit
   int* status;
 };
 
-// What a block works on, the same in all of its threads.
-struct Work {
+// What a block works on.
+struct Unit {
   int b, hk, part;
-  int64_t row0;          // first row in q and out
-  int n;                 // tokens
-  int lo_pos;            // position of the first token
-  int lo_key;            // first key in the window of the first token
+  int n;       // tokens; -1: there is no further unit
+  int lo_pos;  // position of the first token
+  int lo_key;  // first key in the window of the first token
+  int64_t row0;  // first row in q and out
   PagedWalk w;
-  int nt;                // key tiles of this block
+  int nt, nt_w[2];  // key tiles of the unit and of each stream
+  int poison;       // values that are not finite were replaced
 };
 
 // What the issuing warp executes as a whole, one lane of it acting: operands that the compiler knows to be the same in all lanes need not be moved to
@@ -109,12 +112,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <int QA, bool ONE>
 constexpr int tiles_ring() { return QA == 1 ? 4 : ONE ? 3 : 2; }
 template <int QA, bool ONE>
-constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 2 * tiles_ring<QA, ONE>()) * QA * HALF_BYTES + 1024; }
+constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 2 * tiles_ring<QA, ONE>()) * QA * HALF_BYTES + (ONE ? 0 : 8 * 4096) + 1024; }
 
-// The x-th unit of work, a tile of tb tokens of a sequence, in the order of falling positions (of the last token, by 128): the blocks with the most keys
-// start first, those of all sequences, and the short ones fill the SMs at the end. (Sequence by sequence, 4 prompts of 683 to 2048 tokens took 174 us
-// instead of TIME_LPT.) Nobody lists the units: how many of them end at position X or later is a sum over the sequences, so the level of the x-th is searched
-// for, and its sequence found in that level. False behind the last unit. A warp calls it together.
+// The x-th unit of work, a tile of tb tokens of a sequence, in the order of falling positions (of the last token, by 128): those with the most keys come
+// first, of all sequences, and the short ones fill the SMs at the end. Nobody lists the units: how many of them end at position X or later is a sum over
+// the sequences, so the level of the x-th is searched for, and its sequence found in that level. False behind the last unit. A warp calls it together.
 struct UnitSeq {
   int past, n, units;  // of sequence lane + 32 i: tokens before the new ones, new ones, tiles
 };
@@ -183,103 +185,35 @@ __device__ bool find_unit(const PagedView& v, int tb, double inv_tb, int x, int 
 }
 
 template <int QA, bool ONE>
-__global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TilesArgs t) {
   constexpr int TILE = QA * HALF_BYTES, NQ = ONE ? 1 : 2, D = 64 * QA, RING = tiles_ring<QA, ONE>();
+  constexpr int READERS = 11;  // warps that read a unit's description
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t bar_q, k_full[RING], k_empty[RING], v_full[RING], v_ready[RING], v_empty[RING], bar_s[2], bar_p[2][2], bar_o[2];
+  __shared__ __align__(8) uint64_t unit_full[2], unit_empty[2], q_full, q_empty, k_full[RING], k_empty[RING], v_full[RING], v_ready[RING], v_empty[RING], bar_s[2],
+      bar_p[2][2], bar_o[2], o_free[2];
+  __shared__ Unit units[2];
   __shared__ uint32_t tmem_base_slot;
   __shared__ uint32_t page_bits[8];  // pages of a key tile that are there
-  __shared__ int poison;
   const PagedAttnArgs& a = t.a;
-  pdl_wait();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-
-  Work k;
-  {
-    const int per = a.Hkv * t.parts;
-    k.part = blockIdx.x % per / a.Hkv;
-    k.hk = blockIdx.x % a.Hkv;
-    int tile;
-    if (!find_unit(a.at, NQ * t.tw, t.inv_tb, blockIdx.x / per, lane, &k.b, &tile)) return;
-    const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb, len = a.at.lens[k.b], q0 = tile * NQ * t.tw;
-    if (sb < 0 || (int64_t)sb + n_new > a.at.T || q0 < 0 || q0 >= n_new) return;  // starts or lengths that are none
-    k.row0 = sb + q0;
-    k.n = min(NQ * t.tw, n_new - q0);
-    k.lo_pos = len - n_new + q0;
-    k.lo_key = a.window ? max(0, k.lo_pos - a.window + 1) : 0;
-    k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
-    k.nt = share_count(k.w.total, k.part, t.parts, t.ct);
-  }
-  // key tiles of each stream: ONE: every other one; otherwise tile A ends where its last token does
-  int nt[2];
-  if (ONE) {
-    nt[0] = (k.nt + 1) / 2;
-    nt[1] = k.nt / 2;
-  } else {
-    const int end_a = max(0, min(k.w.end, k.lo_pos + min(k.n, t.tw)));
-    nt[0] = min(k.nt, share_count(k.w.first + max(0, (end_a + BKV - 1) / BKV - k.w.lo), k.part, t.parts, t.ct));
-    nt[1] = k.n > t.tw ? k.nt : 0;
-    k.nt = max(nt[0], nt[1]);
-  }
-  auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, t.ct)) * BKV; };  // first key of the block's i-th tile
-
   const uint32_t sQ = smem_u32(smem), sK = sQ + NQ * TILE, sV = sK + RING * TILE;
-  // The copying warp sets up the barriers, requests what has room and meets the others at the barrier below.
-  const int box = min(a.at.page, BKV), boxes = BKV / box;  // keys of a box; boxes of a tile
-  int ready = 0;  // key and value tiles requested
-  auto page_of = [&](int i, int x) {
-    const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
-    return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
-  };
-  PageNames names;
-  unsigned there = 0;
-  auto copy_box = [&](const CUtensorMap* map, uint32_t tile, int i, int page, uint32_t bar) {
-    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(there) * box * 128 * QA));
-    __syncwarp();
-    if (page >= 0) {
-      const int row = (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
-      for (int x = 0; x < QA; x++) tma_load_2d(tile + x * HALF_BYTES + lane * box * 128, map, x * 64, row, bar);
+  if (warp == 9 && lane == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&unit_full[i]), 1); mbar_init(smem_u32(&unit_empty[i]), READERS);
+      mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i][0]), BQ); mbar_init(smem_u32(&bar_p[i][1]), BQ); mbar_init(smem_u32(&bar_o[i]), 1);
+      mbar_init(smem_u32(&o_free[i]), BQ);
     }
-  };
-  auto copy_k = [&](int i) {
-    const int page = names.of(i, boxes, lane, page_of), st = i % RING;
-    there = __ballot_sync(0xffffffffu, page >= 0);
-    if (lane == 0) page_bits[i & 7] = there;
-    copy_box(&map_k, sK + st * TILE, i, page, smem_u32(&k_full[st]));
-    return page;
-  };
-  auto copy_v = [&](int i, int page) { copy_box(&map_v, sV + i % RING * TILE, i, page, smem_u32(&v_full[i % RING])); };
-  if (warp == 9) {
-    if (lane == 0) {
-      mbar_init(smem_u32(&bar_q), 1);
-      for (int i = 0; i < RING; i++) {
-        mbar_init(smem_u32(&k_full[i]), 1); mbar_init(smem_u32(&k_empty[i]), 1);
-        mbar_init(smem_u32(&v_full[i]), 1); mbar_init(smem_u32(&v_ready[i]), 64); mbar_init(smem_u32(&v_empty[i]), 1);
-      }
-      for (int i = 0; i < 2; i++) {
-        mbar_init(smem_u32(&bar_s[i]), 1); mbar_init(smem_u32(&bar_p[i][0]), BQ); mbar_init(smem_u32(&bar_p[i][1]), BQ); mbar_init(smem_u32(&bar_o[i]), 1);
-      }
-      poison = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    mbar_init(smem_u32(&q_full), 1); mbar_init(smem_u32(&q_empty), 1);
+    for (int i = 0; i < RING; i++) {
+      mbar_init(smem_u32(&k_full[i]), 1); mbar_init(smem_u32(&k_empty[i]), 1);
+      mbar_init(smem_u32(&v_full[i]), 1); mbar_init(smem_u32(&v_ready[i]), 64); mbar_init(smem_u32(&v_empty[i]), 1);
     }
-    __syncwarp();
-    if (k.nt > 0) {
-      names.begin(boxes, lane, page_of);
-      if (lane == 0) {
-        const uint32_t bytes = (uint32_t)(t.G * t.tw * 128 * QA);
-        const int nq = !ONE && nt[1] ? 2 : 1;
-        mbar_expect_tx(smem_u32(&bar_q), nq * bytes);
-        for (int w = 0; w < nq; w++)
-          for (int i = 0; i < QA; i++) tma_load_3d(sQ + w * TILE + i * HALF_BYTES, &map_q, i * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&bar_q));
-      }
-      __syncwarp();
-      for (; ready < min(k.nt, RING); ready++) copy_v(ready, copy_k(ready));
-    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  pdl_wait();
   if (warp == 8) {
-    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -290,109 +224,196 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
   const uint32_t tmem = tmem_base_slot;
   constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  const int box = min(a.at.page, BKV), boxes = BKV / box;  // keys of a box; boxes of a tile
+  // A count of phases over all units gives each wait its parity. next_unit: the description of the u-th unit, false behind the last or after a wait that gave up.
+  auto next_unit = [&](int u) { return warp_wait(smem_u32(&unit_full[u & 1]), (uint32_t)(u >> 1 & 1)) && units[u & 1].n >= 0; };
+  auto unit_read = [&](int u) {
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&unit_empty[u & 1])) : "memory");
+  };
 
-  if (warp == 9) {
-    // ---- copies, the first of them requested already
+  // Registers: 384 threads begin with 168 each; the softmax warps end up with 216, the others with 72 (256 * 216 + 128 * 72 = 384 * 168).
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 9) {
+    // ---- units and copies
+    int c = 0, nq = 0;  // key tiles, units with keys
     bool good = true;
-    for (int i = ready; i < k.nt; i++) {
-      const int st = i % RING;
-      const uint32_t ph = (uint32_t)(i / RING & 1) ^ 1;
-      good = warp_wait(smem_u32(&k_empty[st]), ph);
-      if (!good) { if (lane == 0) set_status(t.status, 41); break; }
-      const int page = copy_k(i);
-      good = warp_wait(smem_u32(&v_empty[st]), ph);
-      if (!good) { if (lane == 0) { set_status(t.status, 42); mbar_wait(smem_u32(&k_full[st]), ph ^ 1); } break; }
-      copy_v(i, page);
-      ready = i + 1;
-    }
-    // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
-    if (lane == 0 && k.nt > 0) {
-      mbar_wait(smem_u32(&bar_q), 0);
-      for (int i = max(0, ready - RING); i < ready; i++) {
-        mbar_wait(smem_u32(&k_full[i % RING]), (uint32_t)(i / RING & 1));
-        mbar_wait(smem_u32(&v_full[i % RING]), (uint32_t)(i / RING & 1));
+    for (int u = 0; good; u++) {
+      // every other round of the blocks goes backwards: who had the longest of one has the shortest of the next
+      const int64_t y = (int64_t)u * gridDim.x + (u & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const int per = a.Hkv * t.parts;
+      Unit k;
+      k.n = -1;
+      k.nt = 0;
+      int tile;
+      if (find_unit(a.at, NQ * t.tw, t.inv_tb, (int)(y / per), lane, &k.b, &tile)) {
+        k.part = (int)(y % per) / a.Hkv;
+        k.hk = (int)(y % per) % a.Hkv;
+        const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb, len = a.at.lens[k.b], q0 = tile * NQ * t.tw;
+        k.row0 = (int64_t)sb + q0;
+        k.lo_pos = len - n_new + q0;
+        k.lo_key = a.window ? max(0, k.lo_pos - a.window + 1) : 0;
+        k.n = sb < 0 || (int64_t)sb + n_new > a.at.T || q0 < 0 ? 0 : max(0, min(NQ * t.tw, n_new - q0));  // nothing where starts or lengths are none
+        k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
+        k.nt = k.n ? share_count(k.w.total, k.part, t.parts, t.ct) : 0;
+        if (ONE) {  // every other tile
+          k.nt_w[0] = (k.nt + 1) / 2;
+          k.nt_w[1] = k.nt / 2;
+        } else {    // tile A ends where its last token does
+          const int end_a = max(0, min(k.w.end, k.lo_pos + min(k.n, t.tw)));
+          k.nt_w[0] = min(k.nt, share_count(k.w.first + max(0, (end_a + BKV - 1) / BKV - k.w.lo), k.part, t.parts, t.ct));
+          k.nt_w[1] = k.n > t.tw ? k.nt : 0;
+          k.nt = max(k.nt_w[0], k.nt_w[1]);
+        }
+        k.poison = 0;
+      }
+      if (u >= 2) good = warp_wait(smem_u32(&unit_empty[u & 1]), (uint32_t)(u >> 1 & 1) ^ 1);
+      if (!good) break;
+      if (lane == 0) {
+        units[u & 1] = k;
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&unit_full[u & 1])) : "memory");
+      }
+      __syncwarp();
+      if (k.n < 0) break;
+      if (k.nt == 0) continue;
+      auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, t.ct)) * BKV; };
+      auto page_of = [&](int i, int x) {
+        const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
+        return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
+      };
+      auto copy_boxes = [&](const CUtensorMap* map, uint32_t tile, int row, unsigned there, uint32_t bar) {
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(there) * box * 128 * QA));
+        __syncwarp();
+        if (row >= 0)
+          for (int x = 0; x < QA; x++) tma_load_2d(tile + x * HALF_BYTES + lane * box * 128, map, x * 64, row, bar);
+      };
+      PageNames names;
+      names.begin(boxes, lane, page_of);
+      for (int i = 0; i < k.nt; i++, c++) {
+        const int st = c % RING, page = names.of(i, boxes, lane, page_of);
+        const uint32_t ph = (uint32_t)(c / RING & 1) ^ 1;
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+        const int row = page < 0 ? -1 : (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
+        if (c >= RING) good = warp_wait(smem_u32(&k_empty[st]), ph);
+        if (!good) break;
+        if (lane == 0) page_bits[c & 7] = there;
+        copy_boxes(&map_k, sK + st * TILE, row, there, smem_u32(&k_full[st]));
+        if (i == 0) {
+          if (nq) good = warp_wait(smem_u32(&q_empty), (uint32_t)(nq & 1) ^ 1);
+          if (good && lane == 0) {
+            const int tiles = !ONE && k.nt_w[1] ? 2 : 1;
+            mbar_expect_tx(smem_u32(&q_full), (uint32_t)(tiles * t.G * t.tw * 128 * QA));
+            for (int w = 0; w < tiles; w++)
+              for (int x = 0; x < QA; x++) tma_load_3d(sQ + w * TILE + x * HALF_BYTES, &map_q, x * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&q_full));
+          }
+          if (good) nq++;
+        }
+        if (good && c >= RING) good = warp_wait(smem_u32(&v_empty[st]), ph);
+        if (!good) {
+          warp_wait(smem_u32(&k_full[st]), ph ^ 1);  // landed before this block's memory is somebody else's
+          break;
+        }
+        copy_boxes(&map_v, sV + st * TILE, row, there, smem_u32(&v_full[st]));
       }
     }
-    __syncwarp();
-  } else if (warp == 8) {
+    if (!good && lane == 0) set_status(t.status, 41);
+    // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
+    if (nq) warp_wait(smem_u32(&q_full), (uint32_t)(nq & 1) ^ 1);
+    for (int i = max(0, c - RING); i < c; i++) {
+      warp_wait(smem_u32(&k_full[i % RING]), (uint32_t)(i / RING & 1));
+      warp_wait(smem_u32(&v_full[i % RING]), (uint32_t)(i / RING & 1));
+    }
+    } else if (warp == 8) {
     // ---- products
-    const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0), n_all = __shfl_sync(0xffffffffu, k.nt, 0);
-    if (n_all > 0) {
-      const uint32_t lead = elected();
-      auto issue_s = [&](int w, int st) {
-        const uint32_t tS = tmem + (uint32_t)(w * 256);
+    const uint32_t lead = elected();
+    auto issue_s = [&](int w, int st) {
+      const uint32_t tS = tmem + (uint32_t)(w * 256);
 #pragma unroll
-        for (int s = 0; s < 4 * QA; s++) {
-          const uint32_t off = (uint32_t)((s >> 2) * HALF_BYTES + (s & 3) * 32);
-          warp_mma_ss(lead, tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
-        }
-        warp_commit(lead, smem_u32(&bar_s[w]));
-      };
-      auto issue_pv = [&](int w, int st, bool first, uint32_t ph) {  // by halves of the keys, as their weights come
-        const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
+      for (int s = 0; s < 4 * QA; s++) {
+        const uint32_t off = (uint32_t)((s >> 2) * HALF_BYTES + (s & 3) * 32);
+        warp_mma_ss(lead, tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
+      }
+      warp_commit(lead, smem_u32(&bar_s[w]));
+    };
+    auto issue_pv = [&](int w, int st, bool first, uint32_t ph) {  // by halves of the keys, as their weights come
+      const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
 #pragma unroll
-        for (int s = 0; s < 8; s++) {
-          if ((s & 3) == 0) {
-            if (!warp_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
-            tc_fence_after();
-          }
-          const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
-          const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
-          warp_mma_ts(lead, tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
-          warp_mma_ts(lead, tO, tS + pcol + 16, dv, idesc_pv, 1u);
+      for (int s = 0; s < 8; s++) {
+        if ((s & 3) == 0) {
+          if (!warp_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
+          tc_fence_after();
         }
-        warp_commit(lead, smem_u32(&bar_o[w]));
-        return true;
+        const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
+        const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
+        warp_mma_ts(lead, tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
+        warp_mma_ts(lead, tO, tS + pcol + 16, dv, idesc_pv, 1u);
+      }
+      warp_commit(lead, smem_u32(&bar_o[w]));
+      return true;
+    };
+    int c = 0, nq = 0, step0 = 0, step1 = 0, used0 = 0, used1 = 0;  // key tiles, units with keys; steps and units of each stream
+    bool good = true;
+    for (int u = 0; good && next_unit(u); u++) {
+      const int n_all = __shfl_sync(0xffffffffu, units[u & 1].nt, 0), n0 = __shfl_sync(0xffffffffu, units[u & 1].nt_w[0], 0),
+                n1 = __shfl_sync(0xffffffffu, units[u & 1].nt_w[1], 0);
+      unit_read(u);
+      if (n_all == 0) continue;
+      // O of a stream belongs to the last unit until its rows have been read
+      auto o_mine = [&](int w) { return (w ? used1 : used0) == 0 || warp_wait(smem_u32(&o_free[w]), (uint32_t)((w ? used1 : used0) & 1) ^ 1); };
+      auto k_there = [&](int i) {
+        const bool ok = warp_wait(smem_u32(&k_full[(c + i) % RING]), (uint32_t)((c + i) / RING & 1));
+        tc_fence_after();
+        return ok;
       };
-      bool good = warp_wait(smem_u32(&bar_q), 0);
+      good = warp_wait(smem_u32(&q_full), (uint32_t)(nq & 1));
       if (ONE) {
         for (int w = 0; w < 2 && good; w++) {
           if ((w ? n1 : n0) == 0) break;
-          good = warp_wait(smem_u32(&k_full[w]), 0);
+          good = k_there(w);
           if (!good) break;
-          tc_fence_after();
-          issue_s(w, w);
-          warp_commit(lead, smem_u32(&k_empty[w]));
+          issue_s(w, (c + w) % RING);
+          warp_commit(lead, smem_u32(&k_empty[(c + w) % RING]));
+          if (w == n_all - 1) warp_commit(lead, smem_u32(&q_empty));
         }
         for (int s = 0; s < n0 && good; s++) {
           for (int w = 0; w < 2 && good; w++) {
             if (s >= (w ? n1 : n0)) break;
-            const int i = 2 * s + w;
-            good = warp_wait(smem_u32(&v_ready[i % RING]), (uint32_t)(i / RING & 1)) && issue_pv(w, i % RING, s == 0, (uint32_t)(s & 1));
+            const int i = 2 * s + w, st = (c + i) % RING;
+            good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)((c + i) / RING & 1)) && (s || o_mine(w)) &&
+                   issue_pv(w, st, s == 0, (uint32_t)((w ? step1 : step0) + s & 1));
             if (!good) break;
-            warp_commit(lead, smem_u32(&v_empty[i % RING]));
+            warp_commit(lead, smem_u32(&v_empty[st]));
             if (s + 1 < (w ? n1 : n0)) {
-              const int in = i + 2;
-              good = warp_wait(smem_u32(&k_full[in % RING]), (uint32_t)(in / RING & 1));
+              good = k_there(i + 2);
               if (!good) break;
-              tc_fence_after();
-              issue_s(w, in % RING);
-              warp_commit(lead, smem_u32(&k_empty[in % RING]));
+              issue_s(w, (c + i + 2) % RING);
+              warp_commit(lead, smem_u32(&k_empty[(c + i + 2) % RING]));
+              if (i + 2 == n_all - 1) warp_commit(lead, smem_u32(&q_empty));
             }
           }
         }
       } else {
-        good = good && warp_wait(smem_u32(&k_full[0]), 0);
+        good = good && k_there(0);
         if (good) {
-          tc_fence_after();
           for (int w = 0; w < 2; w++)
-            if ((w ? n1 : n0) > 0) issue_s(w, 0);
-          warp_commit(lead, smem_u32(&k_empty[0]));
+            if ((w ? n1 : n0) > 0) issue_s(w, c % RING);
+          warp_commit(lead, smem_u32(&k_empty[c % RING]));
+          if (n_all == 1) warp_commit(lead, smem_u32(&q_empty));
         }
         for (int i = 0; i < n_all && good; i++) {
-          const int st = i % RING, in = (i + 1) % RING;
-          good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)(i / RING & 1));
+          const int st = (c + i) % RING, in = (c + i + 1) % RING;
+          good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)((c + i) / RING & 1));
           bool k_next = false;
           for (int w = 0; w < 2 && good; w++) {
             if (i < (w ? n1 : n0)) {
-              good = issue_pv(w, st, i == 0, (uint32_t)(i & 1));
+              good = (i || o_mine(w)) && issue_pv(w, st, i == 0, (uint32_t)((w ? step1 : step0) + i & 1));
               if (!good) break;
             }
             if (i + 1 < (w ? n1 : n0)) {
               if (!k_next) {
-                good = warp_wait(smem_u32(&k_full[in]), (uint32_t)((i + 1) / RING & 1));
+                good = k_there(i + 1);
                 if (!good) break;
-                tc_fence_after();
                 k_next = true;
               }
               issue_s(w, in);
@@ -401,219 +422,266 @@ __global__ void __launch_bounds__(THREADS) attn_paged_tiles_kernel(const __grid_
           if (!good) break;
           warp_commit(lead, smem_u32(&v_empty[st]));
           if (i + 1 < n_all) warp_commit(lead, smem_u32(&k_empty[in]));
+          if (i + 2 == n_all) warp_commit(lead, smem_u32(&q_empty));
         }
       }
-      if (!good) {  // what was issued has ended before the tiles are somebody else's
-        if (lane == 0) set_status(t.status, 43);
-        warp_commit(lead, smem_u32(&bar_q));
-        warp_wait(smem_u32(&bar_q), 1);
-      }
+      c += n_all;
+      nq++;
+      step0 += n0;
+      step1 += n1;
+      used0 += n0 > 0;
+      used1 += n1 > 0;
     }
-    __syncwarp();
-  } else if (warp >= 10) {
+    if (!good) {  // what was issued has ended before the tiles are somebody else's
+      if (lane == 0) set_status(t.status, 43);
+      warp_commit(lead, smem_u32(&k_empty[0]));
+      for (int i = 0; i < 2; i++) warp_wait(smem_u32(&k_empty[0]), (uint32_t)i);
+    }
+    } else {
     // ---- values of tiles that not every row sees whole
     const int tid = (int)threadIdx.x - 10 * 32;
+    int c = 0;
     bool good = true;
-    for (int i = 0; i < k.nt && good; i++) {
-      const int st = i % RING, k0 = tile_key(i);
-      good = mbar_wait(smem_u32(&v_full[st]), (uint32_t)(i / RING & 1));
-      if (!good) break;
-      const uint32_t bits = page_bits[i & 7];
-      if (bits != (1u << boxes) - 1 || !sees_all(a, k.w.end, k0, BKV, k.lo_pos, k.lo_pos + k.n - 1)) {
-        uint32_t found = 0;
-        uint4* v = (uint4*)(smem + (NQ + RING + st) * TILE);
-        for (int x = tid; x < QA * BKV * 8; x += 64) {
-          const int r = (x >> 3) & (BKV - 1), j = k0 + r;
-          const bool seen = j < k.w.end && (bits >> (r / box) & 1) && (j >= k.lo_key || j < a.first);
-          if (!seen) {
-            v[x] = make_uint4(0, 0, 0, 0);
-            continue;
+    for (int u = 0; good && next_unit(u); u++) {
+      Unit& k = units[u & 1];
+      const PagedWalk w = k.w;
+      const int nt = k.nt, part = k.part, lo_pos = k.lo_pos, hi_pos = k.lo_pos + k.n - 1, lo_key = k.lo_key;
+      for (int i = 0; i < nt; i++, c++) {
+        const int st = c % RING, k0 = w.tile(share_tile(i, part, t.parts, t.ct)) * BKV;
+        good = warp_wait(smem_u32(&v_full[st]), (uint32_t)(c / RING & 1));
+        if (!good) break;
+        const uint32_t bits = page_bits[c & 7];
+        if (bits != (1u << boxes) - 1 || !sees_all(a, w.end, k0, BKV, lo_pos, hi_pos)) {
+          uint32_t found = 0;
+          uint4* v = (uint4*)(smem + (NQ + RING + st) * TILE);
+#pragma unroll 4
+          for (int x = tid; x < QA * BKV * 8; x += 64) {
+            const int r = (x >> 3) & (BKV - 1), j = k0 + r;
+            const bool seen = j < w.end && (bits >> (r / box) & 1) && (j >= lo_key || j < a.first);
+            const uint4 y = v[x];
+            if (!seen) {
+              v[x] = make_uint4(0, 0, 0, 0);
+            } else if (not_finite(y.x) | not_finite(y.y) | not_finite(y.z) | not_finite(y.w)) {
+              v[x] = make_uint4(only_finite(y.x), only_finite(y.y), only_finite(y.z), only_finite(y.w));
+              found = 1;
+            }
           }
-          const uint4 w = v[x];
-          if (not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w)) {
-            v[x] = make_uint4(only_finite(w.x), only_finite(w.y), only_finite(w.z), only_finite(w.w));
-            found = 1;
-          }
+          if (found) k.poison = 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (found) poison = 1;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&v_ready[st])) : "memory");
       }
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&v_ready[st])) : "memory");
+      unit_read(u);
     }
     if (!good && lane == 0) set_status(t.status, 44);
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax of stream w, a thread per row: its 128 scores stay in registers between the maximum and the exponentials
     const int w = warp >> 2, row = (int)threadIdx.x & (BQ - 1);
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
-    const int tok = row / t.G + (ONE ? 0 : w * t.tw);
-    const bool live = row < t.G * t.tw && tok < k.n;
-    const bool any_live = __any_sync(0xffffffffu, live);  // a warp without rows only keeps step
-    const int pos_a = k.lo_pos + (ONE ? 0 : w * t.tw), pos_b = k.lo_pos + min(k.n, (ONE ? 1 : 1 + w) * t.tw) - 1;  // positions of the stream's tokens
-    const int pos = k.lo_pos + tok;
-    const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const int tok = row / t.G + (ONE ? 0 : w * t.tw), head = row % t.G;
     const float scale_log2 = a.scale * LOG2E;
-    float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;  // after a wait that gave up the steps go on without waiting
-    for (int s = 0; s < nt[w]; s++) {
-      const uint32_t ph = (uint32_t)(s & 1);
-      const int i = ONE ? 2 * s + w : s;
-      ok = ok && mbar_wait(smem_u32(&bar_s[w]), ph);
-      __syncwarp();  // the loads from tensor memory want the warp together
-      tc_fence_after();
-      if (any_live) {
-        uint32_t r[BKV];
-        tc_ld32(tS + lane_base, r);
-        tc_ld32(tS + lane_base + 32, r + 32);
-        const int k0 = tile_key(i);
-        const uint32_t bits = page_bits[i & 7];
-        const bool full = bits == (1u << boxes) - 1 && sees_all(a, k.w.end, k0, BKV, pos_a, pos_b);
-        tc_wait_ld();
-        tc_ld32(tS + lane_base + 64, r + 64);  // on their way while the maximum of the first half is taken
-        tc_ld32(tS + lane_base + 96, r + 96);
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (full) {
+    int c = 0, steps = 0;  // key tiles of all units so far, steps of this stream
+    bool good = true;
+    for (int u = 0; good && next_unit(u); u++) {
+      const Unit& k = units[u & 1];
+      const int nt = k.nt_w[w], n_all = k.nt, part = k.part;
+      const PagedWalk walk = k.w;
+      const bool live = row < t.G * t.tw && tok < k.n;
+      const bool any_live = __any_sync(0xffffffffu, live);  // a warp without rows only keeps step
+      const int pos_a = k.lo_pos + (ONE ? 0 : w * t.tw), pos_b = k.lo_pos + min(k.n, (ONE ? 1 : 1 + w) * t.tw) - 1;  // positions of the stream's tokens
+      const int pos = k.lo_pos + tok;
+      const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int s = 0; s < nt; s++, steps++) {
+        const uint32_t ph = (uint32_t)(steps & 1);
+        const int i = ONE ? 2 * s + w : s;
+        good = warp_wait(smem_u32(&bar_s[w]), ph);
+        if (!good) break;
+        tc_fence_after();
+        if (any_live) {
+          uint32_t r[BKV];
+          tc_ld32(tS + lane_base, r);
+          tc_ld32(tS + lane_base + 32, r + 32);
+          const int k0 = walk.tile(share_tile(i, part, t.parts, t.ct)) * BKV;
+          const uint32_t bits = page_bits[(c + i) & 7];
+          const bool full = bits == (1u << boxes) - 1 && sees_all(a, walk.end, k0, BKV, pos_a, pos_b);
+          tc_wait_ld();
+          tc_ld32(tS + lane_base + 64, r + 64);  // on their way while the maximum of the first half is taken
+          tc_ld32(tS + lane_base + 96, r + 96);
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (full) {
 #pragma unroll
-          for (int j = 0; j < 64; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-        }
-        tc_wait_ld();
-        if (!full) {
-          // keys [0, hi) of the tile without [first, lo) and without pages that are not there
-          const int hi = min(k.w.end, pos + 1) - k0, lw = lo - k0, fi = a.first - k0;
+            for (int j = 0; j < 64; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+          }
+          tc_wait_ld();
+          if (!full) {
+            // keys [0, hi) of the tile without [first, lo) and without pages that are not there
+            const int hi = min(walk.end, pos + 1) - k0, lw = lo - k0, fi = a.first - k0;
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            auto below = [&](int x) { return x - c * 32 >= 32 ? ~0u : x - c * 32 > 0 ? (1u << (x - c * 32)) - 1 : 0u; };
-            uint32_t see = below(hi) & (~below(lw) | below(fi));
-            if (!(bits >> (c * 32 / box) & 1)) see &= 0xFFFF0000u;
-            if (!(bits >> ((c * 32 + 16) / box) & 1)) see &= 0x0000FFFFu;
+            for (int c4 = 0; c4 < 4; c4++) {
+              auto below = [&](int x) { return x - c4 * 32 >= 32 ? ~0u : x - c4 * 32 > 0 ? (1u << (x - c4 * 32)) - 1 : 0u; };
+              uint32_t see = below(hi) & (~below(lw) | below(fi));
+              if (!(bits >> (c4 * 32 / box) & 1)) see &= 0xFFFF0000u;
+              if (!(bits >> ((c4 * 32 + 16) / box) & 1)) see &= 0x0000FFFFu;
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (!(see >> j & 1)) r[c * 32 + j] = 0xFF800000u;  // -inf
+              for (int j = 0; j < 32; j++)
+                if (!(see >> j & 1)) r[c4 * 32 + j] = 0xFF800000u;  // -inf
+            }
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
           }
 #pragma unroll
-          for (int j = 0; j < 64; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-        }
-#pragma unroll
-        for (int j = 64; j < BKV; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-        const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale_log2;
-        const bool grow = m_tile > m_run + 8.0f;
-        const float m_use = grow ? m_tile : m_run;
-        const float corr = grow ? exp2f(m_run - m_use) : 1.0f;
-        m_run = m_use;
-        const float base = m_use == -INFINITY ? 0.f : -m_use;
-        if (s > 0 && __any_sync(0xffffffffu, grow)) {
-          ok = ok && mbar_wait(smem_u32(&bar_o[w]), ph ^ 1);  // the product in front has finished O
-          __syncwarp();
-          tc_fence_after();
+          for (int j = 64; j < BKV; j += 2) m4[(j >> 1) & 3] = max3(m4[(j >> 1) & 3], __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+          const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale_log2;
+          const bool grow = m_tile > m_run + 8.0f;
+          const float m_use = grow ? m_tile : m_run;
+          const float corr = grow ? exp2f(m_run - m_use) : 1.0f;
+          m_run = m_use;
+          const float base = m_use == -INFINITY ? 0.f : -m_use;
+          if (s > 0 && __any_sync(0xffffffffu, grow)) {
+            good = warp_wait(smem_u32(&bar_o[w]), ph ^ 1);  // the product in front has finished O
+            if (!good) break;
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 4 * QA; c++) {
-            uint32_t x[16];
-            tc_ld16(tO + lane_base + (uint32_t)(c * 16), x);
-            tc_wait_ld();
+            for (int x16 = 0; x16 < 4 * QA; x16++) {
+              uint32_t x[16];
+              tc_ld16(tO + lane_base + (uint32_t)(x16 * 16), x);
+              tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * corr);
-            tc_st16(tO + lane_base + (uint32_t)(c * 16), x);
+              for (int j = 0; j < 16; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * corr);
+              tc_st16(tO + lane_base + (uint32_t)(x16 * 16), x);
+            }
           }
+          const uint64_t scale2 = pack2(__float_as_uint(scale_log2), __float_as_uint(scale_log2)), base2 = pack2(__float_as_uint(base), __float_as_uint(base));
+          const uint64_t minus = pack2(0xBF800000u, 0xBF800000u);  // -1, -1
+          uint64_t sum = 0;
+#pragma unroll
+          for (int c4 = 0; c4 < 4; c4++) {
+            uint32_t hi[16], lo16[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+              const uint64_t e = fma2(pack2(r[c4 * 32 + 2 * j], r[c4 * 32 + 2 * j + 1]), scale2, base2);
+              const uint32_t b0 = __float_as_uint(ex2_approx(__uint_as_float((uint32_t)e))), b1 = __float_as_uint(ex2_approx(__uint_as_float((uint32_t)(e >> 32))));
+              const uint64_t p = pack2(b0, b1);
+              sum = add2(sum, p);
+              hi[j] = __byte_perm(b0, b1, 0x7632);
+              const uint64_t rest = fma2(pack2(b0 & 0xFFFF0000u, b1 & 0xFFFF0000u), minus, p);
+              lo16[j] = __byte_perm((uint32_t)rest, (uint32_t)(rest >> 32), 0x7632);
+            }
+            tc_st16(tS + lane_base + (uint32_t)(c4 * 32), hi);
+            tc_st16(tS + lane_base + (uint32_t)(c4 * 32 + 16), lo16);
+            if (c4 == 1) {  // the product of the first 64 keys may begin
+              tc_wait_st();
+              tc_fence_before();
+              asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][0])) : "memory");
+            }
+          }
+          l_run = l_run * corr + (__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)));
+          tc_wait_st();
+        } else {
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][0])) : "memory");
         }
-        const uint64_t scale2 = pack2(__float_as_uint(scale_log2), __float_as_uint(scale_log2)), base2 = pack2(__float_as_uint(base), __float_as_uint(base));
-        const uint64_t minus = pack2(0xBF800000u, 0xBF800000u);  // -1, -1
-        uint64_t sum = 0;
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t hi[16], lo16[16];
-#pragma unroll
-          for (int j = 0; j < 16; j++) {
-            const uint64_t e = fma2(pack2(r[c * 32 + 2 * j], r[c * 32 + 2 * j + 1]), scale2, base2);
-            const uint32_t b0 = __float_as_uint(ex2_approx(__uint_as_float((uint32_t)e))), b1 = __float_as_uint(ex2_approx(__uint_as_float((uint32_t)(e >> 32))));
-            const uint64_t p = pack2(b0, b1);
-            sum = add2(sum, p);
-            hi[j] = __byte_perm(b0, b1, 0x7632);
-            const uint64_t rest = fma2(pack2(b0 & 0xFFFF0000u, b1 & 0xFFFF0000u), minus, p);
-            lo16[j] = __byte_perm((uint32_t)rest, (uint32_t)(rest >> 32), 0x7632);
-          }
-          tc_st16(tS + lane_base + (uint32_t)(c * 32), hi);
-          tc_st16(tS + lane_base + (uint32_t)(c * 32 + 16), lo16);
-          if (c == 1) {  // the product of the first 64 keys may begin
-            tc_wait_st();
-            tc_fence_before();
-            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][0])) : "memory");
-          }
-        }
-        l_run = l_run * corr + (__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)));
-        tc_wait_st();
-      } else {
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][0])) : "memory");
+        tc_fence_before();
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][1])) : "memory");
       }
-      tc_fence_before();
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_p[w][1])) : "memory");
-    }
-    if (nt[w] > 0) {
-      ok = ok && mbar_wait(smem_u32(&bar_o[w]), (uint32_t)((nt[w] - 1) & 1));
-      __syncwarp();
-      tc_fence_after();
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok && lane == 0) set_status(t.status, 45);
-    if (ok && any_live) {
-      const int64_t at = (k.row0 + tok) * a.Hq + k.hk * t.G + row % t.G;
-      const int np = ONE ? 2 * t.parts : t.parts, p = ONE ? 2 * k.part + w : k.part;
-      const bool split = np > 1;
-      const float inv = split ? 1.f : l_run == 0.f ? 0.f : 1.0f / l_run;
-      if (split && live) t.join.ml[at * np + p] = make_float2(m_run, l_run);
-      const bool bad = *(volatile int*)&poison;
-      // Finished rows go through the queries' place in shared memory, which nobody reads any more, so that a warp's stores are whole rows (a thread per row
-      // and store is 32 lines for 512 bytes: 4700 cycles of a block).
-      uint4* stage = (uint4*)(smem + (ONE ? 0 : w * TILE)) + (row & ~31) * (D / 8);  // 32 rows of this warp, chunk c of row r at c ^ (r & 7)
-      if (!split && nt[w] == 0 && k.nt > 0) mbar_wait(smem_u32(&bar_q), 0);  // the queries have come there
+      if (!good) break;
+      if (nt > 0) {
+        good = warp_wait(smem_u32(&bar_o[w]), (uint32_t)(steps & 1) ^ 1);
+        if (!good) break;
+        tc_fence_after();
+      }
+      const int64_t at = (k.row0 + tok) * a.Hq + k.hk * t.G + head;
+      const int np = ONE ? 2 * t.parts : t.parts, p = ONE ? 2 * part + w : part;
+      const float inv = np > 1 ? 1.f : l_run == 0.f ? 0.f : 1.0f / l_run;
+      if (np > 1 && live) t.join.ml[at * np + p] = make_float2(m_run, l_run);
+      const bool bad = nt > 0 && any_live && k.poison;
+      if (bad) {
 #pragma unroll 1
-      for (int c = 0; c < 2 * QA; c++) {
-        uint32_t r[32];
+        for (int c32 = 0; c32 < 2 * QA; c32++) {
+          uint32_t r[32];
+          float f[32];
+          __syncwarp();
+          tc_ld32(tO + lane_base + (uint32_t)(c32 * 32), r);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
+          if (live) add_poison(a, walk, k.b, k.hk, part, t.parts, t.ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt, pos, c32 * 32, 32, f);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; j++) r[j] = __float_as_uint(f[j]);
+          tc_st32(tO + lane_base + (uint32_t)(c32 * 32), r);
+        }
+        tc_wait_st();
+      }
+      // Rows leave through 4 KB of shared memory per warp, 128 bytes of each at a time, so that a store is four whole lines (a thread per row and store is 32
+      // lines for 512 bytes). Chunk x of row i lies at x ^ (i & 7).
+      uint4* stage = (uint4*)(smem + (NQ + 2 * RING) * TILE) + warp * 256;
+      const int64_t to = live ? np > 1 ? (at * np + p) * D * 4 : at * D * 2 : -1;
+      auto leave = [&](int piece) {
+        uint8_t* dst0 = (np > 1 ? (uint8_t*)t.join.o : (uint8_t*)a.out) + piece * 128 + (lane & 7) * 16;
         __syncwarp();
-        if (nt[w] > 0) {
-          tc_ld32(tO + lane_base + (uint32_t)(c * 32), r);
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const int i = x * 4 + (lane >> 3);
+          const int64_t dst = __shfl_sync(0xffffffffu, to, i);
+          const uint4 v = stage[i * 8 + ((lane & 7) ^ (i & 7))];
+          if (dst >= 0) *(uint4*)(dst0 + dst) = v;
+        }
+        __syncwarp();
+      };
+#pragma unroll 1
+      for (int h = 0; h < QA; h++) {
+        uint32_t r[64];
+        if (nt > 0 && any_live) {
+          tc_ld32(tO + lane_base + (uint32_t)(h * 64), r);
+          tc_ld32(tO + lane_base + (uint32_t)(h * 64 + 32), r + 32);
           tc_wait_ld();
         }
-        if (l_run == 0.f) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) r[j] = 0;
-        } else if (bad && live) {
-          float f[32];
-          for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
-          add_poison(a, k.w, k.b, k.hk, k.part, t.parts, t.ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt[w], pos, c * 32, 32, f);
-          for (int j = 0; j < 32; j++) r[j] = __float_as_uint(f[j]);
+        if (nt > 0 && h == QA - 1) {  // O may be begun anew
+          tc_fence_before();
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&o_free[w])) : "memory");
         }
-        if (split) {
-          if (live && l_run != 0.f) {
-            float* dst = t.join.o + (at * np + p) * D + c * 32;
+        if (!any_live) continue;
+        if (l_run == 0.f) {  // nothing seen
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *(uint4*)(dst + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+          for (int j = 0; j < 64; j++) r[j] = 0;
+        }
+        if (ONE) {
+          if (live && l_run != 0.f) {
+            float* dst = t.join.o + (at * np + p) * D + h * 64;
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) *(uint4*)(dst + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+          }
+          __syncwarp();
+        } else if (np > 1) {
+#pragma unroll
+          for (int piece = 0; piece < 2; piece++) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+              const int j = piece * 32 + x * 4;
+              stage[lane * 8 + (x ^ (lane & 7))] = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            }
+            leave(2 * h + piece);
           }
         } else {
+          auto two = [&](int j) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(r[j]) * inv, __uint_as_float(r[j + 1]) * inv);
+            return *(const uint32_t*)&v;
+          };
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 v;
-            v.x = f32_to_bf16_bits(__uint_as_float(r[j]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 1]) * inv) << 16);
-            v.y = f32_to_bf16_bits(__uint_as_float(r[j + 2]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 3]) * inv) << 16);
-            v.z = f32_to_bf16_bits(__uint_as_float(r[j + 4]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 5]) * inv) << 16);
-            v.w = f32_to_bf16_bits(__uint_as_float(r[j + 6]) * inv) | (f32_to_bf16_bits(__uint_as_float(r[j + 7]) * inv) << 16);
-            stage[lane * (D / 8) + ((c * 4 + j / 8) ^ (lane & 7))] = v;
-          }
+          for (int x = 0; x < 8; x++) stage[lane * 8 + (x ^ (lane & 7))] = make_uint4(two(x * 8), two(x * 8 + 2), two(x * 8 + 4), two(x * 8 + 6));
+          leave(h);
         }
       }
-      if (!split) {
-        __syncwarp();
-        constexpr int LANES = D / 8, PASS = 32 / LANES;  // lanes of a row, rows of a pass
-#pragma unroll 4
-        for (int x = 0; x < 32; x += PASS) {
-          const int rr = x + lane / LANES, cc = lane % LANES;
-          const int64_t to = __shfl_sync(0xffffffffu, at, rr);
-          const bool on = __shfl_sync(0xffffffffu, (int)live, rr);
-          const uint4 v = stage[rr * LANES + (cc ^ (rr & 7))];
-          if (on) *(uint4*)(a.out + to * D + cc * 8) = v;
-        }
-      }
+      unit_read(u);
+      c += n_all;
     }
+    if (!good && lane == 0) set_status(t.status, 45);
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
@@ -658,8 +726,7 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   t.ct = (int)((keys + t.parts - 1) / t.parts);
   const int np = (ONE ? 2 : 1) * t.parts;
   if (np > 1) SB_TRY(paged_join_scratch(ctx, a, np, &t.join));
-  const int64_t blocks = tiles * a.Hkv * t.parts;
-  if (blocks > INT32_MAX) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "attention: too many rows and heads for one call");
+  const int64_t blocks = std::min<int64_t>(tiles * a.Hkv * t.parts, ctx->sm_count);
   CUtensorMap mq, mk, mv;
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(map_tokens(&mq, a.q, a.at.T, a.Hq, a.D, t.G, t.tw));

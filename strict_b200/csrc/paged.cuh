@@ -62,10 +62,10 @@ __device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
 }
 // The key tiles (of `kt` positions) that rows at positions lo_pos .. hi_pos walk over: those of the first tokens, then those from the window on.
 struct PagedWalk {
-  int first = 0;   // tiles of the first tokens
-  int lo = 0;      // tile where the window begins
-  int total = 0;
-  int end = 0;     // no row sees this position or a later one
+  int first;  // tiles of the first tokens
+  int lo;     // tile where the window begins
+  int total;
+  int end;    // no row sees this position or a later one
   __device__ __forceinline__ int tile(int t) const { return t < first ? t : lo + t - first; }
 };
 __device__ __forceinline__ PagedWalk paged_walk(const PagedView& v, int len, int lo_pos, int hi_pos, int window, int first, int kt) {

@@ -18,8 +18,8 @@
 // Pages: a tile of 128 keys is 128 / page boxes (or part of a page); the lanes of the copying warp look the pages up, well ahead. A page that
 // the table does not name, or that begins behind the last position any row sees, is not fetched, and its keys are hidden by a bit mask.
 // What lies at hidden positions must not count: scores are replaced by index, but a weight of zero times a value that is not finite is not zero, and
-// places that were not fetched hold anything. So in tiles where some row does not see some key, two warps put zeros over values that no row sees, and over those
-// that are not finite; if there were any of the latter (`poison`), the rows that do see them add them at the end.
+// places that were not fetched hold anything. So in tiles where some row does not see some key, two warps put zeros over values that are not finite; if any
+// row sees one of those (`poison`), it adds them at the end.
 #include <algorithm>
 
 #include "attention_paged.cuh"
@@ -38,6 +38,7 @@ struct TilesArgs {
   int parts, ct;   // blocks that share the keys, tiles of a piece
   int G, tw;       // heads per key/value head, tokens of a tile of 128 rows
   double inv_tb;   // 1 / tokens of a unit
+  int one_round;   // a block for every unit
   int* status;
 };
 
@@ -117,6 +118,21 @@ constexpr size_t tiles_smem() { return (size_t)((ONE ? 1 : 2) + 2 * tiles_ring<Q
 // The x-th unit of work, a tile of tb tokens of a sequence, in the order of falling positions (of the last token, by 128): those with the most keys come
 // first, of all sequences, and the short ones fill the SMs at the end. Nobody lists the units: how many of them end at position X or later is a sum over
 // the sequences, so the level of the x-th is searched for, and its sequence found in that level. False behind the last unit. A warp calls it together.
+// Where every unit has a block of its own the order does not matter: then the tiles of sequence b begin at (starts[b] - starts[0]) / tb + b, room for all.
+__device__ __forceinline__ bool place_unit(const PagedView& v, double inv_tb, int x, int lane, int* b_out, int* tile_out) {
+  const int s0 = v.starts[0];
+  int before = 0, base = 0;
+  for (int b0 = 0; b0 < v.B; b0 += 32) {
+    const int b = b0 + lane, at = b < v.B ? (int)((v.starts[b] - s0 + 0.5) * inv_tb) + b : INT_MAX;
+    const unsigned m = __ballot_sync(0xffffffffu, at <= x);
+    if (m) base = __shfl_sync(0xffffffffu, at, 31 - __clz(m));
+    before += __popc(m);
+    if (m != 0xffffffffu) break;
+  }
+  *b_out = before - 1;
+  *tile_out = x - base;
+  return before > 0;
+}
 struct UnitSeq {
   int past, n, units;  // of sequence lane + 32 i: tokens before the new ones, new ones, tiles
 };
@@ -125,8 +141,9 @@ __device__ __forceinline__ int units_from(const UnitSeq& u, int X, double inv_tb
   if (u.past + u.n < X) return 0;
   return u.units - (X > u.past ? (int)((X - u.past - 1 + 0.5) * inv_tb) : 0);  // (X - past - 1) / tb units end before
 }
+// KEEP: sequences of a lane that stay in registers; more are read again each time.
+template <int KEEP>
 __device__ bool find_unit(const PagedView& v, int tb, double inv_tb, int x, int lane, int* b_out, int* tile_out) {
-  constexpr int KEEP = 4;  // sequences of a lane that stay in registers; more are read again each time
   auto seq = [&](int b) {
     UnitSeq u{0, 0, 0};
     if (b < v.B) {
@@ -186,7 +203,8 @@ __device__ bool find_unit(const PagedView& v, int tb, double inv_tb, int x, int 
 
 template <int QA, bool ONE>
 __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TilesArgs t) {
+                                                                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+                                                                   const __grid_constant__ TilesArgs t) {
   constexpr int TILE = QA * HALF_BYTES, NQ = ONE ? 1 : 2, D = 64 * QA, RING = tiles_ring<QA, ONE>();
   constexpr int READERS = 11;  // warps that read a unit's description
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -247,7 +265,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
       k.n = -1;
       k.nt = 0;
       int tile;
-      if (find_unit(a.at, NQ * t.tw, t.inv_tb, (int)(y / per), lane, &k.b, &tile)) {
+      const int x = (int)(y / per);
+      const bool one_round = t.one_round;
+      if (one_round ? u == 0 && place_unit(a.at, t.inv_tb, x, lane, &k.b, &tile)
+                    : a.at.B <= 32 ? find_unit<1>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile) : find_unit<4>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile)) {
         k.part = (int)(y % per) / a.Hkv;
         k.hk = (int)(y % per) % a.Hkv;
         const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb, len = a.at.lens[k.b], q0 = tile * NQ * t.tw;
@@ -454,16 +475,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
         if (bits != (1u << boxes) - 1 || !sees_all(a, w.end, k0, BKV, lo_pos, hi_pos)) {
           uint32_t found = 0;
           uint4* v = (uint4*)(smem + (NQ + RING + st) * TILE);
-#pragma unroll 4
-          for (int x = tid; x < QA * BKV * 8; x += 64) {
-            const int r = (x >> 3) & (BKV - 1), j = k0 + r;
-            const bool seen = j < w.end && (bits >> (r / box) & 1) && (j >= lo_key || j < a.first);
-            const uint4 y = v[x];
-            if (!seen) {
-              v[x] = make_uint4(0, 0, 0, 0);
-            } else if (not_finite(y.x) | not_finite(y.y) | not_finite(y.z) | not_finite(y.w)) {
-              v[x] = make_uint4(only_finite(y.x), only_finite(y.y), only_finite(y.z), only_finite(y.w));
-              found = 1;
+          constexpr int AHEAD = 8;  // finite values need nothing, whoever sees them: the loads of eight go together
+          for (int x0 = tid; x0 < QA * BKV * 8; x0 += 64 * AHEAD) {
+            uint4 y[AHEAD];
+            uint32_t odd = 0;
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) y[e] = v[x0 + 64 * e];
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) odd |= not_finite(y[e].x) | not_finite(y[e].y) | not_finite(y[e].z) | not_finite(y[e].w);
+            if (!odd) continue;
+            for (int x = x0; x < x0 + 64 * AHEAD; x += 64) {
+              const int r = (x >> 3) & (BKV - 1), j = k0 + r;
+              const bool seen = j < w.end && (bits >> (r / box) & 1) && (j >= lo_key || j < a.first);
+              const uint4 z = v[x];
+              found |= seen && (not_finite(z.x) | not_finite(z.y) | not_finite(z.z) | not_finite(z.w));
+              v[x] = make_uint4(only_finite(z.x), only_finite(z.y), only_finite(z.z), only_finite(z.w));
             }
           }
           if (found) k.poison = 1;
@@ -526,6 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
               uint32_t see = below(hi) & (~below(lw) | below(fi));
               if (!(bits >> (c4 * 32 / box) & 1)) see &= 0xFFFF0000u;
               if (!(bits >> ((c4 * 32 + 16) / box) & 1)) see &= 0x0000FFFFu;
+              if (__all_sync(0xffffffffu, see == ~0u)) continue;  // the rows of a warp are few tokens: most chunks are seen or hidden as a whole
 #pragma unroll
               for (int j = 0; j < 32; j++)
                 if (!(see >> j & 1)) r[c4 * 32 + j] = 0xFF800000u;  // -inf
@@ -616,8 +643,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
         }
         tc_wait_st();
       }
-      // Rows leave through 4 KB of shared memory per warp, 128 bytes of each at a time, so that a store is four whole lines (a thread per row and store is 32
-      // lines for 512 bytes). Chunk x of row i lies at x ^ (i & 7).
+      // Rows leave through 4 KB of shared memory per warp, 128 bytes of each at a time, by one TMA store where the warp's 32 rows are whole tokens of the unit, and
+      // otherwise so that a store is four whole lines (a thread per row and store is 32 lines for 512 bytes). Chunk x of row i lies at x ^ (i & 7).
+      const bool by_tma = !ONE && np == 1 && 32 % t.G == 0 && __all_sync(0xffffffffu, live);
       uint4* stage = (uint4*)(smem + (NQ + 2 * RING) * TILE) + warp * 256;
       const int64_t to = live ? np > 1 ? (at * np + p) * D * 4 : at * D * 2 : -1;
       auto leave = [&](int piece) {
@@ -673,7 +701,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
           };
 #pragma unroll
           for (int x = 0; x < 8; x++) stage[lane * 8 + (x ^ (lane & 7))] = make_uint4(two(x * 8), two(x * 8 + 2), two(x * 8 + 4), two(x * 8 + 6));
-          leave(h);
+          if (by_tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(&map_o), "r"(h * 64), "r"(k.hk * t.G),
+                           "r"((int)(k.row0 + tok)), "r"(smem_u32(stage))
+                           : "memory");
+              asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");  // read before the place is used again
+            }
+            __syncwarp();
+          } else {
+            leave(h);
+          }
         }
       }
       unit_read(u);
@@ -727,15 +767,17 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   const int np = (ONE ? 2 : 1) * t.parts;
   if (np > 1) SB_TRY(paged_join_scratch(ctx, a, np, &t.join));
   const int64_t blocks = std::min<int64_t>(tiles * a.Hkv * t.parts, ctx->sm_count);
-  CUtensorMap mq, mk, mv;
+  t.one_round = tiles * a.Hkv * t.parts <= ctx->sm_count;
+  CUtensorMap mq, mk, mv, mo;
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(map_tokens(&mq, a.q, a.at.T, a.Hq, a.D, t.G, t.tw));
+  SB_TRY(map_tokens(&mo, a.out, a.at.T, a.Hq, a.D, t.G, std::max(1, 32 / t.G)));  // the rows of a warp
   SB_TRY(paged_map_rows(&mk, a.k, rows, a.D, std::min(a.at.page, BKV)));
   SB_TRY(paged_map_rows(&mv, a.v, rows, a.D, std::min(a.at.page, BKV)));
   constexpr size_t smem = tiles_smem<QA, ONE>();
   static SbDeviceOnce once;  // one per instantiation
   SB_CUDA(once.run(ctx->device, [&] { return cudaFuncSetAttribute(attn_paged_tiles_kernel<QA, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
-  SB_CUDA(sb_launch(ctx, attn_paged_tiles_kernel<QA, ONE>, dim3((unsigned)blocks), dim3(THREADS), smem, mq, mk, mv, t));
+  SB_CUDA(sb_launch(ctx, attn_paged_tiles_kernel<QA, ONE>, dim3((unsigned)blocks), dim3(THREADS), smem, mq, mk, mv, mo, t));
   ctx->launches++;
   return np > 1 ? paged_join(ctx, a, t.join) : STRICTB200_OK;
 }

@@ -10,12 +10,15 @@
 //
 // A row is read from memory once: a cluster of up to eight blocks holds it in shared memory (as ordered keys) and passes over it there. What bounds a row is
 // the chain of passes and of meetings of the cluster, two to four microseconds each pair:
-//   load, maximum                                    one meeting
-//   counts (weights) in 1024 bins of (max - l),      two meetings; bins even in l, so that few threads meet at one counter
-//   the bin where top_k (top_p) falls
-//   those in front of and in that bin, if there are at most LIST, go to the first block, which ranks them and ends the row alone
-// Otherwise the place where the order is cut is found among those of the bin (in the first block if there are at most LIST, by bits of the place where more
-// share the bin), and all blocks sum the kept weights and look for the token. Batches: two blocks per SM, so that one row's meetings are another's passes.
+//   load, maximum, largest places of 512 groups of threads                                             one meeting
+//   top_k of up to 128: the k-th largest of those groups' places bounds the first k tokens from below, and what lies above it, seldom more than
+//   a few more, goes to the first block, which ranks them and ends the row alone                       one meeting
+// Otherwise, and where that list would be too long:
+//   counts (weights) in 1024 bins of (max - l), even in l, and the bin where top_k (top_p) falls       two meetings
+//   those in front of and in that bin go to the first block as above, if there are at most LIST        three meetings
+//   otherwise the place where the order is cut is found among those of the bin (in the first block if there are at most LIST, by bits of the place where
+//   more share the bin), and all blocks sum the kept weights and look for the token
+// Batches: two blocks per SM, so that one row's meetings are another's passes.
 #include <algorithm>
 
 #include "common.cuh"
@@ -59,7 +62,7 @@ struct Shared {
   union {
     struct {
       uint32_t count[BINS];
-      unsigned long long sum[BINS];
+      uint32_t sum[3][BINS];  // weights in pieces of 15 bits: counters of 32 bits are added to without a loop, and 2^17 members do not overflow them
     } bin;
     struct {
       uint64_t place[LIST], w[LIST], by_rank[LIST];
@@ -75,6 +78,8 @@ struct Shared {
   // what blocks tell one another: largest place and number of a share that has any weight, a cut, the kept weights
   uint64_t best, there, word, drawn;
   uint32_t n_list;
+  long long fraction[64];  // bits of 2^(43 + i / 64)
+  uint64_t crest[THREADS], crest_own[THREADS];  // largest places of groups of threads: of all blocks, of this one
 };
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -99,9 +104,9 @@ struct Row {
   const uint32_t* keys;  // of the first `held` of this block's `share`
   const void* x;
   int N, f32, first, share, held;
-  int blocks, rank;
+  int blocks, rank, crests;  // crests: groups of this block's threads
   uint32_t top;        // key of the largest logit
-  double m, scale;     // its value, log2(e) / temperature
+  double m, scale;     // its value, 64 log2(e) / temperature
   float m32, bin_scale;
 
   // All blocks of the cluster, all threads.
@@ -116,28 +121,27 @@ struct Row {
   __device__ __forceinline__ uint32_t key(int i) const { return i < held ? keys[i] : load(i); }
   // the place in the row's order, larger is earlier: the key, then the lower index
   __device__ __forceinline__ uint64_t place(uint32_t k, int i) const { return (uint64_t)k << 20 | (uint32_t)(0xFFFFF - (first + i)); }
-  // 2^43 exp((l - max) / T): 2^y with y = n + f, |f| <= 1/2, and the series of exp(f ln 2) to the eleventh power (off by 6e-15), rounded to a whole number by the
-  // addition of 2^52.
+  // 2^43 exp((l - max) / T) rounded to a whole number. y = 64 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 64) is 2^(n / 64), from a table of
+  // the 64 fractions, times the series of exp(f ln(2) / 64) to the fourth power (off by 4e-14, less than half a unit). The sums that round are additions of a
+  // power of two that leaves no bits behind the point.
   __device__ __forceinline__ uint64_t weight(uint32_t k) const {
     if (k == top) return 1ull << 43;
     if (k <= KEY_NONE || top >= KEY_INF) return 0;  // beside +inf nothing has a weight
-    const double y = ((double)of_key(k) - m) * scale;
-    if (!(y > -45.0)) return 0;
-    const double n = rint(y), z = (y - n) * 0.69314718055994530942;
-    double p = 1.0 / 39916800;
-    p = fma(p, z, 1.0 / 3628800);
-    p = fma(p, z, 1.0 / 362880);
-    p = fma(p, z, 1.0 / 40320);
-    p = fma(p, z, 1.0 / 5040);
-    p = fma(p, z, 1.0 / 720);
-    p = fma(p, z, 1.0 / 120);
-    p = fma(p, z, 1.0 / 24);
-    p = fma(p, z, 1.0 / 6);
-    p = fma(p, z, 0.5);
-    p = fma(p, z, 1.0);
-    p = fma(p, z, 1.0);
-    const double two_n = __longlong_as_double((long long)((int)n + 1023 + 43) << 52);
-    return (uint64_t)__double_as_longlong(fma(p, two_n, 4503599627370496.0)) - 0x4330000000000000ull;
+    // the float's bits as a double's (a subnormal one becomes another of no consequence)
+    const uint32_t b = __float_as_uint(of_key(k));
+    const double d = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29)) - m;
+    constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52
+    if (!(d * scale > -2880.0)) return 0;  // 2^-45
+    const double t = fma(d, scale, WHOLE), f = fma(d, scale, WHOLE - t);
+    const int n = __double2loint(t);
+    constexpr double C = 0.69314718055994530942 / 64;
+    double p = C * C * C * C / 24;
+    p = fma(p, f, C * C * C / 6);
+    p = fma(p, f, C * C / 2);
+    p = fma(p, f, C);
+    p = fma(p, f, 1.0);
+    const long long two = s.fraction[n & 63] + ((long long)(n >> 6) << 52);  // 2^(43 + n / 64)
+    return (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0)) - 0x4330000000000000ull;
   }
   // Bins of equal width below the maximum, the last one for all that is further away; never falls with a falling logit.
   __device__ __forceinline__ int bin(uint32_t k) const {
@@ -193,7 +197,7 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
   const int per = BINS / r.blocks;
   r.meet();  // all bins are counted
   const uint32_t* counts = s.bin.count;
-  const unsigned long long* sums = s.bin.sum;
+  auto sum_of = [&](int i) { return s.bin.sum[0][i] + ((uint64_t)s.bin.sum[1][i] << 15) + ((uint64_t)s.bin.sum[2][i] << 30); };
   int owner = 0;
   uint64_t front_c = 0, front_s = 0, all_s = 0;
   if (r.blocks > 1) {
@@ -205,7 +209,10 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
       for (int b = 0; b < MAX_CLUSTER; b++)
         if (b < r.blocks) {
           c[b] = peer32(&s.bin.count[r.rank * per + i], b);
-          if (SUMS) w[b] = peer64((const uint64_t*)&s.bin.sum[r.rank * per + i], b);
+          if (SUMS) {
+            const int at = r.rank * per + i;
+            w[b] = peer32(&s.bin.sum[0][at], b) + ((uint64_t)peer32(&s.bin.sum[1][at], b) << 15) + ((uint64_t)peer32(&s.bin.sum[2][at], b) << 30);
+          }
         }
       uint64_t cc = 0, ww = 0;
 #pragma unroll
@@ -247,7 +254,7 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
       }
   } else if (SUMS && share_p >= 0.f) {
     uint64_t ts = 0;
-    for (int i = threadIdx.x; i < per; i += THREADS) ts += sums[i];
+    for (int i = threadIdx.x; i < per; i += THREADS) ts += sum_of(i);
     all_s = block_sum64(ts, s.red2);
     bool lost;
     *want = share_of(all_s, share_p, &lost);
@@ -262,7 +269,7 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
     const int i = threadIdx.x * each + e;
     if (e < each && i < per) {
       c2[e] = r.blocks > 1 ? peer32(&s.part_count[i], owner) : counts[i];
-      if (SUMS) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : sums[i];
+      if (SUMS) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : sum_of(i);
     }
   }
   uint64_t all, before_c = front_c + block_before64(c2[0] + c2[1], s.red, &all), before_s = 0;
@@ -289,42 +296,45 @@ __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS) {
     s.bin.count[i] = 0;
-    if (sums) s.bin.sum[i] = 0;
+    if (sums) s.bin.sum[0][i] = s.bin.sum[1][i] = s.bin.sum[2][i] = 0;
   }
   __syncthreads();
 }
 
-// A warp's members into their bins; together where they all go to one (the far ones of most rows, rows of equal logits).
+// A member into its bin. Where a warp's members all go to one bin (rows of equal logits, large temperatures) they go together.
 template <bool SUMS>
 __device__ __forceinline__ void add_to_bin(Shared& s, bool in, int b, uint64_t w) {
   const unsigned who = __ballot_sync(0xffffffffu, in);
   if (!who) return;
   const int lead = __ffs(who) - 1, b0 = __shfl_sync(0xffffffffu, b, lead);
+  uint32_t n = 1;
   if (__all_sync(0xffffffffu, !in || b == b0)) {
     if (SUMS) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     }
-    if ((threadIdx.x & 31) == lead) {
-      atomicAdd(&s.bin.count[b0], (uint32_t)__popc(who));
-      if (SUMS && w) atomicAdd(&s.bin.sum[b0], (unsigned long long)w);
-    }
-    return;
+    n = __popc(who);
+    in = (threadIdx.x & 31) == lead;
   }
-  // the last bin may hold nearly all
-  const unsigned last = __ballot_sync(0xffffffffu, in && b == BINS - 1);
-  if (last && (threadIdx.x & 31) == __ffs(last) - 1) atomicAdd(&s.bin.count[BINS - 1], (uint32_t)__popc(last));
-  if (in && b != BINS - 1) atomicAdd(&s.bin.count[b], 1u);
-  if (SUMS && w) atomicAdd(&s.bin.sum[b], (unsigned long long)w);
+  if (!in) return;
+  atomicAdd(&s.bin.count[b], n);
+  if (SUMS && w) {  // at most 2^48
+    atomicAdd(&s.bin.sum[0][b], (uint32_t)w & 0x7FFFu);
+    atomicAdd(&s.bin.sum[1][b], (uint32_t)(w >> 15) & 0x7FFFu);
+    atomicAdd(&s.bin.sum[2][b], (uint32_t)(w >> 30));
+  }
 }
 
 // The members `of` chooses, from all blocks, into the first block's list (at most LIST of them).
-template <typename F>
+// AGAIN: the place of the list was in use.
+template <bool AGAIN, typename F>
 __device__ void gather(Row& r, F&& of) {
   Shared& s = r.s;
-  r.meet();  // nobody reads bins any more
-  if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
-  r.meet();
+  if (AGAIN) {
+    r.meet();  // nobody reads bins any more
+    if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
+    r.meet();
+  }
   for (int i = threadIdx.x; i < r.share; i += THREADS) {
     const uint32_t k = r.key(i);
     const uint64_t p = r.place(k, i);
@@ -371,7 +381,7 @@ __device__ uint64_t cut(Row& r, uint64_t from, uint64_t* want, float share_p, bo
   const int b0 = c.bin;
   *few = c.front + c.count <= LIST;
   if (*few) {
-    gather(r, [&](uint32_t k, uint64_t p) { return p >= from && r.bin(k) <= b0; });
+    gather<true>(r, [&](uint32_t k, uint64_t p) { return p >= from && r.bin(k) <= b0; });
     if (r.rank == 0) rank_list(s, (int)s.n_list);
     return 0;
   }
@@ -386,7 +396,7 @@ __device__ uint64_t cut(Row& r, uint64_t from, uint64_t* want, float share_p, bo
     if (c.count <= LIST) {
       const int sh = shift;
       const uint64_t kn = known;
-      gather(r, [&](uint32_t k, uint64_t p) { return p >= from && r.bin(k) == b0 && (sh == 52 || p >> sh == kn); });
+      gather<true>(r, [&](uint32_t k, uint64_t p) { return p >= from && r.bin(k) == b0 && (sh == 52 || p >> sh == kn); });
       if (r.rank == 0) {
         const int n = (int)s.n_list;
         rank_list(s, n);
@@ -531,11 +541,16 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
 #pragma unroll 4
     for (int i = threadIdx.x; i < r.share; i += THREADS) take(r.load(i), i);
   }
+  // 512 groups in the cluster: threads of a block, or two, four or eight neighbours
+  r.crests = THREADS / r.blocks;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = 1; o < 32; o <<= 1) {
+    if (o == r.blocks && lane % o == 0) s.crest_own[threadIdx.x / o] = best;
     const uint64_t v = __shfl_xor_sync(0xffffffffu, best, o);
     best = v > best ? v : best;
   }
+  if (threadIdx.x < 64) s.fraction[threadIdx.x] = __double_as_longlong(exp2(43.0 + threadIdx.x / 64.0));
+  if (threadIdx.x == 0) s.n_list = 0;
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
   for (int i = 0; i < WARPS; i++) best = s.red[i] > best ? s.red[i] : best;
@@ -562,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
     r.meet();
     return;
   }
-  r.scale = 1.4426950408889634074 / heat;
+  r.scale = 64 * 1.4426950408889634074 / heat;
   r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
   if (r.top >= KEY_INF) r.m32 = 3.4028235e38f;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
   const int k = a.top_k ? a.top_k[row] : 0;
@@ -572,7 +587,31 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
   uint64_t from = (uint64_t)(KEY_NONE + 1) << 20, want = 0;
   bool few = false;
-  if (k > 0 && k < a.N) {
+  if (k > 0 && k < a.N && 4 * k <= r.blocks * r.crests) {
+    // The k-th largest of the groups' largest places has at least k places from it on, and, where the largest are not all in a few groups, not many more.
+    uint64_t* crest = s.crest;
+    const int n = r.blocks * r.crests;
+    uint64_t mine = 0;
+    if (threadIdx.x < n) mine = r.blocks > 1 ? peer64(&s.crest_own[threadIdx.x % r.crests], threadIdx.x / r.crests) : s.crest_own[threadIdx.x];
+    crest[threadIdx.x] = mine;
+    if (threadIdx.x == 0) s.pick[0] = 0;  // fewer than k groups have any
+    __syncthreads();
+    if (threadIdx.x < n) {
+      int above = 0;
+      for (int j = 0; j < n; j++) above += crest[j] > mine;
+      if (above == k - 1) s.pick[0] = mine;
+    }
+    __syncthreads();
+    const uint64_t low = s.pick[0] > from ? s.pick[0] : from;
+    gather<false>(r, [&](uint32_t, uint64_t p) { return p >= low; });
+    few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
+    if (few && r.rank == 0) {
+      rank_list(s, (int)s.n_list);
+      end_row(r, a, row, k, 0, top_p < 1.f, top_p, least, u);
+    }
+    if (!few) r.meet();  // the number has been read
+  }
+  if (!few && k > 0 && k < a.N) {
     want = k;
     if (want < there) {  // otherwise all that have any weight are kept
       from = cut<false>(r, from, &want, -1.f, &few);
@@ -587,26 +626,19 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
     r.meet();
     return;
   }
-  // the draw: warp w has the w-th contiguous part of the block's share
-  const int part = ((r.share + WARPS - 1) / WARPS + 31) / 32 * 32, i0 = min(r.share, warp * part), i1 = min(r.share, i0 + part);
+  // The draw: a thread sums a contiguous part of the block's share (an odd number of keys, so that a warp's reads meet no bank twice), the sums in front of
+  // it tell the one thread whose part holds the token, and its warp looks through that part.
+  const int each_thread = (r.share + THREADS - 1) / THREADS | 1, i0 = min(r.share, (int)threadIdx.x * each_thread), i1 = min(r.share, i0 + each_thread);
   auto kept = [&](int i) -> uint64_t {
     const uint32_t key = r.key(i);
     if (r.place(key, i) < from) return 0;
     const uint64_t w = r.weight(key);
     return w >= least ? w : 0;
   };
-  uint64_t mine = 0;
-  for (int i = i0 + lane; i < i1; i += 32) mine += kept(i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  __syncthreads();
-  if (lane == 0) s.red[warp] = mine;
-  __syncthreads();
-  uint64_t block_total = 0, before = 0, total = 0;
-  for (int i = 0; i < WARPS; i++) {
-    if (i < warp) before += s.red[i];
-    block_total += s.red[i];
-  }
+  uint64_t mine = 0, block_total, total = 0;
+#pragma unroll 4
+  for (int i = i0; i < i1; i++) mine += kept(i);
+  uint64_t before = block_before64(mine, s.red, &block_total);
   if (threadIdx.x == 0) s.drawn = block_total;
   r.meet();
   for (int b = 0; b < r.blocks; b++) {
@@ -617,9 +649,12 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   r.meet();  // nobody leaves while its memory is read
   bool lost;
   const uint64_t target = share_of(total, u, &lost);
-  if (target < before || target >= before + mine) return;
-  for (int i = i0; i < i1; i += 32) {
-    const uint64_t w = i + lane < i1 ? kept(i + lane) : 0;
+  const unsigned mine_it_is = __ballot_sync(0xffffffffu, target >= before && target < before + mine);
+  if (!mine_it_is) return;
+  const int src = __ffs(mine_it_is) - 1, p0 = __shfl_sync(0xffffffffu, i0, src), p1 = __shfl_sync(0xffffffffu, i1, src);
+  before = __shfl_sync(0xffffffffu, before, src);
+  for (int i = p0; i < p1; i += 32) {
+    const uint64_t w = i + lane < p1 ? kept(i + lane) : 0;
     uint64_t sum = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

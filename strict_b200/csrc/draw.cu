@@ -11,7 +11,7 @@
 // A row is read from memory once: a cluster of up to eight blocks holds it in shared memory (as ordered keys) and passes over it there. What bounds a row is
 // the chain of passes and of meetings of the cluster, two to four microseconds each pair:
 //   load, maximum, largest places of 512 groups of threads                                             one meeting
-//   top_k of up to 128: the k-th largest of those groups' places bounds the first k tokens from below, and what lies above it, seldom more than
+//   top_k of up to 256: the k-th largest of those groups' places bounds the first k tokens from below, and what lies above it, seldom more than
 //   a few more, goes to the first block, which ranks them and ends the row alone                       one meeting
 // Otherwise, and where that list would be too long:
 //   counts (weights) in 1024 bins of (max - l), even in l, and the bin where top_k (top_p) falls       two meetings
@@ -43,11 +43,15 @@ struct DrawArgs {
 
 // Larger logits have larger keys; NaN counts as -inf, -0 as 0.
 __device__ __forceinline__ uint32_t key_of(float l) {
-  l = l != l ? -INFINITY : l + 0.f;
-  const uint32_t b = __float_as_uint(l);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t b = __float_as_uint(l != l ? -INFINITY : l + 0.f);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ uint32_t bits_of_key(uint32_t k) { return k ^ (~(uint32_t)((int32_t)k >> 31) | 0x80000000u); }
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(bits_of_key(k)); }
+// A float's bits as a double's: exact for normal numbers, infinities become 2^128 (further than any number), subnormal ones others of no consequence.
+__device__ __forceinline__ double wide(uint32_t b) {
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // of -inf
 constexpr uint32_t KEY_INF = 0xFF800000u;
 
@@ -75,11 +79,10 @@ struct Shared {
   uint64_t total_count, total_sum;
   uint64_t red[WARPS], red2[WARPS];
   uint64_t pick[6];
-  // what blocks tell one another: largest place and number of a share that has any weight, a cut, the kept weights
-  uint64_t best, there, word, drawn;
+  uint64_t best, there, weights, word, drawn;  // what blocks tell one another: largest place, numbers, sums, a cut, the kept weights
   uint32_t n_list;
   long long fraction[64];  // bits of 2^(43 + i / 64)
-  uint64_t crest[THREADS], crest_own[THREADS];  // largest places of groups of threads: of all blocks, of this one
+  uint32_t crest[THREADS];  // largest keys of groups of this block's threads
 };
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -106,7 +109,7 @@ struct Row {
   int N, f32, first, share, held;
   int blocks, rank, crests;  // crests: groups of this block's threads
   uint32_t top;        // key of the largest logit
-  double m, scale;     // its value, 64 log2(e) / temperature
+  double m, scale, least_d;  // its value, 64 log2(e) / temperature, distance from which on a weight is 0
   float m32, bin_scale;
 
   // All blocks of the cluster, all threads.
@@ -124,14 +127,10 @@ struct Row {
   // 2^43 exp((l - max) / T) rounded to a whole number. y = 64 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 64) is 2^(n / 64), from a table of
   // the 64 fractions, times the series of exp(f ln(2) / 64) to the fourth power (off by 4e-14, less than half a unit). The sums that round are additions of a
   // power of two that leaves no bits behind the point.
+  // Straight-line, so that several go side by side; keys of -inf are nobody's to ask for.
   __device__ __forceinline__ uint64_t weight(uint32_t k) const {
-    if (k == top) return 1ull << 43;
-    if (k <= KEY_NONE || top >= KEY_INF) return 0;  // beside +inf nothing has a weight
-    // the float's bits as a double's (a subnormal one becomes another of no consequence)
-    const uint32_t b = __float_as_uint(of_key(k));
-    const double d = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29)) - m;
+    const double d = wide(bits_of_key(k)) - m;
     constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52
-    if (!(d * scale > -2880.0)) return 0;  // 2^-45
     const double t = fma(d, scale, WHOLE), f = fma(d, scale, WHOLE - t);
     const int n = __double2loint(t);
     constexpr double C = 0.69314718055994530942 / 64;
@@ -141,7 +140,8 @@ struct Row {
     p = fma(p, f, C);
     p = fma(p, f, 1.0);
     const long long two = s.fraction[n & 63] + ((long long)(n >> 6) << 52);  // 2^(43 + n / 64)
-    return (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0)) - 0x4330000000000000ull;
+    const uint64_t w = (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0)) - 0x4330000000000000ull;
+    return d > least_d ? w : 0;  // 2^-45
   }
   // Bins of equal width below the maximum, the last one for all that is further away; never falls with a falling logit.
   __device__ __forceinline__ int bin(uint32_t k) const {
@@ -156,10 +156,10 @@ __device__ __forceinline__ uint64_t block_sum64(uint64_t v, uint64_t* red) {
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  uint64_t s = 0;
+  v = red[threadIdx.x & (WARPS - 1)];
 #pragma unroll
-  for (int i = 0; i < WARPS; i++) s += red[i];
-  return s;
+  for (int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 // Sum of v over the threads in front of this one; *all: over all of them.
 __device__ __forceinline__ uint64_t block_before64(uint64_t v, uint64_t* red, uint64_t* all) {
@@ -173,17 +173,39 @@ __device__ __forceinline__ uint64_t block_before64(uint64_t v, uint64_t* red, ui
   __syncthreads();
   if (lane == 31) red[warp] = sum;
   __syncthreads();
-  uint64_t before = 0, total = 0;
+  uint64_t w = red[lane & (WARPS - 1)];
 #pragma unroll
-  for (int i = 0; i < WARPS; i++) {
-    if (i < warp) before += red[i];
-    total += red[i];
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  *all = total;
-  return before + sum - v;
+  *all = __shfl_sync(0xffffffffu, w, WARPS - 1);
+  const uint64_t front = __shfl_sync(0xffffffffu, w, max(0, warp - 1));
+  return (warp ? front : 0) + sum - v;
 }
 
-// The bin where a running sum over the bins (SUMS: of weights, otherwise of counts) reaches `want`; want == 0 and share_p >= 0: share_p of all the weights.
+// f(key, i) for the block's keys from low_key on; four at a time where they are in shared memory.
+template <typename F>
+__device__ __forceinline__ void each_key(const Row& r, uint32_t low_key, F&& f) {
+  const uint4* k4 = (const uint4*)r.keys;
+  const int quads = r.held / 4;
+#pragma unroll 1
+  for (int q = threadIdx.x; q < quads; q += THREADS) {
+    const uint4 k = k4[q];
+    if (max(max(k.x, k.y), max(k.z, k.w)) < low_key) continue;
+    f(k.x, q * 4, k.x >= low_key);
+    f(k.y, q * 4 + 1, k.y >= low_key);
+    f(k.z, q * 4 + 2, k.z >= low_key);
+    f(k.w, q * 4 + 3, k.w >= low_key);
+  }
+#pragma unroll 1
+  for (int i = quads * 4 + threadIdx.x; i < r.share; i += THREADS) {
+    const uint32_t k = r.key(i);
+    f(k, i, k >= low_key);
+  }
+}
+
+// The bin where a running sum over the bins (sums: of weights, otherwise of counts) reaches `want`. The first block's list is empty afterwards, and its place free.
 struct Crossing {
   int bin;
   uint64_t count;         // members of the bin
@@ -191,15 +213,15 @@ struct Crossing {
   uint64_t want;          // of the bin's own
   bool whole;             // the bin is kept as a whole
 };
-template <bool SUMS>
-__device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
+__device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want) {
   Shared& s = r.s;
   const int per = BINS / r.blocks;
+  if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
   r.meet();  // all bins are counted
   const uint32_t* counts = s.bin.count;
   auto sum_of = [&](int i) { return s.bin.sum[0][i] + ((uint64_t)s.bin.sum[1][i] << 15) + ((uint64_t)s.bin.sum[2][i] << 30); };
   int owner = 0;
-  uint64_t front_c = 0, front_s = 0, all_s = 0;
+  uint64_t front_c = 0, front_s = 0;
   if (r.blocks > 1) {
     uint64_t tc = 0, ts = 0;
     for (int i = threadIdx.x; i < per; i += THREADS) {
@@ -209,7 +231,7 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
       for (int b = 0; b < MAX_CLUSTER; b++)
         if (b < r.blocks) {
           c[b] = peer32(&s.bin.count[r.rank * per + i], b);
-          if (SUMS) {
+          if (sums) {
             const int at = r.rank * per + i;
             w[b] = peer32(&s.bin.sum[0][at], b) + ((uint64_t)peer32(&s.bin.sum[1][at], b) << 15) + ((uint64_t)peer32(&s.bin.sum[2][at], b) << 30);
           }
@@ -219,15 +241,15 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
       for (int b = 0; b < MAX_CLUSTER; b++)
         if (b < r.blocks) {
           cc += c[b];
-          if (SUMS) ww += w[b];
+          if (sums) ww += w[b];
         }
       s.part_count[i] = (uint32_t)cc;
-      if (SUMS) s.part_sum[i] = ww;
+      if (sums) s.part_sum[i] = ww;
       tc += cc;
       ts += ww;
     }
     tc = block_sum64(tc, s.red);
-    if (SUMS) ts = block_sum64(ts, s.red2);
+    if (sums) ts = block_sum64(ts, s.red2);
     if (threadIdx.x == 0) s.total_count = tc, s.total_sum = ts;
     r.meet();
     uint64_t c[MAX_CLUSTER], w[MAX_CLUSTER];
@@ -235,31 +257,16 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
     for (int b = 0; b < MAX_CLUSTER; b++)
       if (b < r.blocks) {
         c[b] = peer64(&s.total_count, b);
-        w[b] = SUMS ? peer64(&s.total_sum, b) : 0;
-        all_s += w[b];
+        w[b] = sums ? peer64(&s.total_sum, b) : 0;
       }
-    if (SUMS && share_p >= 0.f) {
-      bool lost;
-      *want = share_of(all_s, share_p, &lost);
-      *want += lost;
-      if (*want < 1) *want = 1;
-    }
     owner = r.blocks - 1;
     bool found = false;
 #pragma unroll
     for (int b = 0; b < MAX_CLUSTER; b++)
       if (b < r.blocks && !found) {
-        if ((SUMS ? front_s + w[b] : front_c + c[b]) >= *want) owner = b, found = true;
+        if ((sums ? front_s + w[b] : front_c + c[b]) >= want) owner = b, found = true;
         else front_c += c[b], front_s += w[b];
       }
-  } else if (SUMS && share_p >= 0.f) {
-    uint64_t ts = 0;
-    for (int i = threadIdx.x; i < per; i += THREADS) ts += sum_of(i);
-    all_s = block_sum64(ts, s.red2);
-    bool lost;
-    *want = share_of(all_s, share_p, &lost);
-    *want += lost;
-    if (*want < 1) *want = 1;
   }
   // the owner's part, two neighbouring bins per thread at most
   uint64_t c2[2] = {0, 0}, w2[2] = {0, 0};
@@ -269,21 +276,21 @@ __device__ Crossing cross(Row& r, uint64_t* want, float share_p) {
     const int i = threadIdx.x * each + e;
     if (e < each && i < per) {
       c2[e] = r.blocks > 1 ? peer32(&s.part_count[i], owner) : counts[i];
-      if (SUMS) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : sum_of(i);
+      if (sums) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : sum_of(i);
     }
   }
   uint64_t all, before_c = front_c + block_before64(c2[0] + c2[1], s.red, &all), before_s = 0;
-  if (SUMS) before_s = front_s + block_before64(w2[0] + w2[1], s.red2, &all);
+  if (sums) before_s = front_s + block_before64(w2[0] + w2[1], s.red2, &all);
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < 2; e++) {
-    const uint64_t here = SUMS ? w2[e] : c2[e], before = SUMS ? before_s : before_c;
-    if (e < each && before < *want && before + here >= *want) {  // one thread, once
+    const uint64_t here = sums ? w2[e] : c2[e], before = sums ? before_s : before_c;
+    if (e < each && before < want && before + here >= want) {  // one thread, once
       s.pick[0] = owner * per + threadIdx.x * each + e;
       s.pick[1] = c2[e];
       s.pick[2] = before_c;
-      s.pick[3] = *want - before;
-      s.pick[4] = SUMS ? c2[e] == 1 : here == *want - before;
+      s.pick[3] = want - before;
+      s.pick[4] = sums ? c2[e] == 1 : here == want - before;
     }
     before_c += c2[e];
     before_s += w2[e];
@@ -301,53 +308,34 @@ __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
   __syncthreads();
 }
 
-// A member into its bin. Where a warp's members all go to one bin (rows of equal logits, large temperatures) they go together.
-template <bool SUMS>
-__device__ __forceinline__ void add_to_bin(Shared& s, bool in, int b, uint64_t w) {
-  const unsigned who = __ballot_sync(0xffffffffu, in);
-  if (!who) return;
-  const int lead = __ffs(who) - 1, b0 = __shfl_sync(0xffffffffu, b, lead);
-  uint32_t n = 1;
-  if (__all_sync(0xffffffffu, !in || b == b0)) {
-    if (SUMS) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    }
-    n = __popc(who);
-    in = (threadIdx.x & 31) == lead;
-  }
-  if (!in) return;
-  atomicAdd(&s.bin.count[b], n);
-  if (SUMS && w) {  // at most 2^48
+__device__ __forceinline__ void add_to_bin(Shared& s, bool sums, int b, uint64_t w) {
+  atomicAdd(&s.bin.count[b], 1u);
+  if (sums) {
     atomicAdd(&s.bin.sum[0][b], (uint32_t)w & 0x7FFFu);
     atomicAdd(&s.bin.sum[1][b], (uint32_t)(w >> 15) & 0x7FFFu);
     atomicAdd(&s.bin.sum[2][b], (uint32_t)(w >> 30));
   }
 }
 
-// The members `of` chooses, from all blocks, into the first block's list (at most LIST of them).
-// AGAIN: the place of the list was in use.
-template <bool AGAIN, typename F>
-__device__ void gather(Row& r, F&& of) {
+// The members with keys from low_key on that `of` chooses, from all blocks, into the first block's list, which is empty (at most LIST of them).
+template <typename F>
+__device__ __forceinline__ void gather(const Row& r, uint32_t low_key, F&& of) {
   Shared& s = r.s;
-  if (AGAIN) {
-    r.meet();  // nobody reads bins any more
-    if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
-    r.meet();
-  }
-  for (int i = threadIdx.x; i < r.share; i += THREADS) {
-    const uint32_t k = r.key(i);
+  auto take = [&](int i, uint32_t k) {
     const uint64_t p = r.place(k, i);
-    if (!of(k, p)) continue;
+    if (!of(k, p)) return;
     uint32_t at;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(remote(&s.n_list, 0)) : "memory");
     if (at < LIST) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&s.list.place[at], 0)), "l"(p) : "memory");
-  }
+  };
+  each_key(r, low_key, [&](uint32_t k, int i, bool in) {
+    if (in) take(i, k);
+  });
   r.meet();
 }
 
 // Ranks of the list's members (the first block): by_rank. Threads share out the comparisons.
-__device__ void rank_list(Shared& s, int n) {
+__device__ __forceinline__ void rank_list(Shared& s, int n) {
   for (int i = threadIdx.x; i < n; i += THREADS) s.list.rank[i] = 0;
   __syncthreads();
   int wide = 1;
@@ -364,79 +352,24 @@ __device__ void rank_list(Shared& s, int n) {
   __syncthreads();
 }
 
-// Lowest place that is kept when the order is cut, among the places from `from` on: after `want` tokens, or (SUMS) where the weight in front reaches share_p of theirs.
-// *few: at most LIST places are kept, and the first block has them and the rest of their bin in its list, ranked; then the value is the cut for COUNTS and not
-// yet known for SUMS (*want: the weight to be reached).
-template <bool SUMS>
-__device__ uint64_t cut(Row& r, uint64_t from, uint64_t* want, float share_p, bool* few) {
-  Shared& s = r.s;
-  clear_bins(s, SUMS);
-  for (int i0 = 0; i0 < r.share; i0 += THREADS) {
-    const int i = i0 + threadIdx.x;
-    const uint32_t k = i < r.share ? r.key(i) : 0;
-    const bool in = i < r.share && r.place(k, i) >= from;
-    add_to_bin<SUMS>(s, in, in ? r.bin(k) : 0, SUMS && in ? r.weight(k) : 0);
-  }
-  Crossing c = cross<SUMS>(r, want, share_p);
-  const int b0 = c.bin;
-  *few = c.front + c.count <= LIST;
-  if (*few) {
-    gather<true>(r, [&](uint32_t k, uint64_t p) { return p >= from && r.bin(k) <= b0; });
-    if (r.rank == 0) rank_list(s, (int)s.n_list);
-    return 0;
-  }
-  uint64_t known = 0, low_place = 0;
-  int shift = 52;
-  bool done = false;
-  while (!done) {
-    if (c.whole && shift < 52) {  // of the bins of a digit: all that begin with it
-      low_place = known << shift;
-      break;
-    }
-    if (c.count <= LIST) {
-      const int sh = shift;
-      const uint64_t kn = known;
-      gather<true>(r, [&](uint32_t k, uint64_t p) { return p >= from && r.bin(k) == b0 && (sh == 52 || p >> sh == kn); });
-      if (r.rank == 0) {
-        const int n = (int)s.n_list;
-        rank_list(s, n);
-        if (!SUMS) {
-          if (threadIdx.x == 0) s.word = s.list.by_rank[c.want - 1];
-        } else {
-          for (int i = threadIdx.x; i < n; i += THREADS) s.list.w[i] = r.weight((uint32_t)(s.list.by_rank[i] >> 20));
-          __syncthreads();
-          uint64_t all;
-          const uint64_t w = threadIdx.x < n ? s.list.w[threadIdx.x] : 0, before = block_before64(w, s.red, &all);
-          if (before < c.want && before + w >= c.want) s.word = s.list.by_rank[threadIdx.x];
-        }
-      }
-      r.meet();
-      low_place = peer64(&s.word, 0);
-      r.meet();
-      break;
-    }
-    // more than LIST in one bin: by the next ten bits of the place
-    const int low = max(0, shift - 10), bits = shift - low;
-    r.meet();
-    clear_bins(s, SUMS);
-    for (int i0 = 0; i0 < r.share; i0 += THREADS) {
-      const int i = i0 + threadIdx.x;
-      const uint32_t k = i < r.share ? r.key(i) : 0;
-      const uint64_t p = r.place(k, i);
-      const bool in = i < r.share && p >= from && r.bin(k) == b0 && (shift == 52 || p >> shift == known);
-      const int d = (1 << bits) - 1 - ((int)(p >> low) & ((1 << bits) - 1));  // larger digits first
-      add_to_bin<SUMS>(s, in, in ? d : 0, SUMS && in ? r.weight(k) : 0);
-    }
-    uint64_t inner = c.want;
-    c = cross<SUMS>(r, &inner, -1.f);
-    known = (shift < 52 ? known << bits : 0) | (uint64_t)((1 << bits) - 1 - c.bin);
-    shift = low;
-  }
-  return low_place > from ? low_place : from;
+// Sum over the cluster of every thread's v; slot: a word of each block's that nothing else has used since the last two meetings.
+__device__ __forceinline__ uint64_t cluster_sum(const Row& r, uint64_t v, uint64_t* slot) {
+  v = block_sum64(v, r.s.red);
+  if (r.blocks == 1) return v;
+  if (threadIdx.x == 0) *slot = v;
+  r.meet();
+  uint64_t c[MAX_CLUSTER], sum = 0;
+#pragma unroll
+  for (int b = 0; b < MAX_CLUSTER; b++)
+    if (b < r.blocks) c[b] = peer64(slot, b);
+#pragma unroll
+  for (int b = 0; b < MAX_CLUSTER; b++)
+    if (b < r.blocks) sum += c[b];
+  return sum;
 }
 
 // The row's end in the first block, from its ranked list: `keep` of it are the kept beginning, or, with want > 0, those up to the weight `want`.
-__device__ void end_row(Row& r, const DrawArgs& a, int64_t row, int keep, uint64_t want, bool p_of_kept, float top_p, uint64_t least, float u) {
+__device__ __forceinline__ void end_row(const Row& r, const DrawArgs& a, int64_t row, int keep, uint64_t want, bool p_of_kept, float top_p, uint64_t least, float u) {
   Shared& s = r.s;
   const int n = min((int)s.n_list, keep), i = threadIdx.x;
   const uint64_t p = i < n ? s.list.by_rank[i] : 0;
@@ -500,12 +433,14 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   r.held = min(r.share, SHARE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  uint64_t best = 0, there = 0;  // the first of the order; how many are not -inf
+  uint32_t top_key = 0;
+  int top_at = 0;
+  auto seen = [&](uint32_t k, int i) {  // a thread's indices rise
+    if (k > top_key) top_key = k, top_at = i;
+  };
   auto take = [&](uint32_t k, int i) {
     if (i < r.held) keys[i] = k;
-    there += k > KEY_NONE;
-    const uint64_t p = r.place(k, i);
-    best = p > best ? p : best;
+    seen(k, i);
   };
   if (a.f32 && ((uintptr_t)((const float*)r.x + r.first) & 15) == 0) {
     const float4* x4 = (const float4*)((const float*)r.x + r.first);
@@ -519,10 +454,12 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
       for (int e = 0; e < AHEAD; e++) {
         const int i = (i0 + e * THREADS) * 4;
         if (i0 + e * THREADS < r.share / 4) {
-          take(key_of(v[e].x), i);
-          take(key_of(v[e].y), i + 1);
-          take(key_of(v[e].z), i + 2);
-          take(key_of(v[e].w), i + 3);
+          const uint4 k = make_uint4(key_of(v[e].x), key_of(v[e].y), key_of(v[e].z), key_of(v[e].w));
+          if (i + 3 < r.held) *(uint4*)(keys + i) = k;  // SHARE is a multiple of four
+          seen(k.x, i);
+          seen(k.y, i + 1);
+          seen(k.z, i + 2);
+          seen(k.w, i + 3);
         }
       }
     }
@@ -541,11 +478,12 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
 #pragma unroll 4
     for (int i = threadIdx.x; i < r.share; i += THREADS) take(r.load(i), i);
   }
+  uint64_t best = top_key ? r.place(top_key, top_at) : 0;
   // 512 groups in the cluster: threads of a block, or two, four or eight neighbours
   r.crests = THREADS / r.blocks;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    if (o == r.blocks && lane % o == 0) s.crest_own[threadIdx.x / o] = best;
+    if (o == r.blocks && lane % o == 0) s.crest[threadIdx.x / o] = (uint32_t)(best >> 20);
     const uint64_t v = __shfl_xor_sync(0xffffffffu, best, o);
     best = v > best ? v : best;
   }
@@ -554,20 +492,18 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
   for (int i = 0; i < WARPS; i++) best = s.red[i] > best ? s.red[i] : best;
-  there = block_sum64(there, s.red2);
-  if (threadIdx.x == 0) s.best = best, s.there = there;
+  if (threadIdx.x == 0) s.best = best;
   r.meet();
   if (r.blocks > 1) {
-    there = 0;
-    for (int b = 0; b < r.blocks; b++) {
-      const uint64_t v = peer64(&s.best, b);
-      best = v > best ? v : best;
-      there += peer64(&s.there, b);
-    }
+    uint64_t v[MAX_CLUSTER];
+#pragma unroll
+    for (int b = 0; b < MAX_CLUSTER; b++) v[b] = b < r.blocks ? peer64(&s.best, b) : 0;
+#pragma unroll
+    for (int b = 0; b < MAX_CLUSTER; b++) best = v[b] > best ? v[b] : best;
   }
   r.top = (uint32_t)(best >> 20);
   r.m32 = of_key(r.top);
-  r.m = r.m32;
+  r.m = wide(bits_of_key(r.top));
   const float heat = a.temperature ? a.temperature[row] : 1.f;
   if (r.top <= KEY_NONE || !(heat > 0.f)) {
     if (rank == 0 && threadIdx.x == 0) {
@@ -577,7 +513,9 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
     r.meet();
     return;
   }
-  r.scale = 64 * 1.4426950408889634074 / heat;
+  // beside +inf nothing has a weight
+  r.scale = r.top >= KEY_INF ? 1e30 : 64 * 1.4426950408889634074 / heat;
+  r.least_d = r.scale > 0 ? -2880.0 / r.scale : -1e300;
   r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
   if (r.top >= KEY_INF) r.m32 = 3.4028235e38f;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
   const int k = a.top_k ? a.top_k[row] : 0;
@@ -585,59 +523,138 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   const uint64_t least = min_p > 0.f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * ONE) : 0;
   float u = a.u[row];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+  // Two cuts, top_k's by counts and top_p's by weights, each unless nothing is asked of it. from: lowest place that is kept so far.
   uint64_t from = (uint64_t)(KEY_NONE + 1) << 20, want = 0;
-  bool few = false;
-  if (k > 0 && k < a.N && 4 * k <= r.blocks * r.crests) {
-    // The k-th largest of the groups' largest places has at least k places from it on, and, where the largest are not all in a few groups, not many more.
-    uint64_t* crest = s.crest;
-    const int n = r.blocks * r.crests;
-    uint64_t mine = 0;
-    if (threadIdx.x < n) mine = r.blocks > 1 ? peer64(&s.crest_own[threadIdx.x % r.crests], threadIdx.x / r.crests) : s.crest_own[threadIdx.x];
-    crest[threadIdx.x] = mine;
-    if (threadIdx.x == 0) s.pick[0] = 0;  // fewer than k groups have any
-    __syncthreads();
-    if (threadIdx.x < n) {
-      int above = 0;
-      for (int j = 0; j < n; j++) above += crest[j] > mine;
-      if (above == k - 1) s.pick[0] = mine;
+  bool few = false;  // the first block has the kept ones (and some more of the order) in its list, ranked
+  bool by_count = false;
+#pragma unroll 1
+  for (int stage = 0; stage < 2 && !few; stage++) {
+    const bool sums = stage == 1;
+    by_count = !sums;
+    uint32_t low_key = (uint32_t)(from >> 20);
+    if (!sums) {
+      if (k <= 0 || k >= a.N) continue;
+      if (2 * k <= THREADS) {
+        // The k-th largest of the groups' largest keys (to 22 bits, downwards) has at least k tokens from it on, and, where the largest are not all in a few
+        // groups, not many more.
+        const uint32_t mine = r.blocks > 1 ? peer32(&s.crest[threadIdx.x % r.crests], threadIdx.x / r.crests) : s.crest[threadIdx.x];
+        uint32_t low = 0;
+#pragma unroll 1
+        for (uint32_t bit = 1u << 31; bit >= 1u << 10; bit >>= 1)
+          if (__syncthreads_count(mine >= (low | bit)) >= k) low |= bit;
+        gather(r, max(low, KEY_NONE + 1), [](uint32_t, uint64_t) { return true; });
+        few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
+        if (few) {
+          if (r.rank == 0) rank_list(s, (int)s.n_list);
+          break;
+        }
+        r.meet();  // the number has been read
+      }
+      uint64_t there = 0;
+      each_key(r, KEY_NONE + 1, [&](uint32_t, int, bool in) { there += in; });
+      if ((uint64_t)k >= cluster_sum(r, there, &s.there)) continue;  // all that have any weight are kept
+      want = k;
+    } else {
+      if (!(top_p < 1.f)) continue;
+      uint64_t sum = 0;
+      each_key(r, low_key, [&](uint32_t key, int i, bool in) {
+        const uint64_t w = r.weight(key);
+        sum += in && r.place(key, i) >= from ? w : 0;
+      });
+      sum = cluster_sum(r, sum, &s.weights);
+      bool lost;
+      want = share_of(sum, top_p, &lost);
+      want = max((uint64_t)1, want + lost);
+      // All weights up to (sum - want) / N together are at most sum - want: the cut is above them, and keys that far down (a thousandth further) stay out of the bins.
+      const double tail = (double)(sum - want) / a.N;
+      if (tail > 0) {
+        const float reach = (float)(heat * log(ONE / tail) * 1.001) + fabsf(r.m32) * 1e-6f;
+        if (reach < 1e30f) low_key = max(low_key, key_of(r.m32 - reach));
+      }
     }
-    __syncthreads();
-    const uint64_t low = s.pick[0] > from ? s.pick[0] : from;
-    gather<false>(r, [&](uint32_t, uint64_t p) { return p >= low; });
-    few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
-    if (few && r.rank == 0) {
-      rank_list(s, (int)s.n_list);
-      end_row(r, a, row, k, 0, top_p < 1.f, top_p, least, u);
+    int b0 = 0, hi = 52;
+    uint64_t known = 0, left = want;
+    bool digits = false;  // within bin b0, where more than LIST share it: by the next ten bits of the place
+#pragma unroll 1
+    while (true) {
+      const int lo = max(0, hi - 10), mask = (1 << (hi - lo)) - 1;
+      clear_bins(s, sums);
+      each_key(r, low_key, [&](uint32_t key, int i, bool in) {
+        const uint64_t p = r.place(key, i), w = sums ? r.weight(key) : 0;
+        int b = r.bin(key);
+        in = in && p >= from;
+        if (digits) {
+          in = in && b == b0 && (hi == 52 || p >> hi == known);
+          b = mask - ((int)(p >> lo) & mask);  // larger digits first
+        }
+        if (in) add_to_bin(s, sums, b, w);
+      });
+      const Crossing c = cross(r, sums, left);
+      left = c.want;
+      if (digits) {
+        known = (hi < 52 ? known << (hi - lo) : 0) | (uint64_t)(mask - c.bin);
+        hi = lo;
+        if (c.whole) {  // all that begin with these bits
+          from = max(from, known << hi);
+          break;
+        }
+      } else {
+        b0 = c.bin;
+        few = c.front + c.count <= LIST;
+      }
+      if (few || c.count <= LIST) {
+        gather(r, low_key, [&](uint32_t key, uint64_t p) {
+          const int b = r.bin(key);
+          return p >= from && (few ? b <= b0 : b == b0 && (!digits || p >> hi == known));
+        });
+        if (r.rank == 0) {
+          const int n = (int)s.n_list;
+          rank_list(s, n);
+          if (!few && !sums && threadIdx.x == 0) s.word = s.list.by_rank[left - 1];
+          if (!few && sums) {
+            uint64_t all;
+            const uint64_t w = threadIdx.x < n ? r.weight((uint32_t)(s.list.by_rank[threadIdx.x] >> 20)) : 0, before = block_before64(w, s.red, &all);
+            if (before < left && before + w >= left) s.word = s.list.by_rank[threadIdx.x];
+          }
+        }
+        if (few) break;
+        r.meet();
+        from = max(from, peer64(&s.word, 0));
+        break;
+      }
+      digits = true;
     }
-    if (!few) r.meet();  // the number has been read
-  }
-  if (!few && k > 0 && k < a.N) {
-    want = k;
-    if (want < there) {  // otherwise all that have any weight are kept
-      from = cut<false>(r, from, &want, -1.f, &few);
-      if (few && r.rank == 0) end_row(r, a, row, k, 0, top_p < 1.f, top_p, least, u);
-    }
-  }
-  if (!few && top_p < 1.f) {
-    from = cut<true>(r, from, &want, fmaxf(top_p, 0.f), &few);
-    if (few && r.rank == 0) end_row(r, a, row, LIST, want, false, top_p, least, u);
   }
   if (few) {
+    if (r.rank == 0) {
+      end_row(r, a, row, by_count ? k : LIST, by_count ? 0 : want, by_count && top_p < 1.f, top_p, least, u);
+    }
     r.meet();
     return;
   }
   // The draw: a thread sums a contiguous part of the block's share (an odd number of keys, so that a warp's reads meet no bank twice), the sums in front of
   // it tell the one thread whose part holds the token, and its warp looks through that part.
   const int each_thread = (r.share + THREADS - 1) / THREADS | 1, i0 = min(r.share, (int)threadIdx.x * each_thread), i1 = min(r.share, i0 + each_thread);
+  const uint32_t from_key = (uint32_t)(from >> 20);
   auto kept = [&](int i) -> uint64_t {
     const uint32_t key = r.key(i);
-    if (r.place(key, i) < from) return 0;
+    if (key < from_key || r.place(key, i) < from) return 0;
     const uint64_t w = r.weight(key);
     return w >= least ? w : 0;
   };
   uint64_t mine = 0, block_total, total = 0;
-#pragma unroll 4
-  for (int i = i0; i < i1; i++) mine += kept(i);
+#pragma unroll 1
+  for (int i = i0; i < i1; i += 4) {
+    uint32_t key[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) key[e] = i + e < i1 ? r.key(i + e) : 0;
+    if (max(max(key[0], key[1]), max(key[2], key[3])) < from_key) continue;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint64_t w = r.weight(key[e]);
+      mine += key[e] >= from_key && r.place(key[e], i + e) >= from && w >= least ? w : 0;
+    }
+  }
   uint64_t before = block_before64(mine, s.red, &block_total);
   if (threadIdx.x == 0) s.drawn = block_total;
   r.meet();

@@ -25,9 +25,11 @@
 
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int GROUPS = 512;  // of threads of a cluster, whose largest keys bound the first of the order
 constexpr int BINS = 1024, LIST = 512;
-constexpr int SHARE = 19200;  // keys of a block in shared memory (75 KB, two blocks per SM); the rest of a longer row is read again in every pass
+// Keys of a block in shared memory: 75 KB where two blocks share an SM, 188 KB where one has it; the rest of a longer share is read again in every pass.
+template <int THREADS>
+constexpr int share_kept() { return THREADS == 512 ? 19200 : 48000; }
 constexpr int MAX_CLUSTER = 8;
 constexpr double ONE = 8796093022208.0;  // 2^43
 
@@ -66,7 +68,7 @@ struct Shared {
   union {
     struct {
       uint32_t count[BINS];
-      uint32_t sum[3][BINS];  // weights in pieces of 15 bits: counters of 32 bits are added to without a loop, and 2^17 members do not overflow them
+      uint32_t sum[4][BINS];  // weights in pieces of 11 bits: counters of 32 bits are added to without a loop, and 2^20 members do not overflow them
     } bin;
     struct {
       uint64_t place[LIST], w[LIST], by_rank[LIST];
@@ -77,12 +79,12 @@ struct Shared {
   uint32_t part_count[BINS / 2];
   uint64_t part_sum[BINS / 2];
   uint64_t total_count, total_sum;
-  uint64_t red[WARPS], red2[WARPS];
+  uint64_t red[32], red2[32];
   uint64_t pick[6];
   uint64_t best, there, weights, word, drawn;  // what blocks tell one another: largest place, numbers, sums, a cut, the kept weights
   uint32_t n_list;
   long long fraction[64];  // bits of 2^(43 + i / 64)
-  uint32_t crest[THREADS];  // largest keys of groups of this block's threads
+  uint32_t crest[GROUPS];  // largest keys of groups of this block's threads
 };
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -106,7 +108,7 @@ struct Row {
   Shared& s;
   const uint32_t* keys;  // of the first `held` of this block's `share`
   const void* x;
-  int N, f32, first, share, held;
+  int N, f32, vec, first, share, held;  // vec: rows begin at 16 bytes
   int blocks, rank, crests;  // crests: groups of this block's threads
   uint32_t top;        // key of the largest logit
   double m, scale, least_d;  // its value, 64 log2(e) / temperature, distance from which on a weight is 0
@@ -121,7 +123,21 @@ struct Row {
     const int64_t at = first + i;
     return key_of(f32 ? ((const float*)x)[at] : __bfloat162float(((const bf16*)x)[at]));
   }
-  __device__ __forceinline__ uint32_t key(int i) const { return i < held ? keys[i] : load(i); }
+  // Four keys from 4 q on, from memory (zeros behind the share), and from wherever they are.
+  __device__ __forceinline__ uint4 far(int q) const {
+    const int i = q * 4;
+    if (vec && i + 3 < share) {
+      if (f32) {
+        const float4 v = *(const float4*)((const float*)x + first + i);
+        return make_uint4(key_of(v.x), key_of(v.y), key_of(v.z), key_of(v.w));
+      }
+      const uint2 v = *(const uint2*)((const bf16*)x + first + i);
+      return make_uint4(key_of(__uint_as_float(v.x << 16)), key_of(__uint_as_float(v.x & 0xFFFF0000u)), key_of(__uint_as_float(v.y << 16)),
+                        key_of(__uint_as_float(v.y & 0xFFFF0000u)));
+    }
+    return make_uint4(i < share ? load(i) : 0, i + 1 < share ? load(i + 1) : 0, i + 2 < share ? load(i + 2) : 0, i + 3 < share ? load(i + 3) : 0);
+  }
+  __device__ __forceinline__ uint4 quad(int q) const { return q < held / 4 ? ((const uint4*)keys)[q] : far(q); }
   // the place in the row's order, larger is earlier: the key, then the lower index
   __device__ __forceinline__ uint64_t place(uint32_t k, int i) const { return (uint64_t)k << 20 | (uint32_t)(0xFFFFF - (first + i)); }
   // 2^43 exp((l - max) / T) rounded to a whole number. y = 64 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 64) is 2^(n / 64), from a table of
@@ -150,18 +166,20 @@ struct Row {
   }
 };
 
+template <int THREADS>
 __device__ __forceinline__ uint64_t block_sum64(uint64_t v, uint64_t* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = red[threadIdx.x & (WARPS - 1)];
+  v = red[threadIdx.x & ((THREADS / 32) - 1)];
 #pragma unroll
-  for (int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = (THREADS / 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 // Sum of v over the threads in front of this one; *all: over all of them.
+template <int THREADS>
 __device__ __forceinline__ uint64_t block_before64(uint64_t v, uint64_t* red, uint64_t* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t sum = v;
@@ -173,35 +191,35 @@ __device__ __forceinline__ uint64_t block_before64(uint64_t v, uint64_t* red, ui
   __syncthreads();
   if (lane == 31) red[warp] = sum;
   __syncthreads();
-  uint64_t w = red[lane & (WARPS - 1)];
+  uint64_t w = red[lane & ((THREADS / 32) - 1)];
 #pragma unroll
-  for (int o = 1; o < WARPS; o <<= 1) {
+  for (int o = 1; o < (THREADS / 32); o <<= 1) {
     const uint64_t y = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += y;
   }
-  *all = __shfl_sync(0xffffffffu, w, WARPS - 1);
+  *all = __shfl_sync(0xffffffffu, w, (THREADS / 32) - 1);
   const uint64_t front = __shfl_sync(0xffffffffu, w, max(0, warp - 1));
   return (warp ? front : 0) + sum - v;
 }
 
-// f(key, i) for the block's keys from low_key on; four at a time where they are in shared memory.
-template <typename F>
+// f(key, i, key >= low_key) for the block's keys, four at a time (0, below every low_key, behind the last); not for four that are all below.
+template <int THREADS, typename F>
 __device__ __forceinline__ void each_key(const Row& r, uint32_t low_key, F&& f) {
-  const uint4* k4 = (const uint4*)r.keys;
-  const int quads = r.held / 4;
-#pragma unroll 1
-  for (int q = threadIdx.x; q < quads; q += THREADS) {
-    const uint4 k = k4[q];
-    if (max(max(k.x, k.y), max(k.z, k.w)) < low_key) continue;
+  auto four = [&](const uint4& k, int q) {
+    if (max(max(k.x, k.y), max(k.z, k.w)) < low_key) return;
     f(k.x, q * 4, k.x >= low_key);
     f(k.y, q * 4 + 1, k.y >= low_key);
     f(k.z, q * 4 + 2, k.z >= low_key);
     f(k.w, q * 4 + 3, k.w >= low_key);
-  }
+  };
+  const int near = r.held / 4, all = (r.share + 3) / 4;
 #pragma unroll 1
-  for (int i = quads * 4 + threadIdx.x; i < r.share; i += THREADS) {
-    const uint32_t k = r.key(i);
-    f(k, i, k >= low_key);
+  for (int q = threadIdx.x; q < near; q += THREADS) four(((const uint4*)r.keys)[q], q);
+#pragma unroll 1
+  for (int q = near + threadIdx.x; q < all; q += 2 * THREADS) {  // two requests on their way
+    const uint4 k0 = r.far(q), k1 = r.far(q + THREADS);
+    four(k0, q);
+    four(k1, q + THREADS);
   }
 }
 
@@ -213,13 +231,16 @@ struct Crossing {
   uint64_t want;          // of the bin's own
   bool whole;             // the bin is kept as a whole
 };
+template <int THREADS>
 __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want) {
   Shared& s = r.s;
   const int per = BINS / r.blocks;
   if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
   r.meet();  // all bins are counted
   const uint32_t* counts = s.bin.count;
-  auto sum_of = [&](int i) { return s.bin.sum[0][i] + ((uint64_t)s.bin.sum[1][i] << 15) + ((uint64_t)s.bin.sum[2][i] << 30); };
+  auto sum_of = [&](int i) {
+    return s.bin.sum[0][i] + ((uint64_t)s.bin.sum[1][i] << 11) + ((uint64_t)s.bin.sum[2][i] << 22) + ((uint64_t)s.bin.sum[3][i] << 33);
+  };
   int owner = 0;
   uint64_t front_c = 0, front_s = 0;
   if (r.blocks > 1) {
@@ -233,7 +254,8 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
           c[b] = peer32(&s.bin.count[r.rank * per + i], b);
           if (sums) {
             const int at = r.rank * per + i;
-            w[b] = peer32(&s.bin.sum[0][at], b) + ((uint64_t)peer32(&s.bin.sum[1][at], b) << 15) + ((uint64_t)peer32(&s.bin.sum[2][at], b) << 30);
+            w[b] = peer32(&s.bin.sum[0][at], b) + ((uint64_t)peer32(&s.bin.sum[1][at], b) << 11) + ((uint64_t)peer32(&s.bin.sum[2][at], b) << 22) +
+                   ((uint64_t)peer32(&s.bin.sum[3][at], b) << 33);
           }
         }
       uint64_t cc = 0, ww = 0;
@@ -248,8 +270,8 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
       tc += cc;
       ts += ww;
     }
-    tc = block_sum64(tc, s.red);
-    if (sums) ts = block_sum64(ts, s.red2);
+    tc = block_sum64<THREADS>(tc, s.red);
+    if (sums) ts = block_sum64<THREADS>(ts, s.red2);
     if (threadIdx.x == 0) s.total_count = tc, s.total_sum = ts;
     r.meet();
     uint64_t c[MAX_CLUSTER], w[MAX_CLUSTER];
@@ -279,8 +301,8 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
       if (sums) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : sum_of(i);
     }
   }
-  uint64_t all, before_c = front_c + block_before64(c2[0] + c2[1], s.red, &all), before_s = 0;
-  if (sums) before_s = front_s + block_before64(w2[0] + w2[1], s.red2, &all);
+  uint64_t all, before_c = front_c + block_before64<THREADS>(c2[0] + c2[1], s.red, &all), before_s = 0;
+  if (sums) before_s = front_s + block_before64<THREADS>(w2[0] + w2[1], s.red2, &all);
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < 2; e++) {
@@ -299,11 +321,12 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
   return Crossing{(int)s.pick[0], s.pick[1], s.pick[2], s.pick[3], s.pick[4] != 0};
 }
 
+template <int THREADS>
 __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS) {
     s.bin.count[i] = 0;
-    if (sums) s.bin.sum[0][i] = s.bin.sum[1][i] = s.bin.sum[2][i] = 0;
+    if (sums) s.bin.sum[0][i] = s.bin.sum[1][i] = s.bin.sum[2][i] = s.bin.sum[3][i] = 0;
   }
   __syncthreads();
 }
@@ -311,14 +334,15 @@ __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
 __device__ __forceinline__ void add_to_bin(Shared& s, bool sums, int b, uint64_t w) {
   atomicAdd(&s.bin.count[b], 1u);
   if (sums) {
-    atomicAdd(&s.bin.sum[0][b], (uint32_t)w & 0x7FFFu);
-    atomicAdd(&s.bin.sum[1][b], (uint32_t)(w >> 15) & 0x7FFFu);
-    atomicAdd(&s.bin.sum[2][b], (uint32_t)(w >> 30));
+    atomicAdd(&s.bin.sum[0][b], (uint32_t)w & 0x7FFu);
+    atomicAdd(&s.bin.sum[1][b], (uint32_t)(w >> 11) & 0x7FFu);
+    atomicAdd(&s.bin.sum[2][b], (uint32_t)(w >> 22) & 0x7FFu);
+    atomicAdd(&s.bin.sum[3][b], (uint32_t)(w >> 33));
   }
 }
 
 // The members with keys from low_key on that `of` chooses, from all blocks, into the first block's list, which is empty (at most LIST of them).
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ void gather(const Row& r, uint32_t low_key, F&& of) {
   Shared& s = r.s;
   auto take = [&](int i, uint32_t k) {
@@ -328,23 +352,33 @@ __device__ __forceinline__ void gather(const Row& r, uint32_t low_key, F&& of) {
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(remote(&s.n_list, 0)) : "memory");
     if (at < LIST) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&s.list.place[at], 0)), "l"(p) : "memory");
   };
-  each_key(r, low_key, [&](uint32_t k, int i, bool in) {
+  each_key<THREADS>(r, low_key, [&](uint32_t k, int i, bool in) {
     if (in) take(i, k);
   });
   r.meet();
 }
 
-// Ranks of the list's members (the first block): by_rank. Threads share out the comparisons.
+// Ranks of the list's members (the first block): by_rank. Threads share out the comparisons, two a load.
+template <int THREADS>
 __device__ __forceinline__ void rank_list(Shared& s, int n) {
-  for (int i = threadIdx.x; i < n; i += THREADS) s.list.rank[i] = 0;
+  const int even = (n + 7) & ~7;
+  for (int i = threadIdx.x; i < LIST; i += THREADS) {
+    s.list.rank[i] = 0;
+    if (i >= n && i < even) s.list.place[i] = 0;
+  }
   __syncthreads();
-  int wide = 1;
+  int wide = 32;
   while (wide < n) wide <<= 1;
-  const int segs = THREADS / min(wide, THREADS), i = threadIdx.x % min(wide, THREADS), seg = threadIdx.x / min(wide, THREADS);
+  const int segs = THREADS / wide, i = threadIdx.x & (wide - 1), seg = threadIdx.x / wide;
   if (i < n) {
     const uint64_t p = s.list.place[i];
     uint32_t above = 0;
-    for (int j = seg; j < n; j += segs) above += s.list.place[j] > p;
+    const ulonglong2* two = (const ulonglong2*)s.list.place;
+#pragma unroll 4
+    for (int j = seg; j < even / 2; j += segs) {
+      const ulonglong2 q = two[j];
+      above += (q.x > p) + (q.y > p);
+    }
     if (above) atomicAdd(&s.list.rank[i], above);
   }
   __syncthreads();
@@ -352,9 +386,23 @@ __device__ __forceinline__ void rank_list(Shared& s, int n) {
   __syncthreads();
 }
 
+// The k-th largest of the groups' largest keys (to 22 bits, downwards) has at least k tokens from it on, and, where the largest are not all in a few
+// groups, not many more.
+template <int THREADS>
+__device__ __forceinline__ uint32_t crest_bound(const Row& r, int k) {
+  const int i = threadIdx.x;
+  const uint32_t mine = i >= GROUPS ? 0 : r.blocks > 1 ? peer32(&r.s.crest[i % r.crests], i / r.crests) : r.s.crest[i];
+  uint32_t low = 0;
+#pragma unroll 1
+  for (uint32_t bit = 1u << 31; bit >= 1u << 10; bit >>= 1)
+    if (__syncthreads_count(mine >= (low | bit)) >= k) low |= bit;
+  return max(low, KEY_NONE + 1);
+}
+
 // Sum over the cluster of every thread's v; slot: a word of each block's that nothing else has used since the last two meetings.
+template <int THREADS>
 __device__ __forceinline__ uint64_t cluster_sum(const Row& r, uint64_t v, uint64_t* slot) {
-  v = block_sum64(v, r.s.red);
+  v = block_sum64<THREADS>(v, r.s.red);
   if (r.blocks == 1) return v;
   if (threadIdx.x == 0) *slot = v;
   r.meet();
@@ -369,12 +417,13 @@ __device__ __forceinline__ uint64_t cluster_sum(const Row& r, uint64_t v, uint64
 }
 
 // The row's end in the first block, from its ranked list: `keep` of it are the kept beginning, or, with want > 0, those up to the weight `want`.
+template <int THREADS>
 __device__ __forceinline__ void end_row(const Row& r, const DrawArgs& a, int64_t row, int keep, uint64_t want, bool p_of_kept, float top_p, uint64_t least, float u) {
   Shared& s = r.s;
   const int n = min((int)s.n_list, keep), i = threadIdx.x;
   const uint64_t p = i < n ? s.list.by_rank[i] : 0;
   uint64_t w = i < n ? r.weight((uint32_t)(p >> 20)) : 0, all;
-  const uint64_t before = block_before64(w, s.red, &all);
+  const uint64_t before = block_before64<THREADS>(w, s.red, &all);
   if (p_of_kept) {  // top_p of what top_k kept
     bool lost;
     want = share_of(all, top_p, &lost);
@@ -384,37 +433,41 @@ __device__ __forceinline__ void end_row(const Row& r, const DrawArgs& a, int64_t
   if (want && before >= want) w = 0;
   if (w < least) w = 0;
   __syncthreads();
-  if (i < n) s.list.w[i] = w;
-  const uint64_t total = block_sum64(w, s.red2);
+  // kept ones are a beginning of the order: m of them
+  const int m = __syncthreads_count(w != 0), even = (m + 3) & ~3;
+  if (i < even) s.list.w[i] = i < m ? w : 0;
+  if (i < LIST) s.list.place[i] = 0;  // becomes the sum of the kept weights up to one's own index
+  const uint64_t total = block_sum64<THREADS>(w, s.red2);
   bool lost;
   const uint64_t target = share_of(total, u, &lost);
   if (i == 0) s.pick[0] = 0xFFFFFFFFull;
-  // sum of the kept weights up to one's own index
-  s.list.place[i] = 0;
   __syncthreads();
-  int wide = 1;
-  while (wide < n) wide <<= 1;
-  const int segs = THREADS / wide, me = i % wide, seg = i / wide;
-  if (me < n && s.list.w[me]) {
+  int wide = 32;
+  while (wide < m) wide <<= 1;
+  const int segs = THREADS / wide, me = i & (wide - 1), seg = i / wide;
+  if (me < m) {
     const uint32_t mine = (uint32_t)(s.list.by_rank[me] & 0xFFFFF);
     uint64_t sum = 0;
-    for (int j = seg; j < n; j += segs)
+#pragma unroll 4
+    for (int j = seg; j < even; j += segs)
       if ((uint32_t)(s.list.by_rank[j] & 0xFFFFF) >= mine) sum += s.list.w[j];  // not a higher index: places hold 2^20 - 1 - index
     if (sum) atomicAdd((unsigned long long*)&s.list.place[me], (unsigned long long)sum);
   }
   __syncthreads();
-  if (i < n && w && s.list.place[i] > target) atomicMin((unsigned long long*)&s.pick[0], (unsigned long long)(0xFFFFF - (p & 0xFFFFF)));
+  if (i < m && s.list.place[i] > target) atomicMin((unsigned long long*)&s.pick[0], (unsigned long long)(0xFFFFF - (p & 0xFFFFF)));
   __syncthreads();
-  if (i < n && w && (0xFFFFF - (p & 0xFFFFF)) == s.pick[0]) {
+  if (i < m && (0xFFFFF - (p & 0xFFFFF)) == s.pick[0]) {
     a.out[row] = (int32_t)s.pick[0];
     if (a.prob) a.prob[row] = (float)((double)w / (double)total);
   }
 }
 
-__global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant__ DrawArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __grid_constant__ DrawArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *(Shared*)smem;
-  uint32_t* keys = (uint32_t*)(smem + (sizeof(Shared) + 15) / 16 * 16);
+  uint32_t* queue = (uint32_t*)(smem + (sizeof(Shared) + 15) / 16 * 16);  // 64 keys of each warp
+  uint32_t* keys = queue + THREADS * 2;
   pdl_wait();
   pdl_trigger();
   uint32_t rank, blocks;
@@ -430,7 +483,8 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   r.rank = (int)rank;
   r.first = min(a.N, (int)rank * each);
   r.share = min(a.N - r.first, each);
-  r.held = min(r.share, SHARE);
+  r.held = min(r.share, share_kept<THREADS>()) & ~3;
+  r.vec = ((uintptr_t)r.x & 15) == 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   uint32_t top_key = 0;
@@ -438,52 +492,29 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   auto seen = [&](uint32_t k, int i) {  // a thread's indices rise
     if (k > top_key) top_key = k, top_at = i;
   };
-  auto take = [&](uint32_t k, int i) {
-    if (i < r.held) keys[i] = k;
-    seen(k, i);
-  };
-  if (a.f32 && ((uintptr_t)((const float*)r.x + r.first) & 15) == 0) {
-    const float4* x4 = (const float4*)((const float*)r.x + r.first);
-    constexpr int AHEAD = 5;  // SHARE / 4 / THREADS is 9.4
-    for (int i0 = threadIdx.x; i0 < r.share / 4; i0 += THREADS * AHEAD) {
-      float4 v[AHEAD];
+  constexpr int AHEAD = 5;
+#pragma unroll 1
+  for (int q0 = threadIdx.x; q0 < (r.share + 3) / 4; q0 += THREADS * AHEAD) {
+    uint4 k[AHEAD];
 #pragma unroll
-      for (int e = 0; e < AHEAD; e++)
-        if (i0 + e * THREADS < r.share / 4) v[e] = x4[i0 + e * THREADS];
+    for (int e = 0; e < AHEAD; e++) k[e] = r.far(q0 + e * THREADS);
 #pragma unroll
-      for (int e = 0; e < AHEAD; e++) {
-        const int i = (i0 + e * THREADS) * 4;
-        if (i0 + e * THREADS < r.share / 4) {
-          const uint4 k = make_uint4(key_of(v[e].x), key_of(v[e].y), key_of(v[e].z), key_of(v[e].w));
-          if (i + 3 < r.held) *(uint4*)(keys + i) = k;  // SHARE is a multiple of four
-          seen(k.x, i);
-          seen(k.y, i + 1);
-          seen(k.z, i + 2);
-          seen(k.w, i + 3);
-        }
-      }
+    for (int e = 0; e < AHEAD; e++) {
+      const int q = q0 + e * THREADS;
+      if (q < r.held / 4) ((uint4*)keys)[q] = k[e];
+      seen(k[e].x, q * 4);
+      seen(k[e].y, q * 4 + 1);
+      seen(k[e].z, q * 4 + 2);
+      seen(k[e].w, q * 4 + 3);
     }
-    for (int i = r.share / 4 * 4 + threadIdx.x; i < r.share; i += THREADS) take(r.load(i), i);
-  } else if (!a.f32 && ((uintptr_t)((const bf16*)r.x + r.first) & 15) == 0) {
-    const uint4* x8 = (const uint4*)((const bf16*)r.x + r.first);
-#pragma unroll 4
-    for (int i = threadIdx.x; i < r.share / 8; i += THREADS) {
-      const uint4 v = x8[i];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 8; e++) take(key_of(__uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16)), i * 8 + e);
-    }
-    for (int i = r.share / 8 * 8 + threadIdx.x; i < r.share; i += THREADS) take(r.load(i), i);
-  } else {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < r.share; i += THREADS) take(r.load(i), i);
   }
   uint64_t best = top_key ? r.place(top_key, top_at) : 0;
-  // 512 groups in the cluster: threads of a block, or two, four or eight neighbours
-  r.crests = THREADS / r.blocks;
+  // groups of neighbouring threads
+  r.crests = GROUPS / r.blocks;
+  const int group = THREADS / r.crests;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    if (o == r.blocks && lane % o == 0) s.crest[threadIdx.x / o] = (uint32_t)(best >> 20);
+    if (o == group && lane % o == 0) s.crest[threadIdx.x / o] = (uint32_t)(best >> 20);
     const uint64_t v = __shfl_xor_sync(0xffffffffu, best, o);
     best = v > best ? v : best;
   }
@@ -491,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   if (threadIdx.x == 0) s.n_list = 0;
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
-  for (int i = 0; i < WARPS; i++) best = s.red[i] > best ? s.red[i] : best;
+  for (int i = 0; i < (THREADS / 32); i++) best = s.red[i] > best ? s.red[i] : best;
   if (threadIdx.x == 0) s.best = best;
   r.meet();
   if (r.blocks > 1) {
@@ -534,37 +565,51 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
     uint32_t low_key = (uint32_t)(from >> 20);
     if (!sums) {
       if (k <= 0 || k >= a.N) continue;
-      if (2 * k <= THREADS) {
-        // The k-th largest of the groups' largest keys (to 22 bits, downwards) has at least k tokens from it on, and, where the largest are not all in a few
-        // groups, not many more.
-        const uint32_t mine = r.blocks > 1 ? peer32(&s.crest[threadIdx.x % r.crests], threadIdx.x / r.crests) : s.crest[threadIdx.x];
-        uint32_t low = 0;
-#pragma unroll 1
-        for (uint32_t bit = 1u << 31; bit >= 1u << 10; bit >>= 1)
-          if (__syncthreads_count(mine >= (low | bit)) >= k) low |= bit;
-        gather(r, max(low, KEY_NONE + 1), [](uint32_t, uint64_t) { return true; });
+      if (2 * k <= GROUPS) {
+        gather<THREADS>(r, crest_bound<THREADS>(r, k), [](uint32_t, uint64_t) { return true; });
         few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
         if (few) {
-          if (r.rank == 0) rank_list(s, (int)s.n_list);
+          if (r.rank == 0) rank_list<THREADS>(s, (int)s.n_list);
           break;
         }
         r.meet();  // the number has been read
       }
       uint64_t there = 0;
-      each_key(r, KEY_NONE + 1, [&](uint32_t, int, bool in) { there += in; });
-      if ((uint64_t)k >= cluster_sum(r, there, &s.there)) continue;  // all that have any weight are kept
+      each_key<THREADS>(r, KEY_NONE + 1, [&](uint32_t, int, bool in) { there += in; });
+      if ((uint64_t)k >= cluster_sum<THREADS>(r, there, &s.there)) continue;  // all that have any weight are kept
       want = k;
     } else {
       if (!(top_p < 1.f)) continue;
       uint64_t sum = 0;
-      each_key(r, low_key, [&](uint32_t key, int i, bool in) {
+      const bool by_key = (from & 0xFFFFF) == 0;
+      each_key<THREADS>(r, low_key, [&](uint32_t key, int i, bool in) {
         const uint64_t w = r.weight(key);
-        sum += in && r.place(key, i) >= from ? w : 0;
+        sum += in && (by_key || r.place(key, i) >= from) ? w : 0;
       });
-      sum = cluster_sum(r, sum, &s.weights);
+      sum = cluster_sum<THREADS>(r, sum, &s.weights);
       bool lost;
       want = share_of(sum, top_p, &lost);
       want = max((uint64_t)1, want + lost);
+      // The 256 largest and some more usually hold top_p.
+      if (k <= 0 || 2 * k > GROUPS) {
+        if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
+        const uint32_t low = max(low_key, crest_bound<THREADS>(r, GROUPS / 2));
+        r.meet();
+        gather<THREADS>(r, low, [&](uint32_t, uint64_t p) { return p >= from; });
+        if (r.rank == 0) {
+          const int n = (int)s.n_list;
+          uint64_t w = 0;
+          if (n <= LIST) w = block_sum64<THREADS>(threadIdx.x < n ? r.weight((uint32_t)(s.list.place[threadIdx.x] >> 20)) : 0, s.red);
+          if (threadIdx.x == 0) s.word = w >= want;
+        }
+        r.meet();
+        few = peer64(&s.word, 0);
+        if (few) {
+          if (r.rank == 0) rank_list<THREADS>(s, (int)s.n_list);
+          break;
+        }
+        r.meet();  // the word has been read
+      }
       // All weights up to (sum - want) / N together are at most sum - want: the cut is above them, and keys that far down (a thousandth further) stay out of the bins.
       const double tail = (double)(sum - want) / a.N;
       if (tail > 0) {
@@ -578,18 +623,46 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
 #pragma unroll 1
     while (true) {
       const int lo = max(0, hi - 10), mask = (1 << (hi - lo)) - 1;
-      clear_bins(s, sums);
-      each_key(r, low_key, [&](uint32_t key, int i, bool in) {
-        const uint64_t p = r.place(key, i), w = sums ? r.weight(key) : 0;
-        int b = r.bin(key);
-        in = in && p >= from;
-        if (digits) {
-          in = in && b == b0 && (hi == 52 || p >> hi == known);
-          b = mask - ((int)(p >> lo) & mask);  // larger digits first
+      clear_bins<THREADS>(s, sums);
+      if (digits) {
+        each_key<THREADS>(r, low_key, [&](uint32_t key, int i, bool in) {
+          const uint64_t p = r.place(key, i);
+          in = in && p >= from && r.bin(key) == b0 && (hi == 52 || p >> hi == known);
+          if (in) add_to_bin(s, sums, mask - ((int)(p >> lo) & mask), sums ? r.weight(key) : 0);  // larger digits first
+        });
+      } else {
+        // Often few keys go into bins, but some of nearly every warp's: they queue, and 32 at a time are weighed and added.
+        uint32_t* line = queue + warp * 64;
+        int n = 0;
+        auto weigh = [&](uint32_t key) { add_to_bin(s, sums, r.bin(key), sums ? r.weight(key) : 0); };
+        const bool by_key = (from & 0xFFFFF) == 0;  // `from` begins a key
+        const int all = (r.share + 3) / 4;
+#pragma unroll 1
+        for (int q0 = warp * 32; q0 < all; q0 += THREADS) {
+          const int q = q0 + lane;
+          const uint4 k = q < all ? r.quad(q) : make_uint4(0, 0, 0, 0);
+          if (!__any_sync(0xffffffffu, max(max(k.x, k.y), max(k.z, k.w)) >= low_key)) continue;
+          const uint32_t one[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const bool in = one[e] >= low_key && (by_key || r.place(one[e], q * 4 + e) >= from);
+            const unsigned who = __ballot_sync(0xffffffffu, in);
+            if (in) line[n + __popc(who & ((1u << lane) - 1))] = one[e];
+            n += __popc(who);
+            if (n >= 32) {
+              __syncwarp();
+              const uint32_t key = line[lane], next = line[32 + lane];
+              __syncwarp();
+              line[lane] = next;
+              n -= 32;
+              weigh(key);
+            }
+          }
         }
-        if (in) add_to_bin(s, sums, b, w);
-      });
-      const Crossing c = cross(r, sums, left);
+        __syncwarp();
+        if (lane < n) weigh(line[lane]);
+      }
+      const Crossing c = cross<THREADS>(r, sums, left);
       left = c.want;
       if (digits) {
         known = (hi < 52 ? known << (hi - lo) : 0) | (uint64_t)(mask - c.bin);
@@ -603,17 +676,19 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
         few = c.front + c.count <= LIST;
       }
       if (few || c.count <= LIST) {
-        gather(r, low_key, [&](uint32_t key, uint64_t p) {
+        // keys of bin b0 and in front of it, and a little more: the bin itself is looked at in what is left
+        const float deep = (b0 + 1.01f) / r.bin_scale + fabsf(r.m32) * 1e-6f;
+        gather<THREADS>(r, b0 < BINS - 1 && deep < 1e30f ? max(low_key, key_of(r.m32 - deep)) : low_key, [&](uint32_t key, uint64_t p) {
           const int b = r.bin(key);
           return p >= from && (few ? b <= b0 : b == b0 && (!digits || p >> hi == known));
         });
         if (r.rank == 0) {
           const int n = (int)s.n_list;
-          rank_list(s, n);
+          rank_list<THREADS>(s, n);
           if (!few && !sums && threadIdx.x == 0) s.word = s.list.by_rank[left - 1];
           if (!few && sums) {
             uint64_t all;
-            const uint64_t w = threadIdx.x < n ? r.weight((uint32_t)(s.list.by_rank[threadIdx.x] >> 20)) : 0, before = block_before64(w, s.red, &all);
+            const uint64_t w = threadIdx.x < n ? r.weight((uint32_t)(s.list.by_rank[threadIdx.x] >> 20)) : 0, before = block_before64<THREADS>(w, s.red, &all);
             if (before < left && before + w >= left) s.word = s.list.by_rank[threadIdx.x];
           }
         }
@@ -627,35 +702,42 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   }
   if (few) {
     if (r.rank == 0) {
-      end_row(r, a, row, by_count ? k : LIST, by_count ? 0 : want, by_count && top_p < 1.f, top_p, least, u);
+      end_row<THREADS>(r, a, row, by_count ? k : LIST, by_count ? 0 : want, by_count && top_p < 1.f, top_p, least, u);
     }
     r.meet();
     return;
   }
-  // The draw: a thread sums a contiguous part of the block's share (an odd number of keys, so that a warp's reads meet no bank twice), the sums in front of
-  // it tell the one thread whose part holds the token, and its warp looks through that part.
-  const int each_thread = (r.share + THREADS - 1) / THREADS | 1, i0 = min(r.share, (int)threadIdx.x * each_thread), i1 = min(r.share, i0 + each_thread);
+  // The draw: a warp sums pieces of 512 keys, the sums in front of the pieces tell which holds the token, and one warp looks through that piece.
   const uint32_t from_key = (uint32_t)(from >> 20);
-  auto kept = [&](int i) -> uint64_t {
-    const uint32_t key = r.key(i);
-    if (key < from_key || r.place(key, i) < from) return 0;
+  auto kept = [&](uint32_t key, int i) -> uint64_t {
     const uint64_t w = r.weight(key);
-    return w >= least ? w : 0;
+    return key >= from_key && r.place(key, i) >= from && w >= least ? w : 0;
   };
-  uint64_t mine = 0, block_total, total = 0;
+  auto kept4 = [&](const uint4& k, int q) -> uint64_t {
+    if (max(max(k.x, k.y), max(k.z, k.w)) < from_key) return 0;
+    return kept(k.x, q * 4) + kept(k.y, q * 4 + 1) + kept(k.z, q * 4 + 2) + kept(k.w, q * 4 + 3);
+  };
+  constexpr int PIECE = 128;  // quads
+  const int pieces = (r.share + 4 * PIECE - 1) / (4 * PIECE);
+  uint64_t* piece_sum = (uint64_t*)&s.bin;  // the bins are done with
+  static_assert(sizeof(s.bin) / 8 >= (1 << 20) / (4 * PIECE), "a sum for every piece of the longest share");
 #pragma unroll 1
-  for (int i = i0; i < i1; i += 4) {
-    uint32_t key[4];
+  for (int p = warp; p < pieces; p += THREADS / 32) {
+    uint4 k[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) key[e] = i + e < i1 ? r.key(i + e) : 0;
-    if (max(max(key[0], key[1]), max(key[2], key[3])) < from_key) continue;
+    for (int e = 0; e < 4; e++) k[e] = r.quad(p * PIECE + e * 32 + lane);
+    uint64_t sum = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const uint64_t w = r.weight(key[e]);
-      mine += key[e] >= from_key && r.place(key[e], i + e) >= from && w >= least ? w : 0;
-    }
+    for (int e = 0; e < 4; e++) sum += kept4(k[e], p * PIECE + e * 32 + lane);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) piece_sum[p] = sum;
   }
-  uint64_t before = block_before64(mine, s.red, &block_total);
+  __syncthreads();
+  const int each_thread = (pieces + THREADS - 1) / THREADS, p0 = threadIdx.x * each_thread;
+  uint64_t mine = 0, block_total, total = 0;
+  for (int p = p0; p < min(pieces, p0 + each_thread); p++) mine += piece_sum[p];
+  uint64_t before = block_before64<THREADS>(mine, s.red, &block_total);
   if (threadIdx.x == 0) s.drawn = block_total;
   r.meet();
   for (int b = 0; b < r.blocks; b++) {
@@ -666,12 +748,16 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
   r.meet();  // nobody leaves while its memory is read
   bool lost;
   const uint64_t target = share_of(total, u, &lost);
-  const unsigned mine_it_is = __ballot_sync(0xffffffffu, target >= before && target < before + mine);
-  if (!mine_it_is) return;
-  const int src = __ffs(mine_it_is) - 1, p0 = __shfl_sync(0xffffffffu, i0, src), p1 = __shfl_sync(0xffffffffu, i1, src);
+  const unsigned owner = __ballot_sync(0xffffffffu, target >= before && target < before + mine);
+  if (!owner) return;
+  const int src = __ffs(owner) - 1;
   before = __shfl_sync(0xffffffffu, before, src);
-  for (int i = p0; i < p1; i += 32) {
-    const uint64_t w = i + lane < p1 ? kept(i + lane) : 0;
+  int p = __shfl_sync(0xffffffffu, p0, src);
+  while (before + piece_sum[p] <= target) before += piece_sum[p++];
+#pragma unroll 1
+  for (int q = p * PIECE + lane; ; q += 32) {
+    const uint4 k = r.quad(q);
+    const uint64_t w = kept4(k, q);
     uint64_t sum = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -681,12 +767,24 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
     const unsigned hit = __ballot_sync(0xffffffffu, before + sum > target);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
-        a.out[row] = r.first + i + lane;
-        if (a.prob) a.prob[row] = (float)((double)w / (double)total);
+        uint64_t up_to = before + sum - w;
+        const uint32_t one[4] = {k.x, k.y, k.z, k.w};
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint64_t we = kept(one[e], q * 4 + e);
+          up_to += we;
+          if (!found && up_to > target) {
+            found = true;
+            a.out[row] = r.first + q * 4 + e;
+            if (a.prob) a.prob[row] = (float)((double)we / (double)total);
+          }
+        }
       }
       return;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
+    if (q - lane >= pieces * PIECE) return;  // not reached: the sums say that it is here
   }
 }
 
@@ -695,11 +793,20 @@ __global__ void __launch_bounds__(THREADS, 2) draw_kernel(const __grid_constant_
 int k_draw(strictb200_ctx* ctx, const void* x, int f32, int64_t M, int64_t N, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
            const float* top_p, const float* min_p, int32_t* out, float* prob) {
   const DrawArgs a{x, ld, (int)N, f32, u, temperature, top_p, min_p, top_k, out, prob};
-  int blocks = 1;  // of a row: as few as hold it, or eight
-  while (blocks < MAX_CLUSTER && N > (int64_t)blocks * SHARE) blocks *= 2;
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)std::min<int64_t>(SHARE, (N + blocks - 1) / blocks + 8) * 4;
+  // Few rows: eight blocks of 512 threads for a long one, fewer where they hold it. Many rows: blocks of 1024 threads that have an SM each, as few to a row as keeps the SMs busy.
+  int blocks = 1;
+  while (blocks < MAX_CLUSTER && N > (int64_t)blocks * share_kept<512>()) blocks *= 2;
+  const bool many = M * blocks > ctx->sm_count && blocks > 1;
+  if (many)
+    while (blocks > 1 && M * blocks > (blocks > 2 ? ctx->sm_count * 7 / 8 : ctx->sm_count)) blocks /= 2;  // clusters of four do not fill every SM
+  const size_t fixed = (sizeof(Shared) + 15) / 16 * 16;
+  const size_t smem = fixed + (many ? 1024 : 512) * 8 + (size_t)std::min<int64_t>(many ? share_kept<1024>() : share_kept<512>(), (N + blocks - 1) / blocks + 8) * 4;
+  const auto kernel = many ? draw_kernel<1024> : draw_kernel<512>;
   static SbDeviceOnce once;
-  SB_CUDA(once.run(ctx->device, [&] { return cudaFuncSetAttribute(draw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((sizeof(Shared) + 15) / 16 * 16 + SHARE * 4)); }));
+  SB_CUDA(once.run(ctx->device, [&] {
+    const cudaError_t e = cudaFuncSetAttribute(draw_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fixed + 512 * 8 + share_kept<512>() * 4);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(draw_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fixed + 1024 * 8 + share_kept<1024>() * 4);
+  }));
   // rows of one launch: as many as the grid takes
   const int64_t most = INT32_MAX / blocks;
   for (int64_t m0 = 0; m0 < M; m0 += most) {
@@ -712,7 +819,7 @@ int k_draw(strictb200_ctx* ctx, const void* x, int f32, int64_t M, int64_t N, in
     if (min_p) part.min_p += m0;
     part.out += m0;
     if (prob) part.prob += m0;
-    SB_CUDA(sb_launch_cluster(ctx, draw_kernel, dim3((unsigned)(std::min(M - m0, most) * blocks)), dim3(THREADS), smem, dim3((unsigned)blocks), part));
+    SB_CUDA(sb_launch_cluster(ctx, kernel, dim3((unsigned)(std::min(M - m0, most) * blocks)), dim3(many ? 1024 : 512), smem, dim3((unsigned)blocks), part));
     ctx->launches++;
   }
   return STRICTB200_OK;

@@ -71,8 +71,7 @@ struct Shared {
       uint32_t sum[4][BINS];  // weights in pieces of 11 bits: counters of 32 bits are added to without a loop, and 2^20 members do not overflow them
     } bin;
     struct {
-      uint64_t place[LIST], w[LIST], by_rank[LIST];
-      uint32_t rank[LIST];
+      uint64_t place[LIST], by_rank[LIST];
     } list;
   };
   // sums over the cluster of this block's part of the bins (whole for a cluster of one)
@@ -83,7 +82,7 @@ struct Shared {
   uint64_t pick[6];
   uint64_t best, there, weights, word, drawn;  // what blocks tell one another: largest place, numbers, sums, a cut, the kept weights
   uint32_t n_list;
-  long long fraction[64];  // bits of 2^(43 + i / 64)
+  long long fraction[256];  // bits of 2^(43 + i / 256)
   uint32_t crest[GROUPS];  // largest keys of groups of this block's threads
 };
 
@@ -111,7 +110,7 @@ struct Row {
   int N, f32, vec, first, share, held;  // vec: rows begin at 16 bytes
   int blocks, rank, crests;  // crests: groups of this block's threads
   uint32_t top;        // key of the largest logit
-  double m, scale, least_d;  // its value, 64 log2(e) / temperature, distance from which on a weight is 0
+  double m, scale, least_d;  // its value, 256 log2(e) / temperature, distance from which on a weight is 0
   float m32, bin_scale;
 
   // All blocks of the cluster, all threads.
@@ -140,8 +139,8 @@ struct Row {
   __device__ __forceinline__ uint4 quad(int q) const { return q < held / 4 ? ((const uint4*)keys)[q] : far(q); }
   // the place in the row's order, larger is earlier: the key, then the lower index
   __device__ __forceinline__ uint64_t place(uint32_t k, int i) const { return (uint64_t)k << 20 | (uint32_t)(0xFFFFF - (first + i)); }
-  // 2^43 exp((l - max) / T) rounded to a whole number. y = 64 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 64) is 2^(n / 64), from a table of
-  // the 64 fractions, times the series of exp(f ln(2) / 64) to the fourth power (off by 4e-14, less than half a unit). The sums that round are additions of a
+  // 2^43 exp((l - max) / T) rounded to a whole number. y = 256 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 256) is 2^(n / 256), from a table
+  // of the 256 fractions, times the series of exp(f ln(2) / 256) to the third power (off by 1.4e-13 of the weight, 1.2 units at most). The sums that round are additions of a
   // power of two that leaves no bits behind the point.
   // Straight-line, so that several go side by side; keys of -inf are nobody's to ask for.
   __device__ __forceinline__ uint64_t weight(uint32_t k) const {
@@ -149,13 +148,12 @@ struct Row {
     constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52
     const double t = fma(d, scale, WHOLE), f = fma(d, scale, WHOLE - t);
     const int n = __double2loint(t);
-    constexpr double C = 0.69314718055994530942 / 64;
-    double p = C * C * C * C / 24;
-    p = fma(p, f, C * C * C / 6);
+    constexpr double C = 0.69314718055994530942 / 256;
+    double p = C * C * C / 6;
     p = fma(p, f, C * C / 2);
     p = fma(p, f, C);
     p = fma(p, f, 1.0);
-    const long long two = s.fraction[n & 63] + ((long long)(n >> 6) << 52);  // 2^(43 + n / 64)
+    const long long two = s.fraction[n & 255] + ((long long)(n >> 8) << 52);  // 2^(43 + n / 256)
     const uint64_t w = (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0)) - 0x4330000000000000ull;
     return d > least_d ? w : 0;  // 2^-45
   }
@@ -245,30 +243,28 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
   uint64_t front_c = 0, front_s = 0;
   if (r.blocks > 1) {
     uint64_t tc = 0, ts = 0;
-    for (int i = threadIdx.x; i < per; i += THREADS) {
-      uint32_t c[MAX_CLUSTER];
-      uint64_t w[MAX_CLUSTER];
-#pragma unroll
-      for (int b = 0; b < MAX_CLUSTER; b++)
-        if (b < r.blocks) {
-          c[b] = peer32(&s.bin.count[r.rank * per + i], b);
-          if (sums) {
-            const int at = r.rank * per + i;
-            w[b] = peer32(&s.bin.sum[0][at], b) + ((uint64_t)peer32(&s.bin.sum[1][at], b) << 11) + ((uint64_t)peer32(&s.bin.sum[2][at], b) << 22) +
-                   ((uint64_t)peer32(&s.bin.sum[3][at], b) << 33);
-          }
-        }
-      uint64_t cc = 0, ww = 0;
-#pragma unroll
-      for (int b = 0; b < MAX_CLUSTER; b++)
-        if (b < r.blocks) {
-          cc += c[b];
-          if (sums) ww += w[b];
-        }
-      s.part_count[i] = (uint32_t)cc;
+    // the threads of a bin (THREADS / per of them, one or more neighbours) read from every that-many-th block
+    const int readers = THREADS / per, i = threadIdx.x / readers;
+    uint32_t cc = 0;
+    uint64_t ww = 0;
+    for (int b = threadIdx.x % readers; b < r.blocks; b += readers) {
+      const int at = r.rank * per + i;
+      const uint32_t c0 = peer32(&s.bin.count[at], b);
+      if (sums) {
+        const uint64_t w0 = peer32(&s.bin.sum[0][at], b), w1 = peer32(&s.bin.sum[1][at], b), w2 = peer32(&s.bin.sum[2][at], b), w3 = peer32(&s.bin.sum[3][at], b);
+        ww += w0 + (w1 << 11) + (w2 << 22) + (w3 << 33);
+      }
+      cc += c0;
+    }
+    for (int o = 1; o < readers; o <<= 1) {
+      cc += __shfl_xor_sync(0xffffffffu, cc, o);
+      if (sums) ww += __shfl_xor_sync(0xffffffffu, ww, o);
+    }
+    if (threadIdx.x % readers == 0) {
+      s.part_count[i] = cc;
       if (sums) s.part_sum[i] = ww;
-      tc += cc;
-      ts += ww;
+      tc = cc;
+      ts = ww;
     }
     tc = block_sum64<THREADS>(tc, s.red);
     if (sums) ts = block_sum64<THREADS>(ts, s.red2);
@@ -358,31 +354,39 @@ __device__ __forceinline__ void gather(const Row& r, uint32_t low_key, F&& of) {
   r.meet();
 }
 
-// Ranks of the list's members (the first block): by_rank. Threads share out the comparisons, two a load.
+// Values of threads 0 .. n - 1 in falling order (a bitonic network over the next power of two; the others hold 0 and get what is left): thread i's is returned.
+// Steps between lanes by shuffles, between warps through `line` (LIST values). All threads of the block.
+template <int THREADS>
+__device__ __forceinline__ uint64_t sorted(uint64_t v, int n, uint64_t* line) {
+  const int i = threadIdx.x;
+  int wide = 2;
+  while (wide < n) wide <<= 1;
+#pragma unroll 1
+  for (int size = 2; size <= wide; size <<= 1)
+#pragma unroll 1
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      uint64_t other;
+      if (step >= 32) {
+        __syncthreads();
+        if (i < LIST) line[i] = v;
+        __syncthreads();
+        other = i < LIST ? line[i ^ step] : 0;
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, v, step);
+      }
+      const bool larger = ((i & size) == 0) == ((i & step) == 0);  // this end of the pair keeps the larger
+      v = larger == (v > other) ? v : other;
+    }
+  __syncthreads();
+  return v;
+}
+
+// The list's members (the first block) in the order of their places: by_rank.
 template <int THREADS>
 __device__ __forceinline__ void rank_list(Shared& s, int n) {
-  const int even = (n + 7) & ~7;
-  for (int i = threadIdx.x; i < LIST; i += THREADS) {
-    s.list.rank[i] = 0;
-    if (i >= n && i < even) s.list.place[i] = 0;
-  }
-  __syncthreads();
-  int wide = 32;
-  while (wide < n) wide <<= 1;
-  const int segs = THREADS / wide, i = threadIdx.x & (wide - 1), seg = threadIdx.x / wide;
-  if (i < n) {
-    const uint64_t p = s.list.place[i];
-    uint32_t above = 0;
-    const ulonglong2* two = (const ulonglong2*)s.list.place;
-#pragma unroll 4
-    for (int j = seg; j < even / 2; j += segs) {
-      const ulonglong2 q = two[j];
-      above += (q.x > p) + (q.y > p);
-    }
-    if (above) atomicAdd(&s.list.rank[i], above);
-  }
-  __syncthreads();
-  for (int j = threadIdx.x; j < n; j += THREADS) s.list.by_rank[s.list.rank[j]] = s.list.place[j];
+  const int i = threadIdx.x;
+  const uint64_t p = sorted<THREADS>(i < n ? s.list.place[i] : 0, n, s.list.by_rank);
+  if (i < LIST) s.list.by_rank[i] = p;
   __syncthreads();
 }
 
@@ -433,32 +437,16 @@ __device__ __forceinline__ void end_row(const Row& r, const DrawArgs& a, int64_t
   if (want && before >= want) w = 0;
   if (w < least) w = 0;
   __syncthreads();
-  // kept ones are a beginning of the order: m of them
-  const int m = __syncthreads_count(w != 0), even = (m + 3) & ~3;
-  if (i < even) s.list.w[i] = i < m ? w : 0;
-  if (i < LIST) s.list.place[i] = 0;  // becomes the sum of the kept weights up to one's own index
+  // in the order of the indices, which falling (2^20 - 1 - index, weight) is: 20 bits and 44
+  const int kept = __syncthreads_count(w != 0);
   const uint64_t total = block_sum64<THREADS>(w, s.red2);
   bool lost;
   const uint64_t target = share_of(total, u, &lost);
-  if (i == 0) s.pick[0] = 0xFFFFFFFFull;
-  __syncthreads();
-  int wide = 32;
-  while (wide < m) wide <<= 1;
-  const int segs = THREADS / wide, me = i & (wide - 1), seg = i / wide;
-  if (me < m) {
-    const uint32_t mine = (uint32_t)(s.list.by_rank[me] & 0xFFFFF);
-    uint64_t sum = 0;
-#pragma unroll 4
-    for (int j = seg; j < even; j += segs)
-      if ((uint32_t)(s.list.by_rank[j] & 0xFFFFF) >= mine) sum += s.list.w[j];  // not a higher index: places hold 2^20 - 1 - index
-    if (sum) atomicAdd((unsigned long long*)&s.list.place[me], (unsigned long long)sum);
-  }
-  __syncthreads();
-  if (i < m && s.list.place[i] > target) atomicMin((unsigned long long*)&s.pick[0], (unsigned long long)(0xFFFFF - (p & 0xFFFFF)));
-  __syncthreads();
-  if (i < m && (0xFFFFF - (p & 0xFFFFF)) == s.pick[0]) {
-    a.out[row] = (int32_t)s.pick[0];
-    if (a.prob) a.prob[row] = (float)((double)w / (double)total);
+  const uint64_t member = sorted<THREADS>(w ? (p & 0xFFFFF) << 44 | w : 0, kept, s.list.place);  // the kept ones are a beginning of the order
+  const uint64_t mine = member & ((1ull << 44) - 1), front = block_before64<THREADS>(mine, s.red, &all);
+  if (front <= target && front + mine > target) {  // one thread
+    a.out[row] = 0xFFFFF - (int)(member >> 44);
+    if (a.prob) a.prob[row] = (float)((double)mine / (double)total);
   }
 }
 
@@ -518,7 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     const uint64_t v = __shfl_xor_sync(0xffffffffu, best, o);
     best = v > best ? v : best;
   }
-  if (threadIdx.x < 64) s.fraction[threadIdx.x] = __double_as_longlong(exp2(43.0 + threadIdx.x / 64.0));
+  if (threadIdx.x < 256) s.fraction[threadIdx.x] = __double_as_longlong(exp2(43.0 + threadIdx.x / 256.0));
   if (threadIdx.x == 0) s.n_list = 0;
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
@@ -545,8 +533,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     return;
   }
   // beside +inf nothing has a weight
-  r.scale = r.top >= KEY_INF ? 1e30 : 64 * 1.4426950408889634074 / heat;
-  r.least_d = r.scale > 0 ? -2880.0 / r.scale : -1e300;
+  r.scale = r.top >= KEY_INF ? 1e30 : 256 * 1.4426950408889634074 / heat;
+  r.least_d = r.scale > 0 ? -11520.0 / r.scale : -1e300;
   r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
   if (r.top >= KEY_INF) r.m32 = 3.4028235e38f;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
   const int k = a.top_k ? a.top_k[row] : 0;

@@ -8,7 +8,7 @@
 // result depends on the order in which threads add, and a comparison with a sum falls as it does in 64-bit arithmetic except where the two sides agree
 // to about 2^-40 of the largest weight.
 //
-// A row is read from memory once: a cluster of up to eight blocks holds it in shared memory (as ordered keys) and passes over it there. What bounds a row is
+// A row is read from memory once: a cluster of up to eight blocks holds it in shared memory and passes over it there. What bounds a row is
 // the chain of passes and of meetings of the cluster, two to four microseconds each pair:
 //   load, maximum, largest places of 512 groups of threads                                             one meeting
 //   top_k of up to 256: the k-th largest of those groups' places bounds the first k tokens from below, and what lies above it, seldom more than
@@ -43,19 +43,19 @@ struct DrawArgs {
   float* prob;
 };
 
-// Larger logits have larger keys; NaN counts as -inf, -0 as 0.
+// Larger logits have larger keys; -0 counts as 0. NaN counts as -inf: it is left out by every comparison and has no key.
 __device__ __forceinline__ uint32_t key_of(float l) {
-  const uint32_t b = __float_as_uint(l != l ? -INFINITY : l + 0.f);
+  const uint32_t b = __float_as_uint(l + 0.f);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ uint32_t bits_of_key(uint32_t k) { return k ^ (~(uint32_t)((int32_t)k >> 31) | 0x80000000u); }
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(bits_of_key(k)); }
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ (~(uint32_t)((int32_t)k >> 31) | 0x80000000u)); }
+__device__ __forceinline__ float of_place(uint64_t p) { return of_key((uint32_t)(p >> 20)); }
 // A float's bits as a double's: exact for normal numbers, infinities become 2^128 (further than any number), subnormal ones others of no consequence.
 __device__ __forceinline__ double wide(uint32_t b) {
   return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
 }
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // of -inf
-constexpr uint32_t KEY_INF = 0xFF800000u;
+constexpr float LEAST = -3.402823466e38f;  // of the logits that can be drawn
 
 // f * x, f in [0, 1), rounded down, and whether something was lost
 __device__ __forceinline__ uint64_t share_of(uint64_t x, float f, bool* lost) {
@@ -105,12 +105,11 @@ __device__ __forceinline__ uint32_t peer32(const uint32_t* p, int rank) {
 
 struct Row {
   Shared& s;
-  const uint32_t* keys;  // of the first `held` of this block's `share`
+  const float* near;  // the first `held` of this block's `share` of the logits
   const void* x;
   int N, f32, vec, first, share, held;  // vec: rows begin at 16 bytes
   int blocks, rank, crests;  // crests: groups of this block's threads
-  uint32_t top;        // key of the largest logit
-  double m, scale, least_d;  // its value, 256 log2(e) / temperature, distance from which on a weight is 0
+  double m, scale, least_d;  // the largest logit, 256 log2(e) / temperature, distance from which on a weight is 0
   float m32, bin_scale;
 
   // All blocks of the cluster, all threads.
@@ -118,33 +117,30 @@ struct Row {
     __syncthreads();
     if (blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  __device__ __forceinline__ uint32_t load(int i) const {  // of the block's i-th
+  __device__ __forceinline__ float load(int i) const {  // the block's i-th logit
     const int64_t at = first + i;
-    return key_of(f32 ? ((const float*)x)[at] : __bfloat162float(((const bf16*)x)[at]));
+    return f32 ? ((const float*)x)[at] : __bfloat162float(((const bf16*)x)[at]);
   }
-  // Four keys from 4 q on, from memory (zeros behind the share), and from wherever they are.
-  __device__ __forceinline__ uint4 far(int q) const {
+  // Four logits from 4 q on, from memory (-inf behind the share), and from wherever they are.
+  __device__ __forceinline__ float4 far(int q) const {
     const int i = q * 4;
     if (vec && i + 3 < share) {
-      if (f32) {
-        const float4 v = *(const float4*)((const float*)x + first + i);
-        return make_uint4(key_of(v.x), key_of(v.y), key_of(v.z), key_of(v.w));
-      }
+      if (f32) return *(const float4*)((const float*)x + first + i);
       const uint2 v = *(const uint2*)((const bf16*)x + first + i);
-      return make_uint4(key_of(__uint_as_float(v.x << 16)), key_of(__uint_as_float(v.x & 0xFFFF0000u)), key_of(__uint_as_float(v.y << 16)),
-                        key_of(__uint_as_float(v.y & 0xFFFF0000u)));
+      return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
     }
-    return make_uint4(i < share ? load(i) : 0, i + 1 < share ? load(i + 1) : 0, i + 2 < share ? load(i + 2) : 0, i + 3 < share ? load(i + 3) : 0);
+    return make_float4(i < share ? load(i) : -INFINITY, i + 1 < share ? load(i + 1) : -INFINITY, i + 2 < share ? load(i + 2) : -INFINITY,
+                       i + 3 < share ? load(i + 3) : -INFINITY);
   }
-  __device__ __forceinline__ uint4 quad(int q) const { return q < held / 4 ? ((const uint4*)keys)[q] : far(q); }
+  __device__ __forceinline__ float4 quad(int q) const { return q < held / 4 ? ((const float4*)near)[q] : far(q); }
   // the place in the row's order, larger is earlier: the key, then the lower index
-  __device__ __forceinline__ uint64_t place(uint32_t k, int i) const { return (uint64_t)k << 20 | (uint32_t)(0xFFFFF - (first + i)); }
+  __device__ __forceinline__ uint64_t place(float l, int i) const { return (uint64_t)key_of(l) << 20 | (uint32_t)(0xFFFFF - (first + i)); }
   // 2^43 exp((l - max) / T) rounded to a whole number. y = 256 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 256) is 2^(n / 256), from a table
   // of the 256 fractions, times the series of exp(f ln(2) / 256) to the third power (off by 1.4e-13 of the weight, 1.2 units at most). The sums that round are additions of a
   // power of two that leaves no bits behind the point.
-  // Straight-line, so that several go side by side; keys of -inf are nobody's to ask for.
-  __device__ __forceinline__ uint64_t weight(uint32_t k) const {
-    const double d = wide(bits_of_key(k)) - m;
+  // Straight-line, so that several go side by side; of -inf and NaN nobody asks.
+  __device__ __forceinline__ uint64_t weight(float l) const {
+    const double d = wide(__float_as_uint(l)) - m;
     constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52
     const double t = fma(d, scale, WHOLE), f = fma(d, scale, WHOLE - t);
     const int n = __double2loint(t);
@@ -158,8 +154,8 @@ struct Row {
     return d > least_d ? w : 0;  // 2^-45
   }
   // Bins of equal width below the maximum, the last one for all that is further away; never falls with a falling logit.
-  __device__ __forceinline__ int bin(uint32_t k) const {
-    const float d = (m32 - of_key(k)) * bin_scale;
+  __device__ __forceinline__ int bin(float l) const {
+    const float d = (m32 - l) * bin_scale;
     return d < (float)(BINS - 1) ? max(0, (int)d) : BINS - 1;
   }
 };
@@ -200,24 +196,24 @@ __device__ __forceinline__ uint64_t block_before64(uint64_t v, uint64_t* red, ui
   return (warp ? front : 0) + sum - v;
 }
 
-// f(key, i, key >= low_key) for the block's keys, four at a time (0, below every low_key, behind the last); not for four that are all below.
+// f(l, i, l >= low) for the block's logits, four at a time (-inf behind the last); not for four that are all below.
 template <int THREADS, typename F>
-__device__ __forceinline__ void each_key(const Row& r, uint32_t low_key, F&& f) {
-  auto four = [&](const uint4& k, int q) {
-    if (max(max(k.x, k.y), max(k.z, k.w)) < low_key) return;
-    f(k.x, q * 4, k.x >= low_key);
-    f(k.y, q * 4 + 1, k.y >= low_key);
-    f(k.z, q * 4 + 2, k.z >= low_key);
-    f(k.w, q * 4 + 3, k.w >= low_key);
+__device__ __forceinline__ void each(const Row& r, float low, F&& f) {
+  auto four = [&](const float4& v, int q) {
+    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= low)) return;
+    f(v.x, q * 4, v.x >= low);
+    f(v.y, q * 4 + 1, v.y >= low);
+    f(v.z, q * 4 + 2, v.z >= low);
+    f(v.w, q * 4 + 3, v.w >= low);
   };
   const int near = r.held / 4, all = (r.share + 3) / 4;
 #pragma unroll 1
-  for (int q = threadIdx.x; q < near; q += THREADS) four(((const uint4*)r.keys)[q], q);
+  for (int q = threadIdx.x; q < near; q += THREADS) four(((const float4*)r.near)[q], q);
 #pragma unroll 1
   for (int q = near + threadIdx.x; q < all; q += 2 * THREADS) {  // two requests on their way
-    const uint4 k0 = r.far(q), k1 = r.far(q + THREADS);
-    four(k0, q);
-    four(k1, q + THREADS);
+    const float4 v0 = r.far(q), v1 = r.far(q + THREADS);
+    four(v0, q);
+    four(v1, q + THREADS);
   }
 }
 
@@ -337,19 +333,16 @@ __device__ __forceinline__ void add_to_bin(Shared& s, bool sums, int b, uint64_t
   }
 }
 
-// The members with keys from low_key on that `of` chooses, from all blocks, into the first block's list, which is empty (at most LIST of them).
+// The logits from `low` on that `of` chooses, from all blocks, into the first block's list, which is empty (at most LIST of them).
 template <int THREADS, typename F>
-__device__ __forceinline__ void gather(const Row& r, uint32_t low_key, F&& of) {
+__device__ __forceinline__ void gather(const Row& r, float low, F&& of) {
   Shared& s = r.s;
-  auto take = [&](int i, uint32_t k) {
-    const uint64_t p = r.place(k, i);
-    if (!of(k, p)) return;
+  each<THREADS>(r, low, [&](float l, int i, bool in) {
+    const uint64_t p = r.place(l, i);
+    if (!in || !of(l, p)) return;
     uint32_t at;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(remote(&s.n_list, 0)) : "memory");
     if (at < LIST) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&s.list.place[at], 0)), "l"(p) : "memory");
-  };
-  each_key<THREADS>(r, low_key, [&](uint32_t k, int i, bool in) {
-    if (in) take(i, k);
   });
   r.meet();
 }
@@ -393,14 +386,14 @@ __device__ __forceinline__ void rank_list(Shared& s, int n) {
 // The k-th largest of the groups' largest keys (to 22 bits, downwards) has at least k tokens from it on, and, where the largest are not all in a few
 // groups, not many more.
 template <int THREADS>
-__device__ __forceinline__ uint32_t crest_bound(const Row& r, int k) {
+__device__ __forceinline__ float crest_bound(const Row& r, int k) {
   const int i = threadIdx.x;
   const uint32_t mine = i >= GROUPS ? 0 : r.blocks > 1 ? peer32(&r.s.crest[i % r.crests], i / r.crests) : r.s.crest[i];
   uint32_t low = 0;
 #pragma unroll 1
   for (uint32_t bit = 1u << 31; bit >= 1u << 10; bit >>= 1)
     if (__syncthreads_count(mine >= (low | bit)) >= k) low |= bit;
-  return max(low, KEY_NONE + 1);
+  return low > KEY_NONE ? of_key(low) : LEAST;
 }
 
 // Sum over the cluster of every thread's v; slot: a word of each block's that nothing else has used since the last two meetings.
@@ -426,7 +419,7 @@ __device__ __forceinline__ void end_row(const Row& r, const DrawArgs& a, int64_t
   Shared& s = r.s;
   const int n = min((int)s.n_list, keep), i = threadIdx.x;
   const uint64_t p = i < n ? s.list.by_rank[i] : 0;
-  uint64_t w = i < n ? r.weight((uint32_t)(p >> 20)) : 0, all;
+  uint64_t w = i < n ? r.weight(of_place(p)) : 0, all;
   const uint64_t before = block_before64<THREADS>(w, s.red, &all);
   if (p_of_kept) {  // top_p of what top_k kept
     bool lost;
@@ -454,49 +447,49 @@ template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __grid_constant__ DrawArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *(Shared*)smem;
-  uint32_t* queue = (uint32_t*)(smem + (sizeof(Shared) + 15) / 16 * 16);  // 64 keys of each warp
-  uint32_t* keys = queue + THREADS * 2;
+  float* queue = (float*)(smem + (sizeof(Shared) + 15) / 16 * 16);  // 64 logits of each warp
+  float* near = queue + THREADS * 2;
   pdl_wait();
   pdl_trigger();
   uint32_t rank, blocks;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
   const int64_t row = blockIdx.x / blocks;
-  const int each = ((a.N + (int)blocks - 1) / (int)blocks + 7) / 8 * 8;
-  Row r{s, keys};
+  const int span = ((a.N + (int)blocks - 1) / (int)blocks + 7) / 8 * 8;
+  Row r{s, near};
   r.x = (const char*)a.x + row * a.ld * (a.f32 ? 4 : 2);
   r.N = a.N;
   r.f32 = a.f32;
   r.blocks = (int)blocks;
   r.rank = (int)rank;
-  r.first = min(a.N, (int)rank * each);
-  r.share = min(a.N - r.first, each);
+  r.first = min(a.N, (int)rank * span);
+  r.share = min(a.N - r.first, span);
   r.held = min(r.share, share_kept<THREADS>()) & ~3;
   r.vec = ((uintptr_t)r.x & 15) == 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  uint32_t top_key = 0;
+  float top = -INFINITY;
   int top_at = 0;
-  auto seen = [&](uint32_t k, int i) {  // a thread's indices rise
-    if (k > top_key) top_key = k, top_at = i;
+  auto seen = [&](float l, int i) {  // a thread's indices rise, and NaN is not larger
+    if (l > top) top = l, top_at = i;
   };
   constexpr int AHEAD = 5;
 #pragma unroll 1
   for (int q0 = threadIdx.x; q0 < (r.share + 3) / 4; q0 += THREADS * AHEAD) {
-    uint4 k[AHEAD];
+    float4 v[AHEAD];
 #pragma unroll
-    for (int e = 0; e < AHEAD; e++) k[e] = r.far(q0 + e * THREADS);
+    for (int e = 0; e < AHEAD; e++) v[e] = r.far(q0 + e * THREADS);
 #pragma unroll
     for (int e = 0; e < AHEAD; e++) {
       const int q = q0 + e * THREADS;
-      if (q < r.held / 4) ((uint4*)keys)[q] = k[e];
-      seen(k[e].x, q * 4);
-      seen(k[e].y, q * 4 + 1);
-      seen(k[e].z, q * 4 + 2);
-      seen(k[e].w, q * 4 + 3);
+      if (q < r.held / 4) ((float4*)near)[q] = v[e];
+      seen(v[e].x, q * 4);
+      seen(v[e].y, q * 4 + 1);
+      seen(v[e].z, q * 4 + 2);
+      seen(v[e].w, q * 4 + 3);
     }
   }
-  uint64_t best = top_key ? r.place(top_key, top_at) : 0;
+  uint64_t best = top > -INFINITY ? r.place(top, top_at) : 0;
   // groups of neighbouring threads
   r.crests = GROUPS / r.blocks;
   const int group = THREADS / r.crests;
@@ -520,23 +513,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
 #pragma unroll
     for (int b = 0; b < MAX_CLUSTER; b++) best = v[b] > best ? v[b] : best;
   }
-  r.top = (uint32_t)(best >> 20);
-  r.m32 = of_key(r.top);
-  r.m = wide(bits_of_key(r.top));
+  const bool none = best >> 20 <= KEY_NONE;
   const float heat = a.temperature ? a.temperature[row] : 1.f;
-  if (r.top <= KEY_NONE || !(heat > 0.f)) {
+  if (none || !(heat > 0.f)) {
     if (rank == 0 && threadIdx.x == 0) {
-      a.out[row] = r.top <= KEY_NONE ? -1 : 0xFFFFF - (int)(best & 0xFFFFF);
-      if (a.prob) a.prob[row] = r.top <= KEY_NONE ? 0.f : 1.f;
+      a.out[row] = none ? -1 : 0xFFFFF - (int)(best & 0xFFFFF);
+      if (a.prob) a.prob[row] = none ? 0.f : 1.f;
     }
     r.meet();
     return;
   }
+  r.m32 = of_place(best);
+  r.m = wide(__float_as_uint(r.m32));
   // beside +inf nothing has a weight
-  r.scale = r.top >= KEY_INF ? 1e30 : 256 * 1.4426950408889634074 / heat;
+  r.scale = r.m32 == INFINITY ? 1e30 : 256 * 1.4426950408889634074 / heat;
   r.least_d = r.scale > 0 ? -11520.0 / r.scale : -1e300;
   r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
-  if (r.top >= KEY_INF) r.m32 = 3.4028235e38f;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
+  if (r.m32 == INFINITY) r.m32 = -LEAST;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
   const int k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
   const uint64_t least = min_p > 0.f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * ONE) : 0;
@@ -550,11 +543,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   for (int stage = 0; stage < 2 && !few; stage++) {
     const bool sums = stage == 1;
     by_count = !sums;
-    uint32_t low_key = (uint32_t)(from >> 20);
+    float low = of_place(from);
     if (!sums) {
       if (k <= 0 || k >= a.N) continue;
       if (2 * k <= GROUPS) {
-        gather<THREADS>(r, crest_bound<THREADS>(r, k), [](uint32_t, uint64_t) { return true; });
+        gather<THREADS>(r, crest_bound<THREADS>(r, k), [](float, uint64_t) { return true; });
         few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
         if (few) {
           if (r.rank == 0) rank_list<THREADS>(s, (int)s.n_list);
@@ -563,16 +556,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         r.meet();  // the number has been read
       }
       uint64_t there = 0;
-      each_key<THREADS>(r, KEY_NONE + 1, [&](uint32_t, int, bool in) { there += in; });
+      each<THREADS>(r, LEAST, [&](float, int, bool in) { there += in; });
       if ((uint64_t)k >= cluster_sum<THREADS>(r, there, &s.there)) continue;  // all that have any weight are kept
       want = k;
     } else {
       if (!(top_p < 1.f)) continue;
       uint64_t sum = 0;
       const bool by_key = (from & 0xFFFFF) == 0;
-      each_key<THREADS>(r, low_key, [&](uint32_t key, int i, bool in) {
-        const uint64_t w = r.weight(key);
-        sum += in && (by_key || r.place(key, i) >= from) ? w : 0;
+      each<THREADS>(r, low, [&](float l, int i, bool in) {
+        const uint64_t w = r.weight(l);
+        sum += in && (by_key || r.place(l, i) >= from) ? w : 0;
       });
       sum = cluster_sum<THREADS>(r, sum, &s.weights);
       bool lost;
@@ -581,13 +574,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
       // The 256 largest and some more usually hold top_p.
       if (k <= 0 || 2 * k > GROUPS) {
         if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
-        const uint32_t low = max(low_key, crest_bound<THREADS>(r, GROUPS / 2));
+        const float bound = fmaxf(low, crest_bound<THREADS>(r, GROUPS / 2));
         r.meet();
-        gather<THREADS>(r, low, [&](uint32_t, uint64_t p) { return p >= from; });
+        gather<THREADS>(r, bound, [&](float, uint64_t p) { return p >= from; });
         if (r.rank == 0) {
           const int n = (int)s.n_list;
           uint64_t w = 0;
-          if (n <= LIST) w = block_sum64<THREADS>(threadIdx.x < n ? r.weight((uint32_t)(s.list.place[threadIdx.x] >> 20)) : 0, s.red);
+          if (n <= LIST) w = block_sum64<THREADS>(threadIdx.x < n ? r.weight(of_place(s.list.place[threadIdx.x])) : 0, s.red);
           if (threadIdx.x == 0) s.word = w >= want;
         }
         r.meet();
@@ -598,11 +591,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         }
         r.meet();  // the word has been read
       }
-      // All weights up to (sum - want) / N together are at most sum - want: the cut is above them, and keys that far down (a thousandth further) stay out of the bins.
+      // All weights up to (sum - want) / N together are at most sum - want: the cut is above them, and logits that far down (a thousandth further) stay out of the bins.
       const double tail = (double)(sum - want) / a.N;
       if (tail > 0) {
         const float reach = (float)(heat * log(ONE / tail) * 1.001) + fabsf(r.m32) * 1e-6f;
-        if (reach < 1e30f) low_key = max(low_key, key_of(r.m32 - reach));
+        if (reach < 1e30f) low = fmaxf(low, r.m32 - reach);
       }
     }
     int b0 = 0, hi = 52;
@@ -613,37 +606,37 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
       const int lo = max(0, hi - 10), mask = (1 << (hi - lo)) - 1;
       clear_bins<THREADS>(s, sums);
       if (digits) {
-        each_key<THREADS>(r, low_key, [&](uint32_t key, int i, bool in) {
-          const uint64_t p = r.place(key, i);
-          in = in && p >= from && r.bin(key) == b0 && (hi == 52 || p >> hi == known);
-          if (in) add_to_bin(s, sums, mask - ((int)(p >> lo) & mask), sums ? r.weight(key) : 0);  // larger digits first
+        each<THREADS>(r, low, [&](float l, int i, bool in) {
+          const uint64_t p = r.place(l, i);
+          in = in && p >= from && r.bin(l) == b0 && (hi == 52 || p >> hi == known);
+          if (in) add_to_bin(s, sums, mask - ((int)(p >> lo) & mask), sums ? r.weight(l) : 0);  // larger digits first
         });
       } else {
-        // Often few keys go into bins, but some of nearly every warp's: they queue, and 32 at a time are weighed and added.
-        uint32_t* line = queue + warp * 64;
+        // Often few logits go into bins, but some of nearly every warp's: they queue, and 32 at a time are weighed and added.
+        float* line = queue + warp * 64;
         int n = 0;
-        auto weigh = [&](uint32_t key) { add_to_bin(s, sums, r.bin(key), sums ? r.weight(key) : 0); };
+        auto weigh = [&](float l) { add_to_bin(s, sums, r.bin(l), sums ? r.weight(l) : 0); };
         const bool by_key = (from & 0xFFFFF) == 0;  // `from` begins a key
         const int all = (r.share + 3) / 4;
 #pragma unroll 1
         for (int q0 = warp * 32; q0 < all; q0 += THREADS) {
           const int q = q0 + lane;
-          const uint4 k = q < all ? r.quad(q) : make_uint4(0, 0, 0, 0);
-          if (!__any_sync(0xffffffffu, max(max(k.x, k.y), max(k.z, k.w)) >= low_key)) continue;
-          const uint32_t one[4] = {k.x, k.y, k.z, k.w};
+          const float4 v = q < all ? r.quad(q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= low)) continue;
+          const float one[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const bool in = one[e] >= low_key && (by_key || r.place(one[e], q * 4 + e) >= from);
+            const bool in = one[e] >= low && (by_key || r.place(one[e], q * 4 + e) >= from);
             const unsigned who = __ballot_sync(0xffffffffu, in);
             if (in) line[n + __popc(who & ((1u << lane) - 1))] = one[e];
             n += __popc(who);
             if (n >= 32) {
               __syncwarp();
-              const uint32_t key = line[lane], next = line[32 + lane];
+              const float l = line[lane], next = line[32 + lane];
               __syncwarp();
               line[lane] = next;
               n -= 32;
-              weigh(key);
+              weigh(l);
             }
           }
         }
@@ -664,10 +657,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         few = c.front + c.count <= LIST;
       }
       if (few || c.count <= LIST) {
-        // keys of bin b0 and in front of it, and a little more: the bin itself is looked at in what is left
+        // logits of bin b0 and in front of it, and a little more: the bin itself is looked at in what is left
         const float deep = (b0 + 1.01f) / r.bin_scale + fabsf(r.m32) * 1e-6f;
-        gather<THREADS>(r, b0 < BINS - 1 && deep < 1e30f ? max(low_key, key_of(r.m32 - deep)) : low_key, [&](uint32_t key, uint64_t p) {
-          const int b = r.bin(key);
+        gather<THREADS>(r, b0 < BINS - 1 && deep < 1e30f ? fmaxf(low, r.m32 - deep) : low, [&](float l, uint64_t p) {
+          const int b = r.bin(l);
           return p >= from && (few ? b <= b0 : b == b0 && (!digits || p >> hi == known));
         });
         if (r.rank == 0) {
@@ -676,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
           if (!few && !sums && threadIdx.x == 0) s.word = s.list.by_rank[left - 1];
           if (!few && sums) {
             uint64_t all;
-            const uint64_t w = threadIdx.x < n ? r.weight((uint32_t)(s.list.by_rank[threadIdx.x] >> 20)) : 0, before = block_before64<THREADS>(w, s.red, &all);
+            const uint64_t w = threadIdx.x < n ? r.weight(of_place(s.list.by_rank[threadIdx.x])) : 0, before = block_before64<THREADS>(w, s.red, &all);
             if (before < left && before + w >= left) s.word = s.list.by_rank[threadIdx.x];
           }
         }
@@ -696,14 +689,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     return;
   }
   // The draw: a warp sums pieces of 512 keys, the sums in front of the pieces tell which holds the token, and one warp looks through that piece.
-  const uint32_t from_key = (uint32_t)(from >> 20);
-  auto kept = [&](uint32_t key, int i) -> uint64_t {
-    const uint64_t w = r.weight(key);
-    return key >= from_key && r.place(key, i) >= from && w >= least ? w : 0;
+  const float low = of_place(from);
+  const bool by_key = (from & 0xFFFFF) == 0;
+  auto kept = [&](float l, int i) -> uint64_t {
+    const uint64_t w = r.weight(l);
+    return l >= low && (by_key || r.place(l, i) >= from) && w >= least ? w : 0;
   };
-  auto kept4 = [&](const uint4& k, int q) -> uint64_t {
-    if (max(max(k.x, k.y), max(k.z, k.w)) < from_key) return 0;
-    return kept(k.x, q * 4) + kept(k.y, q * 4 + 1) + kept(k.z, q * 4 + 2) + kept(k.w, q * 4 + 3);
+  auto kept4 = [&](const float4& v, int q) -> uint64_t {
+    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= low)) return 0;
+    return kept(v.x, q * 4) + kept(v.y, q * 4 + 1) + kept(v.z, q * 4 + 2) + kept(v.w, q * 4 + 3);
   };
   constexpr int PIECE = 128;  // quads
   const int pieces = (r.share + 4 * PIECE - 1) / (4 * PIECE);
@@ -711,12 +705,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   static_assert(sizeof(s.bin) / 8 >= (1 << 20) / (4 * PIECE), "a sum for every piece of the longest share");
 #pragma unroll 1
   for (int p = warp; p < pieces; p += THREADS / 32) {
-    uint4 k[4];
+    float4 v[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) k[e] = r.quad(p * PIECE + e * 32 + lane);
+    for (int e = 0; e < 4; e++) v[e] = r.quad(p * PIECE + e * 32 + lane);
     uint64_t sum = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) sum += kept4(k[e], p * PIECE + e * 32 + lane);
+    for (int e = 0; e < 4; e++) sum += kept4(v[e], p * PIECE + e * 32 + lane);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) piece_sum[p] = sum;
@@ -744,19 +738,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   while (before + piece_sum[p] <= target) before += piece_sum[p++];
 #pragma unroll 1
   for (int q = p * PIECE + lane; ; q += 32) {
-    const uint4 k = r.quad(q);
-    const uint64_t w = kept4(k, q);
+    const float4 v = r.quad(q);
+    const uint64_t w = kept4(v, q);
     uint64_t sum = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
+      const uint64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, before + sum > target);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
         uint64_t up_to = before + sum - w;
-        const uint32_t one[4] = {k.x, k.y, k.z, k.w};
+        const float one[4] = {v.x, v.y, v.z, v.w};
         bool found = false;
 #pragma unroll
         for (int e = 0; e < 4; e++) {

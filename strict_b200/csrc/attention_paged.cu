@@ -1,6 +1,6 @@
 // Softmax attention of new tokens over a paged cache, grouped heads of 64 or 128 dims, bf16.
 //
-// Few rows, where a row is one query head of one new token: at most 32 per sequence and key/value head. More: attention_paged_tc.cu.
+// Few rows, where a row is one query head of one new token: at most 16 per sequence and key/value head. More: attention_paged_tc.cu.
 #include <algorithm>
 #include <cmath>
 
@@ -15,7 +15,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // Bound by HBM: every key and value is read once. A block is one key/value head of one sequence and a share of its tiles of 64 keys. The last warp copies:
 // its lanes look the pages up, well ahead, and request the tile by TMA (boxes of min(page, 64) keys x 64 dims, 128-byte swizzle) into a ring
-// of `stages`. The others have 16 keys of every tile and 8 NB rows each (RG groups of them), with a softmax of their own; the four shares of the keys are
+// of `stages`. The others have 16 keys of every tile and all 8 NB rows each, with a softmax of their own; the four shares of the keys are
 // joined at the end.
 // Products are mma.sync m16n8k16 with keys (then dims) as the 16 rows and attention rows as the 8 columns, S^T = K Q^T and O^T = V^T P^T: at most eight
 // rows waste nothing that way. (With the rows as rows, half of everything was idle: 874 instructions per warp and tile, 166 registers and 5.3 TB/s.)
@@ -27,7 +27,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 // blocks leave (maximum, sum, unnormalised output) in scratch for attn_paged_join_kernel, 2 they are one cluster and join through distributed shared memory.
 constexpr int KT = 64;
 constexpr int MAX_STAGES = 6;
-constexpr int FEW_ROWS = 32;
+// Up to here this kernel, beyond it attention_paged_tc.cu: 64 sequences of 1 to 16 thousand keys with 16 rows take 332 us here and 417 there, 16 equal ones of 8
+// thousand with 12 rows 105 and 135 (uneven ones 93 and 84).
+constexpr int FEW_ROWS = 16;
 enum { JOIN_NONE = 0, JOIN_SCRATCH = 1, JOIN_CLUSTER = 2 };
 constexpr int CLUSTER_MAX = 8;
 
@@ -44,11 +46,15 @@ constexpr size_t few_smem(int HD, int rows, int stages) {
   return (ring > join ? ring : join) + 1024;
 }
 
-template <int HD, int NB, int RG, int JOIN>
-__global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+// blocks that fit on an SM: shared memory of two stages (8 rows of 128 dims), registers (otherwise)
+template <int HD, int NB>
+constexpr int few_fit() { return NB == 2 ? (HD == 128 ? 2 : 3) : HD == 128 ? 3 : 4; }
+
+template <int HD, int NB, int JOIN>
+__global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                        const __grid_constant__ PagedAttnArgs a, PagedJoin join, int ct, int stages, int* status) {
   constexpr int ATOM = KT * 128, TILE = ATOM * (HD / 64);  // bytes of 64 keys x 64 dims, and of a tile
-  constexpr int WARPS = 4 * RG, ROWS = 8 * NB * RG, BLOCK = 32 * (WARPS + 1);
+  constexpr int WARPS = 4, ROWS = 8 * NB, BLOCK = 32 * (WARPS + 1);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES];
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __g
   auto row_head = [&](int row) { return (t0 + row / G) * a.Hq + hk * G + row % G; };  // place among all rows and heads
 
   float o[HD / 16][NB][4], m_run[NB][2], l_run[NB][2];
-  const int kg = warp & 3, row0 = (warp >> 2) * 8 * NB;  // keys 16 kg .. of a tile, rows row0 .. of this warp
+  const int kg = warp & 3;  // keys 16 kg .. of a tile
   if (warp == WARPS) {
     auto page_of = [&](int i, int x) {
       const int j = i < n ? w.tile(share_tile(i, part, parts, ct)) * KT + x * box : w.end;
@@ -119,11 +125,11 @@ __global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __g
     for (int i = max(0, got - stages); i < got; i++) tc::mbar_wait(smem_u32(&full[i % stages]), (uint32_t)((i / stages) & 1));
     __syncwarp();
   } else {
-    // queries as columns: row row0 + 8 nb + g, dims 16 ks + 2 tig ..
+    // queries as columns: row 8 nb + g, dims 16 ks + 2 tig ..
     uint32_t qf[HD / 16][NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-      const int row = row0 + 8 * nb + g;
+      const int row = 8 * nb + g;
       const bf16* q = a.q + (row < R ? row_head(row) * HD : 0) + 2 * tig;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++) {
@@ -142,10 +148,11 @@ __global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __g
       for (int h = 0; h < 2; h++) {
         m_run[nb][h] = -INFINITY;
         l_run[nb][h] = 0.f;
-        pos[nb][h] = lo_pos + (row0 + 8 * nb + 2 * tig + h) / G;
+        pos[nb][h] = lo_pos + (8 * nb + 2 * tig + h) / G;
       }
     }
     const float scale_log2 = a.scale * LOG2E;
+    const int lo_key = a.window ? lo_pos - a.window + 1 : 0;
     const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
     uint32_t found = 0;
     bool ok = true;
@@ -159,6 +166,15 @@ __global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __g
       const uint32_t tK = sK + st * TILE + kg * 16 * 128, tV = sV + st * TILE + kg * 16 * 128;
       const bool there = page_bits[st] >> (kg * 16 / box) & 1;
       const bool whole = there && sees_all(a, w.end, j0, 16, lo_pos, hi_pos);
+      // values that some row may see: what lies behind them, or where nothing was fetched (the last sums of an earlier block, say), is not looked for again
+      uint32_t seen[2] = {0, 0};
+      if (there && !whole) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int j = j0 + (e >> 1) * 8 + 2 * tig + (e & 1);
+          if (j < w.end && (j >= lo_key || j < a.first)) seen[e >> 1] |= e & 1 ? 0xFFFF0000u : 0xFFFFu;
+        }
+      }
       // scores: keys g and g + 8, rows 2 tig and 2 tig + 1
       float s[NB][4], s2[NB][4];  // two sums, so that half as many products wait for one another
 #pragma unroll
@@ -229,7 +245,7 @@ __global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __g
           for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-              found |= not_finite(vf[j][x]);
+              found |= not_finite(vf[j][x] & seen[x >> 1]);  // this thread's keys are j0 + 8 (x / 2) + 2 tig and the next one
               vf[j][x] = only_finite(vf[j][x]);
             }
         }
@@ -267,7 +283,7 @@ __global__ void __launch_bounds__(128 * RG + 32) attn_paged_few_kernel(const __g
     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int row = row0 + 8 * nb + 2 * tig + h;
+        const int row = 8 * nb + 2 * tig + h;
         if (row < R) {
 #pragma unroll
           for (int j = 0; j < HD / 16; j++) {
@@ -402,51 +418,58 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(PagedAttnArgs a, P
 struct FewPlan {
   int parts = 1, stages = 2, join = JOIN_NONE;
 };
-// How the keys are cut, from the sizes, by a model in microseconds: a block starts after 3 and has a tile every 1.3 / stages at best (the latency of a copy) and
-// every `chain` (its products and its softmax one after the other); an SM takes 46 GB/s; blocks beyond those that fit run in further rounds, with half a round of unevenness; the join in a cluster takes 1.5, the one through scratch 4 and its bytes.
-// Ring: what shared memory leaves the blocks that share an SM. Clusters need all their blocks at once: one wave only, counted with 7/8 of the SMs, and
-// with shared memory for two blocks on each, or those that find no eight empty SMs wait for a second wave.
-FewPlan plan_few(const strictb200_ctx* ctx, int HD, int rows, int64_t units, int64_t tiles, double out_floats) {
-  const double stage = 2.0 * few_tile_bytes(HD), tile_us = stage / 46e3, sms = ctx->sm_count;
-  const double chain = (HD == 128 ? 0.8 : 0.6) * (rows > 8 ? 1.4 : 1);
-  // blocks per SM with two stages: shared memory (8 rows of 128 dims), registers (otherwise)
-  const int fit = rows > 16 ? (HD == 128 ? 1 : 2) : rows > 8 ? (HD == 128 ? 2 : 4) : HD == 128 ? 3 : 5;
+// How the keys are cut, from the sizes, by a model in microseconds. A tile costs a block `tile` times the blocks on its SM (an SM's share of HBM, 46 GB/s), but
+// at least `chain` (its products and its softmax one after the other) and 1.3 / stages (the latency of a copy); starting and ending, 3 for the first blocks,
+// 7 for every further round of them; the join in a cluster 1.5, the one through scratch 4 and its bytes. Only the longest sequence's length is known here, and the
+// blocks of a shorter one that have no tile leave at once. So a cut is costed twice, for sequences that are all as long and for lengths spread
+// below that one (mean 0.65, and half a block more per unit that is not full), and the sum counts: 16 sequences of 5 to 8 thousand keys, two new tokens and eight
+// heads took 79 us in the two parts that suit equal lengths, 61 in four.
+// Ring: what shared memory leaves the blocks that share an SM. Clusters need all their blocks at once: one round only, counted with 7/8 of the SMs, and
+// with shared memory for two blocks on each, or those that find no eight empty SMs wait for a second one.
+FewPlan plan_few(const strictb200_ctx* ctx, int HD, int fit, double chain, int64_t B, int64_t units, int64_t tiles, double out_floats) {
+  const double stage = 2.0 * few_tile_bytes(HD), tile = stage / 46e3, sms = ctx->sm_count, slots = fit * sms;
+  auto ring = [&](int share) { return (int)((double)(220 << 10) / share / stage - 0.1); };
   FewPlan best;
   double best_us = 1e30;
-  for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 128); parts += parts < 16 ? 1 : parts / 8) {
+  for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 128); parts += parts < 16 ? 1 : parts / 4) {
+    if (parts > 1 && out_floats * parts * 4 > (double)(512 << 20)) break;  // scratch
     const double ct = (double)((tiles + parts - 1) / parts), blocks = (double)(units * parts);
-    const int resident = (int)std::min<double>(fit, std::ceil(blocks / sms));
+    const bool cluster = parts > 1 && parts <= CLUSTER_MAX && blocks <= 0.875 * slots;
     FewPlan p;
     p.parts = (int)parts;
-    const bool one_wave = blocks <= (parts > 1 ? 0.875 : 1) * fit * sms;
-    const int share = one_wave && parts > 1 && parts <= CLUSTER_MAX ? std::max(2, resident) : resident;
-    p.stages = std::max(2, std::min<int>({MAX_STAGES, (int)ct, (int)((double)(220 << 10) / share / stage - 0.1)}));
-    double us = 3 + ct * std::max({tile_us * resident, chain, 1.3 / p.stages});
-    if (!one_wave) us = 3 + ct * tile_us * fit * (blocks / (fit * sms) + 0.5);
-    if (parts > 1) {
-      p.join = one_wave && parts <= CLUSTER_MAX ? JOIN_CLUSTER : JOIN_SCRATCH;
-      us += p.join == JOIN_CLUSTER ? 1.5 : 4 + out_floats * parts * 8 / 6e6;
+    p.join = parts == 1 ? JOIN_NONE : cluster ? JOIN_CLUSTER : JOIN_SCRATCH;
+    const int share = blocks <= slots ? std::max(cluster ? 2 : 1, (int)std::ceil(blocks / sms)) : parts == 1 ? 2 : fit;
+    p.stages = std::max(2, std::min<int>({MAX_STAGES, (int)ct, ring(share)}));
+    const double alone = std::max(chain, 1.3 / p.stages);
+    auto round = [&](double n) { return n > 0 ? ct * std::max(tile * std::ceil(n / sms), alone) : 0; };  // of n blocks
+    const double full = std::floor(blocks / slots);
+    double us = full * round(slots) + round(blocks - full * slots) + 7 * blocks / slots;
+    if (B > 1) {
+      const double some = std::min(blocks, units * (0.65 * parts + 0.5)), work = units * tiles * 0.65 / sms * std::max(tile, alone / fit);
+      us += some <= slots ? round(some) + 7 * some / slots : work + 0.25 * ct * chain * std::min(1.0, sms / some) + 7 * some / slots;
+    } else {
+      us *= 2;
     }
-    if (us < best_us * 0.99) best_us = us, best = p;
-    if (parts > 1 && out_floats * (parts + 1) * 4 > (double)(512 << 20)) break;  // scratch
+    us = us / 2 + (parts == 1 ? 0 : cluster ? 1.5 : 4 + out_floats * parts * 8 / 6e6);
+    if (us < best_us * 0.97) best_us = us, best = p;
   }
   return best;
 }
 
-template <int HD, int NB, int RG>
+template <int HD, int NB>
 int few_rows(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   static SbDeviceOnce once;
   SB_CUDA(once.run(ctx->device, [&] {
-    for (auto f : {attn_paged_few_kernel<HD, NB, RG, JOIN_NONE>, attn_paged_few_kernel<HD, NB, RG, JOIN_SCRATCH>, attn_paged_few_kernel<HD, NB, RG, JOIN_CLUSTER>}) {
-      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(HD, 8 * NB * RG, MAX_STAGES));
+    for (auto f : {attn_paged_few_kernel<HD, NB, JOIN_NONE>, attn_paged_few_kernel<HD, NB, JOIN_SCRATCH>, attn_paged_few_kernel<HD, NB, JOIN_CLUSTER>}) {
+      cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(HD, 8 * NB, MAX_STAGES));
       if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
   }));
   const int64_t tiles = std::max<int64_t>(1, paged_walk_tiles(a, KT));
-  const FewPlan plan = plan_few(ctx, HD, 8 * NB * RG, (int64_t)a.at.B * a.Hkv, tiles, (double)a.at.T * a.Hq * HD);
+  const FewPlan plan = plan_few(ctx, HD, few_fit<HD, NB>(), (HD == 128 ? 0.8 : 0.6) * (NB == 2 ? 1.4 : 1), a.at.B, (int64_t)a.at.B * a.Hkv, tiles, (double)a.at.T * a.Hq * HD);
   const int parts = plan.parts, ct = (int)((tiles + parts - 1) / parts), stages = plan.stages;
-  const size_t smem = few_smem(HD, 8 * NB * RG, stages);
+  const size_t smem = few_smem(HD, 8 * NB, stages);
   const dim3 grid((unsigned)parts, (unsigned)a.Hkv, (unsigned)a.at.B);
   PagedJoin buf;
   if (plan.join == JOIN_SCRATCH) SB_TRY(paged_join_scratch(ctx, a, parts, &buf));
@@ -454,10 +477,10 @@ int few_rows(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(paged_map_rows(&mk, a.k, rows, HD, std::min(a.at.page, KT)));
   SB_TRY(paged_map_rows(&mv, a.v, rows, HD, std::min(a.at.page, KT)));
-  const dim3 block(128 * RG + 32);
-  if (plan.join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_few_kernel<HD, NB, RG, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
-  else if (plan.join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_few_kernel<HD, NB, RG, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
-  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_few_kernel<HD, NB, RG, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, stages, ctx->d_status));
+  const dim3 block(160);
+  if (plan.join == JOIN_NONE) SB_CUDA(sb_launch(ctx, attn_paged_few_kernel<HD, NB, JOIN_NONE>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
+  else if (plan.join == JOIN_SCRATCH) SB_CUDA(sb_launch(ctx, attn_paged_few_kernel<HD, NB, JOIN_SCRATCH>, grid, block, smem, mk, mv, a, buf, ct, stages, ctx->d_status));
+  else SB_CUDA(sb_launch_cluster(ctx, attn_paged_few_kernel<HD, NB, JOIN_CLUSTER>, grid, block, smem, dim3((unsigned)parts), mk, mv, a, buf, ct, stages, ctx->d_status));
   ctx->launches++;
   return plan.join == JOIN_SCRATCH ? paged_join(ctx, a, buf) : STRICTB200_OK;
 }
@@ -488,7 +511,6 @@ int64_t paged_walk_tiles(const PagedAttnArgs& a, int kt) {
 int k_attn_paged(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   const int64_t rows = (int64_t)std::max(1, a.max_new) * (a.Hq / a.Hkv);
   if (rows > FEW_ROWS || a.at.B > 65535) return k_attn_paged_tiles(ctx, a);
-  if (rows > 16) return a.D == 128 ? few_rows<128, 2, 2>(ctx, a) : few_rows<64, 2, 2>(ctx, a);
-  if (rows > 8) return a.D == 128 ? few_rows<128, 2, 1>(ctx, a) : few_rows<64, 2, 1>(ctx, a);
-  return a.D == 128 ? few_rows<128, 1, 1>(ctx, a) : few_rows<64, 1, 1>(ctx, a);
+  if (rows > 8) return a.D == 128 ? few_rows<128, 2>(ctx, a) : few_rows<64, 2>(ctx, a);
+  return a.D == 128 ? few_rows<128, 1>(ctx, a) : few_rows<64, 1>(ctx, a);
 }

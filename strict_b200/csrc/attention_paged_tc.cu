@@ -21,6 +21,7 @@
 // places that were not fetched hold anything. So in tiles where some row does not see some key, two warps put zeros over values that are not finite; if any
 // row sees one of those (`poison`), it adds them at the end.
 #include <algorithm>
+#include <cmath>
 
 #include "attention_paged.cuh"
 
@@ -35,7 +36,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct TilesArgs {
   PagedAttnArgs a;
   PagedJoin join;  // parts of the output: ONE: 2 * parts, otherwise parts
-  int parts, ct;   // blocks that share the keys, tiles of a piece
+  int parts;       // blocks that share the keys of a unit
   int G, tw;       // heads per key/value head, tokens of a tile of 128 rows
   double inv_tb;   // 1 / tokens of a unit
   int one_round;   // a block for every unit
@@ -50,6 +51,7 @@ struct Unit {
   int lo_key;  // first key in the window of the first token
   int64_t row0;  // first row in q and out
   PagedWalk w;
+  int ct;           // tiles of a part: what a unit sees is cut evenly (pieces cut by the longest sequence took 132 us where these take 84, uneven drafts)
   int nt, nt_w[2];  // key tiles of the unit and of each stream
   int poison;       // values that are not finite were replaced
 };
@@ -254,252 +256,253 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 9) {
-    // ---- units and copies
-    int c = 0, nq = 0;  // key tiles, units with keys
-    bool good = true;
-    for (int u = 0; good; u++) {
-      // every other round of the blocks goes backwards: who had the longest of one has the shortest of the next
-      const int64_t y = (int64_t)u * gridDim.x + (u & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-      const int per = a.Hkv * t.parts;
-      Unit k;
-      k.n = -1;
-      k.nt = 0;
-      int tile;
-      const int x = (int)(y / per);
-      const bool one_round = t.one_round;
-      if (one_round ? u == 0 && place_unit(a.at, t.inv_tb, x, lane, &k.b, &tile)
-                    : a.at.B <= 32 ? find_unit<1>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile) : find_unit<4>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile)) {
-        k.part = (int)(y % per) / a.Hkv;
-        k.hk = (int)(y % per) % a.Hkv;
-        const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb, len = a.at.lens[k.b], q0 = tile * NQ * t.tw;
-        k.row0 = (int64_t)sb + q0;
-        k.lo_pos = len - n_new + q0;
-        k.lo_key = a.window ? max(0, k.lo_pos - a.window + 1) : 0;
-        k.n = sb < 0 || (int64_t)sb + n_new > a.at.T || q0 < 0 ? 0 : max(0, min(NQ * t.tw, n_new - q0));  // nothing where starts or lengths are none
-        k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
-        k.nt = k.n ? share_count(k.w.total, k.part, t.parts, t.ct) : 0;
-        if (ONE) {  // every other tile
-          k.nt_w[0] = (k.nt + 1) / 2;
-          k.nt_w[1] = k.nt / 2;
-        } else {    // tile A ends where its last token does
-          const int end_a = max(0, min(k.w.end, k.lo_pos + min(k.n, t.tw)));
-          k.nt_w[0] = min(k.nt, share_count(k.w.first + max(0, (end_a + BKV - 1) / BKV - k.w.lo), k.part, t.parts, t.ct));
-          k.nt_w[1] = k.n > t.tw ? k.nt : 0;
-          k.nt = max(k.nt_w[0], k.nt_w[1]);
-        }
-        k.poison = 0;
-      }
-      if (u >= 2) good = warp_wait(smem_u32(&unit_empty[u & 1]), (uint32_t)(u >> 1 & 1) ^ 1);
-      if (!good) break;
-      if (lane == 0) {
-        units[u & 1] = k;
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&unit_full[u & 1])) : "memory");
-      }
-      __syncwarp();
-      if (k.n < 0) break;
-      if (k.nt == 0) continue;
-      auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, t.ct)) * BKV; };
-      auto page_of = [&](int i, int x) {
-        const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
-        return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
-      };
-      auto copy_boxes = [&](const CUtensorMap* map, uint32_t tile, int row, unsigned there, uint32_t bar) {
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(there) * box * 128 * QA));
-        __syncwarp();
-        if (row >= 0)
-          for (int x = 0; x < QA; x++) tma_load_2d(tile + x * HALF_BYTES + lane * box * 128, map, x * 64, row, bar);
-      };
-      PageNames names;
-      names.begin(boxes, lane, page_of);
-      for (int i = 0; i < k.nt; i++, c++) {
-        const int st = c % RING, page = names.of(i, boxes, lane, page_of);
-        const uint32_t ph = (uint32_t)(c / RING & 1) ^ 1;
-        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-        const int row = page < 0 ? -1 : (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
-        if (c >= RING) good = warp_wait(smem_u32(&k_empty[st]), ph);
-        if (!good) break;
-        if (lane == 0) page_bits[c & 7] = there;
-        copy_boxes(&map_k, sK + st * TILE, row, there, smem_u32(&k_full[st]));
-        if (i == 0) {
-          if (nq) good = warp_wait(smem_u32(&q_empty), (uint32_t)(nq & 1) ^ 1);
-          if (good && lane == 0) {
-            const int tiles = !ONE && k.nt_w[1] ? 2 : 1;
-            mbar_expect_tx(smem_u32(&q_full), (uint32_t)(tiles * t.G * t.tw * 128 * QA));
-            for (int w = 0; w < tiles; w++)
-              for (int x = 0; x < QA; x++) tma_load_3d(sQ + w * TILE + x * HALF_BYTES, &map_q, x * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&q_full));
+      // ---- units and copies
+      int c = 0, nq = 0;  // key tiles, units with keys
+      bool good = true;
+      for (int u = 0; good; u++) {
+        // every other round of the blocks goes backwards: who had the longest of one has the shortest of the next
+        const int64_t y = (int64_t)u * gridDim.x + (u & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const int per = a.Hkv * t.parts;
+        Unit k;
+        k.n = -1;
+        k.nt = 0;
+        int tile;
+        const int x = (int)(y / per);
+        const bool one_round = t.one_round;
+        if (one_round ? u == 0 && place_unit(a.at, t.inv_tb, x, lane, &k.b, &tile)
+                      : a.at.B <= 32 ? find_unit<1>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile) : find_unit<4>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile)) {
+          k.part = (int)(y % per) / a.Hkv;
+          k.hk = (int)(y % per) % a.Hkv;
+          const int sb = a.at.starts[k.b], n_new = a.at.starts[k.b + 1] - sb, len = a.at.lens[k.b], q0 = tile * NQ * t.tw;
+          k.row0 = (int64_t)sb + q0;
+          k.lo_pos = len - n_new + q0;
+          k.lo_key = a.window ? max(0, k.lo_pos - a.window + 1) : 0;
+          k.n = sb < 0 || (int64_t)sb + n_new > a.at.T || q0 < 0 ? 0 : max(0, min(NQ * t.tw, n_new - q0));  // nothing where starts or lengths are none
+          k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
+          k.ct = max(1, (k.w.total + t.parts - 1) / t.parts);
+          k.nt = k.n ? share_count(k.w.total, k.part, t.parts, k.ct) : 0;
+          if (ONE) {  // every other tile
+            k.nt_w[0] = (k.nt + 1) / 2;
+            k.nt_w[1] = k.nt / 2;
+          } else {    // tile A ends where its last token does
+            const int end_a = max(0, min(k.w.end, k.lo_pos + min(k.n, t.tw)));
+            k.nt_w[0] = min(k.nt, share_count(k.w.first + max(0, (end_a + BKV - 1) / BKV - k.w.lo), k.part, t.parts, k.ct));
+            k.nt_w[1] = k.n > t.tw ? k.nt : 0;
+            k.nt = max(k.nt_w[0], k.nt_w[1]);
           }
-          if (good) nq++;
+          k.poison = 0;
         }
-        if (good && c >= RING) good = warp_wait(smem_u32(&v_empty[st]), ph);
-        if (!good) {
-          warp_wait(smem_u32(&k_full[st]), ph ^ 1);  // landed before this block's memory is somebody else's
-          break;
+        if (u >= 2) good = warp_wait(smem_u32(&unit_empty[u & 1]), (uint32_t)(u >> 1 & 1) ^ 1);
+        if (!good) break;
+        if (lane == 0) {
+          units[u & 1] = k;
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&unit_full[u & 1])) : "memory");
         }
-        copy_boxes(&map_v, sV + st * TILE, row, there, smem_u32(&v_full[st]));
-      }
-    }
-    if (!good && lane == 0) set_status(t.status, 41);
-    // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
-    if (nq) warp_wait(smem_u32(&q_full), (uint32_t)(nq & 1) ^ 1);
-    for (int i = max(0, c - RING); i < c; i++) {
-      warp_wait(smem_u32(&k_full[i % RING]), (uint32_t)(i / RING & 1));
-      warp_wait(smem_u32(&v_full[i % RING]), (uint32_t)(i / RING & 1));
-    }
-    } else if (warp == 8) {
-    // ---- products
-    const uint32_t lead = elected();
-    auto issue_s = [&](int w, int st) {
-      const uint32_t tS = tmem + (uint32_t)(w * 256);
-#pragma unroll
-      for (int s = 0; s < 4 * QA; s++) {
-        const uint32_t off = (uint32_t)((s >> 2) * HALF_BYTES + (s & 3) * 32);
-        warp_mma_ss(lead, tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
-      }
-      warp_commit(lead, smem_u32(&bar_s[w]));
-    };
-    auto issue_pv = [&](int w, int st, bool first, uint32_t ph) {  // by halves of the keys, as their weights come
-      const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
-#pragma unroll
-      for (int s = 0; s < 8; s++) {
-        if ((s & 3) == 0) {
-          if (!warp_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
-          tc_fence_after();
-        }
-        const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
-        const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
-        warp_mma_ts(lead, tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
-        warp_mma_ts(lead, tO, tS + pcol + 16, dv, idesc_pv, 1u);
-      }
-      warp_commit(lead, smem_u32(&bar_o[w]));
-      return true;
-    };
-    int c = 0, nq = 0, step0 = 0, step1 = 0, used0 = 0, used1 = 0;  // key tiles, units with keys; steps and units of each stream
-    bool good = true;
-    for (int u = 0; good && next_unit(u); u++) {
-      const int n_all = __shfl_sync(0xffffffffu, units[u & 1].nt, 0), n0 = __shfl_sync(0xffffffffu, units[u & 1].nt_w[0], 0),
-                n1 = __shfl_sync(0xffffffffu, units[u & 1].nt_w[1], 0);
-      unit_read(u);
-      if (n_all == 0) continue;
-      // O of a stream belongs to the last unit until its rows have been read
-      auto o_mine = [&](int w) { return (w ? used1 : used0) == 0 || warp_wait(smem_u32(&o_free[w]), (uint32_t)((w ? used1 : used0) & 1) ^ 1); };
-      auto k_there = [&](int i) {
-        const bool ok = warp_wait(smem_u32(&k_full[(c + i) % RING]), (uint32_t)((c + i) / RING & 1));
-        tc_fence_after();
-        return ok;
-      };
-      good = warp_wait(smem_u32(&q_full), (uint32_t)(nq & 1));
-      if (ONE) {
-        for (int w = 0; w < 2 && good; w++) {
-          if ((w ? n1 : n0) == 0) break;
-          good = k_there(w);
+        __syncwarp();
+        if (k.n < 0) break;
+        if (k.nt == 0) continue;
+        auto tile_key = [&](int i) { return k.w.tile(share_tile(i, k.part, t.parts, k.ct)) * BKV; };
+        auto page_of = [&](int i, int x) {
+          const int j = i < k.nt ? tile_key(i) + x * box : k.w.end;
+          return j < k.w.end ? paged_page(a.at, k.b, j >> a.at.shift) : -1;
+        };
+        auto copy_boxes = [&](const CUtensorMap* map, uint32_t tile, int row, unsigned there, uint32_t bar) {
+          if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(there) * box * 128 * QA));
+          __syncwarp();
+          if (row >= 0)
+            for (int x = 0; x < QA; x++) tma_load_2d(tile + x * HALF_BYTES + lane * box * 128, map, x * 64, row, bar);
+        };
+        PageNames names;
+        names.begin(boxes, lane, page_of);
+        for (int i = 0; i < k.nt; i++, c++) {
+          const int st = c % RING, page = names.of(i, boxes, lane, page_of);
+          const uint32_t ph = (uint32_t)(c / RING & 1) ^ 1;
+          const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+          const int row = page < 0 ? -1 : (int)((page * (int64_t)a.Hkv + k.hk) * a.at.page) + ((tile_key(i) + lane * box) & (a.at.page - 1));
+          if (c >= RING) good = warp_wait(smem_u32(&k_empty[st]), ph);
           if (!good) break;
-          issue_s(w, (c + w) % RING);
-          warp_commit(lead, smem_u32(&k_empty[(c + w) % RING]));
-          if (w == n_all - 1) warp_commit(lead, smem_u32(&q_empty));
+          if (lane == 0) page_bits[c & 7] = there;
+          copy_boxes(&map_k, sK + st * TILE, row, there, smem_u32(&k_full[st]));
+          if (i == 0) {
+            if (nq) good = warp_wait(smem_u32(&q_empty), (uint32_t)(nq & 1) ^ 1);
+            if (good && lane == 0) {
+              const int tiles = !ONE && k.nt_w[1] ? 2 : 1;
+              mbar_expect_tx(smem_u32(&q_full), (uint32_t)(tiles * t.G * t.tw * 128 * QA));
+              for (int w = 0; w < tiles; w++)
+                for (int x = 0; x < QA; x++) tma_load_3d(sQ + w * TILE + x * HALF_BYTES, &map_q, x * 64, k.hk * t.G, (int)(k.row0 + w * t.tw), smem_u32(&q_full));
+            }
+            if (good) nq++;
+          }
+          if (good && c >= RING) good = warp_wait(smem_u32(&v_empty[st]), ph);
+          if (!good) {
+            warp_wait(smem_u32(&k_full[st]), ph ^ 1);  // landed before this block's memory is somebody else's
+            break;
+          }
+          copy_boxes(&map_v, sV + st * TILE, row, there, smem_u32(&v_full[st]));
         }
-        for (int s = 0; s < n0 && good; s++) {
+      }
+      if (!good && lane == 0) set_status(t.status, 41);
+      // copies in flight have landed before this block's memory is somebody else's; only needed where the waits of the others gave up
+      if (nq) warp_wait(smem_u32(&q_full), (uint32_t)(nq & 1) ^ 1);
+      for (int i = max(0, c - RING); i < c; i++) {
+        warp_wait(smem_u32(&k_full[i % RING]), (uint32_t)(i / RING & 1));
+        warp_wait(smem_u32(&v_full[i % RING]), (uint32_t)(i / RING & 1));
+      }
+    } else if (warp == 8) {
+      // ---- products
+      const uint32_t lead = elected();
+      auto issue_s = [&](int w, int st) {
+        const uint32_t tS = tmem + (uint32_t)(w * 256);
+#pragma unroll
+        for (int s = 0; s < 4 * QA; s++) {
+          const uint32_t off = (uint32_t)((s >> 2) * HALF_BYTES + (s & 3) * 32);
+          warp_mma_ss(lead, tS, desc_kmajor(sQ + (ONE ? 0 : w * TILE) + off), desc_kmajor(sK + st * TILE + off), idesc_s, s ? 1u : 0u);
+        }
+        warp_commit(lead, smem_u32(&bar_s[w]));
+      };
+      auto issue_pv = [&](int w, int st, bool first, uint32_t ph) {  // by halves of the keys, as their weights come
+        const uint32_t tS = tmem + (uint32_t)(w * 256), tO = tS + 128;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+          if ((s & 3) == 0) {
+            if (!warp_wait(smem_u32(&bar_p[w][s >> 2]), ph)) return false;
+            tc_fence_after();
+          }
+          const uint64_t dv = desc_mnmajor(sV + st * TILE + (uint32_t)(s * 2048));
+          const uint32_t pcol = (uint32_t)((s >> 1) * 32 + (s & 1) * 8);
+          warp_mma_ts(lead, tO, tS + pcol, dv, idesc_pv, (s || !first) ? 1u : 0u);
+          warp_mma_ts(lead, tO, tS + pcol + 16, dv, idesc_pv, 1u);
+        }
+        warp_commit(lead, smem_u32(&bar_o[w]));
+        return true;
+      };
+      int c = 0, nq = 0, step0 = 0, step1 = 0, used0 = 0, used1 = 0;  // key tiles, units with keys; steps and units of each stream
+      bool good = true;
+      for (int u = 0; good && next_unit(u); u++) {
+        const int n_all = __shfl_sync(0xffffffffu, units[u & 1].nt, 0), n0 = __shfl_sync(0xffffffffu, units[u & 1].nt_w[0], 0),
+                  n1 = __shfl_sync(0xffffffffu, units[u & 1].nt_w[1], 0);
+        unit_read(u);
+        if (n_all == 0) continue;
+        // O of a stream belongs to the last unit until its rows have been read
+        auto o_mine = [&](int w) { return (w ? used1 : used0) == 0 || warp_wait(smem_u32(&o_free[w]), (uint32_t)((w ? used1 : used0) & 1) ^ 1); };
+        auto k_there = [&](int i) {
+          const bool ok = warp_wait(smem_u32(&k_full[(c + i) % RING]), (uint32_t)((c + i) / RING & 1));
+          tc_fence_after();
+          return ok;
+        };
+        good = warp_wait(smem_u32(&q_full), (uint32_t)(nq & 1));
+        if (ONE) {
           for (int w = 0; w < 2 && good; w++) {
-            if (s >= (w ? n1 : n0)) break;
-            const int i = 2 * s + w, st = (c + i) % RING;
-            good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)((c + i) / RING & 1)) && (s || o_mine(w)) &&
-                   issue_pv(w, st, s == 0, (uint32_t)((w ? step1 : step0) + s & 1));
+            if ((w ? n1 : n0) == 0) break;
+            good = k_there(w);
+            if (!good) break;
+            issue_s(w, (c + w) % RING);
+            warp_commit(lead, smem_u32(&k_empty[(c + w) % RING]));
+            if (w == n_all - 1) warp_commit(lead, smem_u32(&q_empty));
+          }
+          for (int s = 0; s < n0 && good; s++) {
+            for (int w = 0; w < 2 && good; w++) {
+              if (s >= (w ? n1 : n0)) break;
+              const int i = 2 * s + w, st = (c + i) % RING;
+              good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)((c + i) / RING & 1)) && (s || o_mine(w)) &&
+                     issue_pv(w, st, s == 0, (uint32_t)((w ? step1 : step0) + s & 1));
+              if (!good) break;
+              warp_commit(lead, smem_u32(&v_empty[st]));
+              if (s + 1 < (w ? n1 : n0)) {
+                good = k_there(i + 2);
+                if (!good) break;
+                issue_s(w, (c + i + 2) % RING);
+                warp_commit(lead, smem_u32(&k_empty[(c + i + 2) % RING]));
+                if (i + 2 == n_all - 1) warp_commit(lead, smem_u32(&q_empty));
+              }
+            }
+          }
+        } else {
+          good = good && k_there(0);
+          if (good) {
+            for (int w = 0; w < 2; w++)
+              if ((w ? n1 : n0) > 0) issue_s(w, c % RING);
+            warp_commit(lead, smem_u32(&k_empty[c % RING]));
+            if (n_all == 1) warp_commit(lead, smem_u32(&q_empty));
+          }
+          for (int i = 0; i < n_all && good; i++) {
+            const int st = (c + i) % RING, in = (c + i + 1) % RING;
+            good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)((c + i) / RING & 1));
+            bool k_next = false;
+            for (int w = 0; w < 2 && good; w++) {
+              if (i < (w ? n1 : n0)) {
+                good = (i || o_mine(w)) && issue_pv(w, st, i == 0, (uint32_t)((w ? step1 : step0) + i & 1));
+                if (!good) break;
+              }
+              if (i + 1 < (w ? n1 : n0)) {
+                if (!k_next) {
+                  good = k_there(i + 1);
+                  if (!good) break;
+                  k_next = true;
+                }
+                issue_s(w, in);
+              }
+            }
             if (!good) break;
             warp_commit(lead, smem_u32(&v_empty[st]));
-            if (s + 1 < (w ? n1 : n0)) {
-              good = k_there(i + 2);
-              if (!good) break;
-              issue_s(w, (c + i + 2) % RING);
-              warp_commit(lead, smem_u32(&k_empty[(c + i + 2) % RING]));
-              if (i + 2 == n_all - 1) warp_commit(lead, smem_u32(&q_empty));
-            }
+            if (i + 1 < n_all) warp_commit(lead, smem_u32(&k_empty[in]));
+            if (i + 2 == n_all) warp_commit(lead, smem_u32(&q_empty));
           }
         }
-      } else {
-        good = good && k_there(0);
-        if (good) {
-          for (int w = 0; w < 2; w++)
-            if ((w ? n1 : n0) > 0) issue_s(w, c % RING);
-          warp_commit(lead, smem_u32(&k_empty[c % RING]));
-          if (n_all == 1) warp_commit(lead, smem_u32(&q_empty));
-        }
-        for (int i = 0; i < n_all && good; i++) {
-          const int st = (c + i) % RING, in = (c + i + 1) % RING;
-          good = warp_wait(smem_u32(&v_ready[st]), (uint32_t)((c + i) / RING & 1));
-          bool k_next = false;
-          for (int w = 0; w < 2 && good; w++) {
-            if (i < (w ? n1 : n0)) {
-              good = (i || o_mine(w)) && issue_pv(w, st, i == 0, (uint32_t)((w ? step1 : step0) + i & 1));
-              if (!good) break;
-            }
-            if (i + 1 < (w ? n1 : n0)) {
-              if (!k_next) {
-                good = k_there(i + 1);
-                if (!good) break;
-                k_next = true;
-              }
-              issue_s(w, in);
-            }
-          }
-          if (!good) break;
-          warp_commit(lead, smem_u32(&v_empty[st]));
-          if (i + 1 < n_all) warp_commit(lead, smem_u32(&k_empty[in]));
-          if (i + 2 == n_all) warp_commit(lead, smem_u32(&q_empty));
-        }
+        c += n_all;
+        nq++;
+        step0 += n0;
+        step1 += n1;
+        used0 += n0 > 0;
+        used1 += n1 > 0;
       }
-      c += n_all;
-      nq++;
-      step0 += n0;
-      step1 += n1;
-      used0 += n0 > 0;
-      used1 += n1 > 0;
-    }
-    if (!good) {  // what was issued has ended before the tiles are somebody else's
-      if (lane == 0) set_status(t.status, 43);
-      warp_commit(lead, smem_u32(&k_empty[0]));
-      for (int i = 0; i < 2; i++) warp_wait(smem_u32(&k_empty[0]), (uint32_t)i);
-    }
+      if (!good) {  // what was issued has ended before the tiles are somebody else's
+        if (lane == 0) set_status(t.status, 43);
+        warp_commit(lead, smem_u32(&k_empty[0]));
+        for (int i = 0; i < 2; i++) warp_wait(smem_u32(&k_empty[0]), (uint32_t)i);
+      }
     } else {
-    // ---- values of tiles that not every row sees whole
-    const int tid = (int)threadIdx.x - 10 * 32;
-    int c = 0;
-    bool good = true;
-    for (int u = 0; good && next_unit(u); u++) {
-      Unit& k = units[u & 1];
-      const PagedWalk w = k.w;
-      const int nt = k.nt, part = k.part, lo_pos = k.lo_pos, hi_pos = k.lo_pos + k.n - 1, lo_key = k.lo_key;
-      for (int i = 0; i < nt; i++, c++) {
-        const int st = c % RING, k0 = w.tile(share_tile(i, part, t.parts, t.ct)) * BKV;
-        good = warp_wait(smem_u32(&v_full[st]), (uint32_t)(c / RING & 1));
-        if (!good) break;
-        const uint32_t bits = page_bits[c & 7];
-        if (bits != (1u << boxes) - 1 || !sees_all(a, w.end, k0, BKV, lo_pos, hi_pos)) {
-          uint32_t found = 0;
-          uint4* v = (uint4*)(smem + (NQ + RING + st) * TILE);
-          constexpr int AHEAD = 8;  // finite values need nothing, whoever sees them: the loads of eight go together
-          for (int x0 = tid; x0 < QA * BKV * 8; x0 += 64 * AHEAD) {
-            uint4 y[AHEAD];
-            uint32_t odd = 0;
+      // ---- values of tiles that not every row sees whole
+      const int tid = (int)threadIdx.x - 10 * 32;
+      int c = 0;
+      bool good = true;
+      for (int u = 0; good && next_unit(u); u++) {
+        Unit& k = units[u & 1];
+        const PagedWalk w = k.w;
+        const int nt = k.nt, part = k.part, ct = k.ct, lo_pos = k.lo_pos, hi_pos = k.lo_pos + k.n - 1, lo_key = k.lo_key;
+        for (int i = 0; i < nt; i++, c++) {
+          const int st = c % RING, k0 = w.tile(share_tile(i, part, t.parts, ct)) * BKV;
+          good = warp_wait(smem_u32(&v_full[st]), (uint32_t)(c / RING & 1));
+          if (!good) break;
+          const uint32_t bits = page_bits[c & 7];
+          if (bits != (1u << boxes) - 1 || !sees_all(a, w.end, k0, BKV, lo_pos, hi_pos)) {
+            uint32_t found = 0;
+            uint4* v = (uint4*)(smem + (NQ + RING + st) * TILE);
+            constexpr int AHEAD = 8;  // finite values need nothing, whoever sees them: the loads of eight go together
+            for (int x0 = tid; x0 < QA * BKV * 8; x0 += 64 * AHEAD) {
+              uint4 y[AHEAD];
+              uint32_t odd = 0;
 #pragma unroll
-            for (int e = 0; e < AHEAD; e++) y[e] = v[x0 + 64 * e];
+              for (int e = 0; e < AHEAD; e++) y[e] = v[x0 + 64 * e];
 #pragma unroll
-            for (int e = 0; e < AHEAD; e++) odd |= not_finite(y[e].x) | not_finite(y[e].y) | not_finite(y[e].z) | not_finite(y[e].w);
-            if (!odd) continue;
-            for (int x = x0; x < x0 + 64 * AHEAD; x += 64) {
-              const int r = (x >> 3) & (BKV - 1), j = k0 + r;
-              const bool seen = j < w.end && (bits >> (r / box) & 1) && (j >= lo_key || j < a.first);
-              const uint4 z = v[x];
-              found |= seen && (not_finite(z.x) | not_finite(z.y) | not_finite(z.z) | not_finite(z.w));
-              v[x] = make_uint4(only_finite(z.x), only_finite(z.y), only_finite(z.z), only_finite(z.w));
+              for (int e = 0; e < AHEAD; e++) odd |= not_finite(y[e].x) | not_finite(y[e].y) | not_finite(y[e].z) | not_finite(y[e].w);
+              if (!odd) continue;
+              for (int x = x0; x < x0 + 64 * AHEAD; x += 64) {
+                const int r = (x >> 3) & (BKV - 1), j = k0 + r;
+                const bool seen = j < w.end && (bits >> (r / box) & 1) && (j >= lo_key || j < a.first);
+                const uint4 z = v[x];
+                found |= seen && (not_finite(z.x) | not_finite(z.y) | not_finite(z.z) | not_finite(z.w));
+                v[x] = make_uint4(only_finite(z.x), only_finite(z.y), only_finite(z.z), only_finite(z.w));
+              }
             }
+            if (found) k.poison = 1;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
-          if (found) k.poison = 1;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&v_ready[st])) : "memory");
         }
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&v_ready[st])) : "memory");
+        unit_read(u);
       }
-      unit_read(u);
-    }
-    if (!good && lane == 0) set_status(t.status, 44);
+      if (!good && lane == 0) set_status(t.status, 44);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
     bool good = true;
     for (int u = 0; good && next_unit(u); u++) {
       const Unit& k = units[u & 1];
-      const int nt = k.nt_w[w], n_all = k.nt, part = k.part;
+      const int nt = k.nt_w[w], n_all = k.nt, part = k.part, ct = k.ct;
       const PagedWalk walk = k.w;
       const bool live = row < t.G * t.tw && tok < k.n;
       const bool any_live = __any_sync(0xffffffffu, live);  // a warp without rows only keeps step
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
           uint32_t r[BKV];
           tc_ld32(tS + lane_base, r);
           tc_ld32(tS + lane_base + 32, r + 32);
-          const int k0 = walk.tile(share_tile(i, part, t.parts, t.ct)) * BKV;
+          const int k0 = walk.tile(share_tile(i, part, t.parts, ct)) * BKV;
           const uint32_t bits = page_bits[(c + i) & 7];
           const bool full = bits == (1u << boxes) - 1 && sees_all(a, walk.end, k0, BKV, pos_a, pos_b);
           tc_wait_ld();
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
-          if (live) add_poison(a, walk, k.b, k.hk, part, t.parts, t.ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt, pos, c32 * 32, 32, f);
+          if (live) add_poison(a, walk, k.b, k.hk, part, t.parts, ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt, pos, c32 * 32, 32, f);
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 32; j++) r[j] = __float_as_uint(f[j]);
@@ -754,17 +757,24 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   const int tb = (ONE ? 1 : 2) * t.tw;
   t.inv_tb = 1.0 / tb;
   const int64_t tiles = a.at.T / tb + a.at.B;  // room for the tiles of all sequences
-  // Parts: the fewest rounds of key tiles over the SMs, a block counted with three tiles more (its start and its end) and the join with four.
-  const int64_t units = std::max<int64_t>((a.at.T + tb - 1) / tb, a.at.B) * a.Hkv, keys = std::max<int64_t>(1, paged_walk_tiles(a, BKV));
-  int64_t best = INT64_MAX;
+  // Parts, by key tiles as the unit of time (2.6 us; 1.5 with one tile): rounds of units that are all as long, each with three tiles more for its start and
+  // its end, and, where there are several sequences, lengths spread below max_len (mean 0.65): then the longest unit, or what the SMs have to do together.
+  // A prompt's rows see half of it. The join costs 4 us and its bytes. (16 sequences of 1.5 to 8 thousand keys, five new tokens, eight heads:
+  // one part 121 us, two 84, four 96; one of 16 thousand, 512 new tokens: two 176, three 229, four 193.)
+  const double units = (double)std::max<int64_t>((a.at.T + tb - 1) / tb, a.at.B) * a.Hkv, sms = ctx->sm_count;
+  const double keys = (double)std::max<int64_t>(1, paged_walk_tiles(a, BKV)), seen = keys * (1 - 0.5 * std::min(1.0, (double)a.max_new / std::max(1, a.max_len)));
+  const int outs = ONE ? 2 : 1;
+  double best = 1e30;
   t.parts = 1;
-  for (int p = 1; p <= 64 && p <= keys; p++) {
-    if (p > 1 && (size_t)a.at.T * a.Hq * p * (ONE ? 2 : 1) * (64 * QA + 2) * 4 > ((size_t)256 << 20)) break;
-    const int64_t cost = (units * p + ctx->sm_count - 1) / ctx->sm_count * ((keys + p - 1) / p + 3) + (p > 1 ? 4 : 0);
-    if (cost < best) best = cost, t.parts = p;
+  for (int p = 1; p <= 64 && p <= keys; p += p < 8 ? 1 : p / 4) {
+    const double out_bytes = (double)a.at.T * a.Hq * p * outs * (64 * QA + 2) * 4;
+    if (p > 1 && out_bytes > (double)(256 << 20)) break;
+    const double longest = std::ceil(keys / p) + 3, even = std::ceil(units * p / sms) * (std::ceil(seen / p) + 3);
+    const double spread = a.at.B > 1 ? std::max(longest, (units * seen * 0.65 + 3 * units * p) / sms) : even;
+    const double cost = (even + spread) / 2 + (p * outs > 1 ? (4 + out_bytes / 2.5e6) / (ONE ? 1.5 : 2.6) : 0);
+    if (cost < best * 0.98) best = cost, t.parts = p;
   }
-  t.ct = (int)((keys + t.parts - 1) / t.parts);
-  const int np = (ONE ? 2 : 1) * t.parts;
+  const int np = outs * t.parts;
   if (np > 1) SB_TRY(paged_join_scratch(ctx, a, np, &t.join));
   const int64_t blocks = std::min<int64_t>(tiles * a.Hkv * t.parts, ctx->sm_count);
   t.one_round = tiles * a.Hkv * t.parts <= ctx->sm_count;

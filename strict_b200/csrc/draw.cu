@@ -27,9 +27,10 @@ namespace {
 
 constexpr int GROUPS = 512;  // of threads of a cluster, whose largest keys bound the first of the order
 constexpr int BINS = 1024, LIST = 512;
-// Keys of a block in shared memory: 75 KB where two blocks share an SM, 188 KB where one has it; the rest of a longer share is read again in every pass.
+constexpr int PIECE = 128;  // quads of logits that a warp sums at a time for the draw
+// Keys of a block in shared memory: 75 KB where two blocks share an SM, 186 KB where one has it; the rest of a longer share is read again in every pass.
 template <int THREADS>
-constexpr int share_kept() { return THREADS == 512 ? 19200 : 48000; }
+constexpr int share_kept() { return THREADS == 512 ? 19072 : 47488; }
 constexpr int MAX_CLUSTER = 8;
 constexpr double ONE = 8796093022208.0;  // 2^43
 
@@ -68,11 +69,12 @@ struct Shared {
   union {
     struct {
       uint32_t count[BINS];
-      uint32_t sum[4][BINS];  // weights in pieces of 11 bits: counters of 32 bits are added to without a loop, and 2^20 members do not overflow them
+      uint64_t sum[BINS];
     } bin;
     struct {
       uint64_t place[LIST], by_rank[LIST];
     } list;
+    uint64_t piece_sum[(1 << 20) / (4 * PIECE)];  // of the draw's pieces of the longest share
   };
   // sums over the cluster of this block's part of the bins (whole for a cluster of one)
   uint32_t part_count[BINS / 2];
@@ -82,7 +84,7 @@ struct Shared {
   uint64_t pick[6];
   uint64_t best, there, weights, word, drawn;  // what blocks tell one another: largest place, numbers, sums, a cut, the kept weights
   uint32_t n_list;
-  long long fraction[256];  // bits of 2^(43 + i / 256)
+  long long fraction[64 * 8];  // bits of 2^(43 + i / 64), eight copies side by side: neighbouring lanes read other banks
   uint32_t crest[GROUPS];  // largest keys of groups of this block's threads
 };
 
@@ -109,8 +111,9 @@ struct Row {
   const void* x;
   int N, f32, vec, first, share, held;  // vec: rows begin at 16 bytes
   int blocks, rank, crests;  // crests: groups of this block's threads
-  double m, scale, least_d;  // the largest logit, 256 log2(e) / temperature, distance from which on a weight is 0
-  float m32, bin_scale;
+  double m, scale;  // the largest logit, 64 log2(e) / temperature
+  float m32, bin_scale, least_l, zero_l;  // least_l: from here on a weight is not 0 (2^-45 of the largest); zero_l: a little below
+  bool plain;  // zero_l is near enough, and the largest logit is finite
 
   // All blocks of the cluster, all threads.
   __device__ __forceinline__ void meet() const {
@@ -135,23 +138,36 @@ struct Row {
   __device__ __forceinline__ float4 quad(int q) const { return q < held / 4 ? ((const float4*)near)[q] : far(q); }
   // the place in the row's order, larger is earlier: the key, then the lower index
   __device__ __forceinline__ uint64_t place(float l, int i) const { return (uint64_t)key_of(l) << 20 | (uint32_t)(0xFFFFF - (first + i)); }
-  // 2^43 exp((l - max) / T) rounded to a whole number. y = 256 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 256) is 2^(n / 256), from a table
-  // of the 256 fractions, times the series of exp(f ln(2) / 256) to the third power (off by 1.4e-13 of the weight, 1.2 units at most). The sums that round are additions of a
-  // power of two that leaves no bits behind the point.
-  // Straight-line, so that several go side by side; of -inf and NaN nobody asks.
-  __device__ __forceinline__ uint64_t weight(float l) const {
-    const double d = wide(__float_as_uint(l)) - m;
+  // 2^43 exp((l - max) / T) rounded to a whole number. y = 64 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 64) is 2^(n / 64), from a table of
+  // the 64 fractions, times the series of exp(f ln(2) / 64) to the fourth power (off by 4e-14 of the weight, a third of a unit at most). The sums that
+  // round are additions of a power of two that leaves no bits behind the point. Straight-line, so that several go side by side.
+  // This is of a logit as a 64-bit number, with the bias of that addition; neither far away nor above the largest.
+  static constexpr uint64_t BIAS = 0x4330000000000000ull;
+  __device__ __forceinline__ uint64_t weight_of(double x) const {
+    const double d = x - m;
     constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52
     const double t = fma(d, scale, WHOLE), f = fma(d, scale, WHOLE - t);
     const int n = __double2loint(t);
-    constexpr double C = 0.69314718055994530942 / 256;
-    double p = C * C * C / 6;
+    constexpr double C = 0.69314718055994530942 / 64;
+    double p = C * C * C * C / 24;
+    p = fma(p, f, C * C * C / 6);
     p = fma(p, f, C * C / 2);
     p = fma(p, f, C);
     p = fma(p, f, 1.0);
-    const long long two = s.fraction[n & 255] + ((long long)(n >> 8) << 52);  // 2^(43 + n / 256)
-    const uint64_t w = (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0)) - 0x4330000000000000ull;
-    return d > least_d ? w : 0;  // 2^-45
+    const long long two = s.fraction[(n & 63) << 3 | (threadIdx.x & 7)] + ((long long)(n >> 6) << 52);  // 2^(43 + n / 64)
+    return (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0));
+  }
+  __device__ __forceinline__ uint64_t weight(float l) const {  // of any logit
+    const uint64_t w = weight_of(wide(__float_as_uint(l))) - BIAS;
+    return l >= least_l ? w : 0;
+  }
+  // The weights of four logits from `cut` on together, where `plain`: what is below counts as zero_l, whose weight is 0. (With a choice behind each weight, and
+  // a place in the order to compare: 67 instructions a logit for a row without filters, 45 this
+  // way: 256 rows 139 us and 105.)
+  __device__ __forceinline__ uint64_t weights(const float4& v, float cut) const {
+    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= cut)) return 0;
+    return weight_of(v.x >= cut ? v.x : zero_l) + weight_of(v.y >= cut ? v.y : zero_l) + weight_of(v.z >= cut ? v.z : zero_l) +
+           weight_of(v.w >= cut ? v.w : zero_l) - 4 * BIAS;
   }
   // Bins of equal width below the maximum, the last one for all that is further away; never falls with a falling logit.
   __device__ __forceinline__ int bin(float l) const {
@@ -232,9 +248,6 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
   if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
   r.meet();  // all bins are counted
   const uint32_t* counts = s.bin.count;
-  auto sum_of = [&](int i) {
-    return s.bin.sum[0][i] + ((uint64_t)s.bin.sum[1][i] << 11) + ((uint64_t)s.bin.sum[2][i] << 22) + ((uint64_t)s.bin.sum[3][i] << 33);
-  };
   int owner = 0;
   uint64_t front_c = 0, front_s = 0;
   if (r.blocks > 1) {
@@ -247,8 +260,7 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
       const int at = r.rank * per + i;
       const uint32_t c0 = peer32(&s.bin.count[at], b);
       if (sums) {
-        const uint64_t w0 = peer32(&s.bin.sum[0][at], b), w1 = peer32(&s.bin.sum[1][at], b), w2 = peer32(&s.bin.sum[2][at], b), w3 = peer32(&s.bin.sum[3][at], b);
-        ww += w0 + (w1 << 11) + (w2 << 22) + (w3 << 33);
+        ww += peer64(&s.bin.sum[at], b);
       }
       cc += c0;
     }
@@ -290,7 +302,7 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
     const int i = threadIdx.x * each + e;
     if (e < each && i < per) {
       c2[e] = r.blocks > 1 ? peer32(&s.part_count[i], owner) : counts[i];
-      if (sums) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : sum_of(i);
+      if (sums) w2[e] = r.blocks > 1 ? peer64(&s.part_sum[i], owner) : s.bin.sum[i];
     }
   }
   uint64_t all, before_c = front_c + block_before64<THREADS>(c2[0] + c2[1], s.red, &all), before_s = 0;
@@ -318,32 +330,48 @@ __device__ __forceinline__ void clear_bins(Shared& s, bool sums) {
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS) {
     s.bin.count[i] = 0;
-    if (sums) s.bin.sum[0][i] = s.bin.sum[1][i] = s.bin.sum[2][i] = s.bin.sum[3][i] = 0;
+    if (sums) s.bin.sum[i] = 0;
   }
   __syncthreads();
 }
 
 __device__ __forceinline__ void add_to_bin(Shared& s, bool sums, int b, uint64_t w) {
   atomicAdd(&s.bin.count[b], 1u);
-  if (sums) {
-    atomicAdd(&s.bin.sum[0][b], (uint32_t)w & 0x7FFu);
-    atomicAdd(&s.bin.sum[1][b], (uint32_t)(w >> 11) & 0x7FFu);
-    atomicAdd(&s.bin.sum[2][b], (uint32_t)(w >> 22) & 0x7FFu);
-    atomicAdd(&s.bin.sum[3][b], (uint32_t)(w >> 33));
+  if (sums) {  // in halves, the carry by what the lower one held: an addition of 64 bits is a loop here
+    uint32_t* half = (uint32_t*)&s.bin.sum[b];
+    const uint32_t lo = (uint32_t)w, old = atomicAdd(half, lo);
+    atomicAdd(half + 1, (uint32_t)(w >> 32) + (old + lo < lo));
   }
 }
 
-// The logits from `low` on that `of` chooses, from all blocks, into the first block's list, which is empty (at most LIST of them).
+// The logits from `low` to `high` that `of` chooses, from all blocks, into the first block's list, which is empty (at most LIST of them).
 template <int THREADS, typename F>
-__device__ __forceinline__ void gather(const Row& r, float low, F&& of) {
+__device__ __forceinline__ void gather(const Row& r, float low, float high, F&& of) {
   Shared& s = r.s;
-  each<THREADS>(r, low, [&](float l, int i, bool in) {
+  auto take = [&](float l, int i) {
+    if (!(l >= low && l <= high)) return;
     const uint64_t p = r.place(l, i);
-    if (!in || !of(l, p)) return;
+    if (!of(l, p)) return;
     uint32_t at;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(remote(&s.n_list, 0)) : "memory");
     if (at < LIST) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&s.list.place[at], 0)), "l"(p) : "memory");
-  });
+  };
+  auto four = [&](const float4& v, int q) {
+    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= low)) return;
+    take(v.x, q * 4);
+    take(v.y, q * 4 + 1);
+    take(v.z, q * 4 + 2);
+    take(v.w, q * 4 + 3);
+  };
+  const int near = r.held / 4, all = (r.share + 3) / 4;
+#pragma unroll 1
+  for (int q = threadIdx.x; q < near; q += THREADS) four(((const float4*)r.near)[q], q);
+#pragma unroll 1
+  for (int q = near + threadIdx.x; q < all; q += 2 * THREADS) {
+    const float4 v0 = r.far(q), v1 = r.far(q + THREADS);
+    four(v0, q);
+    four(v1, q + THREADS);
+  }
   r.meet();
 }
 
@@ -386,9 +414,9 @@ __device__ __forceinline__ void rank_list(Shared& s, int n) {
 // The k-th largest of the groups' largest keys (to 22 bits, downwards) has at least k tokens from it on, and, where the largest are not all in a few
 // groups, not many more.
 template <int THREADS>
-__device__ __forceinline__ float crest_bound(const Row& r, int k) {
+__device__ __forceinline__ float crest_bound(const Row& r, int k, uint32_t* own) {
   const int i = threadIdx.x;
-  const uint32_t mine = i >= GROUPS ? 0 : r.blocks > 1 ? peer32(&r.s.crest[i % r.crests], i / r.crests) : r.s.crest[i];
+  const uint32_t mine = *own = i >= GROUPS ? 0 : r.blocks > 1 ? peer32(&r.s.crest[i % r.crests], i / r.crests) : r.s.crest[i];
   uint32_t low = 0;
 #pragma unroll 1
   for (uint32_t bit = 1u << 31; bit >= 1u << 10; bit >>= 1)
@@ -469,10 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   float top = -INFINITY;
-  int top_at = 0;
-  auto seen = [&](float l, int i) {  // a thread's indices rise, and NaN is not larger
-    if (l > top) top = l, top_at = i;
-  };
+  int top_q = -1;  // a thread's indices rise, and NaN is not larger
   constexpr int AHEAD = 5;
 #pragma unroll 1
   for (int q0 = threadIdx.x; q0 < (r.share + 3) / 4; q0 += THREADS * AHEAD) {
@@ -483,11 +508,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     for (int e = 0; e < AHEAD; e++) {
       const int q = q0 + e * THREADS;
       if (q < r.held / 4) ((float4*)near)[q] = v[e];
-      seen(v[e].x, q * 4);
-      seen(v[e].y, q * 4 + 1);
-      seen(v[e].z, q * 4 + 2);
-      seen(v[e].w, q * 4 + 3);
+      const float l = fmaxf(fmaxf(v[e].x, v[e].y), fmaxf(v[e].z, v[e].w));
+      if (l > top) top = l, top_q = q;
     }
+  }
+  int top_at = 0;
+  if (top_q >= 0) {
+    const float4 v = r.quad(top_q);  // what this thread has written
+    top_at = top_q * 4 + (v.x == top ? 0 : v.y == top ? 1 : v.z == top ? 2 : 3);
   }
   uint64_t best = top > -INFINITY ? r.place(top, top_at) : 0;
   // groups of neighbouring threads
@@ -499,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     const uint64_t v = __shfl_xor_sync(0xffffffffu, best, o);
     best = v > best ? v : best;
   }
-  if (threadIdx.x < 256) s.fraction[threadIdx.x] = __double_as_longlong(exp2(43.0 + threadIdx.x / 256.0));
+  if (threadIdx.x < 512) s.fraction[threadIdx.x] = __double_as_longlong(exp2(43.0 + threadIdx.x / 8 / 64.0));
   if (threadIdx.x == 0) s.n_list = 0;
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
@@ -526,8 +554,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   r.m32 = of_place(best);
   r.m = wide(__float_as_uint(r.m32));
   // beside +inf nothing has a weight
-  r.scale = r.m32 == INFINITY ? 1e30 : 256 * 1.4426950408889634074 / heat;
-  r.least_d = r.scale > 0 ? -11520.0 / r.scale : -1e300;
+  r.scale = r.m32 == INFINITY ? 1e30 : 64 * 1.4426950408889634074 / heat;
+  // 45 * 64 further down; to the next float above, since of the logits only floats are asked about
+  r.least_l = r.m32 == INFINITY ? INFINITY : r.scale > 0 ? __double2float_ru(r.m - 2880.0 / r.scale) : LEAST;
+  r.zero_l = __double2float_rd(r.m - 2944.0 / r.scale);
+  const double down = (r.m - (double)r.zero_l) * r.scale;  // what is left of it where floats lie far apart
+  r.plain = r.m32 < INFINITY && r.scale > 0 && r.zero_l >= LEAST && down >= 2912.0 && down <= 60000.0;
   r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
   if (r.m32 == INFINITY) r.m32 = -LEAST;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
   const int k = a.top_k ? a.top_k[row] : 0;
@@ -547,7 +579,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     if (!sums) {
       if (k <= 0 || k >= a.N) continue;
       if (2 * k <= GROUPS) {
-        gather<THREADS>(r, crest_bound<THREADS>(r, k), [](float, uint64_t) { return true; });
+        uint32_t own;
+        gather<THREADS>(r, crest_bound<THREADS>(r, k, &own), INFINITY, [](float, uint64_t) { return true; });
         few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
         if (few) {
           if (r.rank == 0) rank_list<THREADS>(s, (int)s.n_list);
@@ -563,20 +596,40 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
       if (!(top_p < 1.f)) continue;
       uint64_t sum = 0;
       const bool by_key = (from & 0xFFFFF) == 0;
-      each<THREADS>(r, low, [&](float l, int i, bool in) {
-        const uint64_t w = r.weight(l);
-        sum += in && (by_key || r.place(l, i) >= from) ? w : 0;
-      });
+      if (by_key && r.plain) {
+        const float cut = fmaxf(low, r.least_l);
+        const int near = r.held / 4, all = (r.share + 3) / 4;
+#pragma unroll 1
+        for (int q = threadIdx.x; q < near; q += THREADS) sum += r.weights(((const float4*)r.near)[q], cut);
+#pragma unroll 1
+        for (int q = near + threadIdx.x; q < all; q += 2 * THREADS) {
+          const float4 v0 = r.far(q), v1 = r.far(q + THREADS);
+          sum += r.weights(v0, cut) + r.weights(v1, cut);
+        }
+      } else {
+        each<THREADS>(r, low, [&](float l, int i, bool in) {
+          const uint64_t w = r.weight(l);
+          sum += in && (by_key || r.place(l, i) >= from) ? w : 0;
+        });
+      }
       sum = cluster_sum<THREADS>(r, sum, &s.weights);
       bool lost;
       want = share_of(sum, top_p, &lost);
       want = max((uint64_t)1, want + lost);
-      // The 256 largest and some more usually hold top_p.
+      // The 256 largest and some more usually hold top_p. They hold little more than the largest of the groups: where those do not come near,
+      // the pass is saved.
+      bool near_it = false;
+      float bound = 0.f;
       if (k <= 0 || 2 * k > GROUPS) {
+        uint32_t own;
+        bound = fmaxf(low, crest_bound<THREADS>(r, GROUPS / 2, &own));
+        const uint64_t crests = block_sum64<THREADS>(of_key(own) >= bound ? r.weight(of_key(own)) : 0, s.red);
+        near_it = crests + crests / 16 >= want;
+      }
+      if (near_it) {
         if (r.rank == 0 && threadIdx.x == 0) s.n_list = 0;
-        const float bound = fmaxf(low, crest_bound<THREADS>(r, GROUPS / 2));
         r.meet();
-        gather<THREADS>(r, bound, [&](float, uint64_t p) { return p >= from; });
+        gather<THREADS>(r, bound, INFINITY, [&](float, uint64_t p) { return p >= from; });
         if (r.rank == 0) {
           const int n = (int)s.n_list;
           uint64_t w = 0;
@@ -597,6 +650,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         const float reach = (float)(heat * log(ONE / tail) * 1.001) + fabsf(r.m32) * 1e-6f;
         if (reach < 1e30f) low = fmaxf(low, r.m32 - reach);
       }
+      // bins of what is left
+      const float width = r.m32 - low;
+      if (width < 32.f * heat) r.bin_scale = fminf((BINS - 1) / width, 1e30f);
     }
     int b0 = 0, hi = 52;
     uint64_t known = 0, left = want;
@@ -618,10 +674,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         auto weigh = [&](float l) { add_to_bin(s, sums, r.bin(l), sums ? r.weight(l) : 0); };
         const bool by_key = (from & 0xFFFFF) == 0;  // `from` begins a key
         const int all = (r.share + 3) / 4;
+        auto get = [&](int q) { return q < all ? r.quad(q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); };
+        float4 ahead[3];  // requested before they are needed: far ones come from memory
+#pragma unroll
+        for (int e = 0; e < 3; e++) ahead[e] = get(warp * 32 + lane + e * THREADS);
 #pragma unroll 1
         for (int q0 = warp * 32; q0 < all; q0 += THREADS) {
           const int q = q0 + lane;
-          const float4 v = q < all ? r.quad(q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          const float4 v = ahead[0];
+          ahead[0] = ahead[1];
+          ahead[1] = ahead[2];
+          ahead[2] = get(q + 3 * THREADS);
           if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= low)) continue;
           const float one[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -658,8 +721,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
       }
       if (few || c.count <= LIST) {
         // logits of bin b0 and in front of it, and a little more: the bin itself is looked at in what is left
-        const float deep = (b0 + 1.01f) / r.bin_scale + fabsf(r.m32) * 1e-6f;
-        gather<THREADS>(r, b0 < BINS - 1 && deep < 1e30f ? fmaxf(low, r.m32 - deep) : low, [&](float l, uint64_t p) {
+        const float slack = fabsf(r.m32) * 1e-6f, deep = (b0 + 1.01f) / r.bin_scale + slack, flat = (b0 - 0.01f) / r.bin_scale - slack;
+        gather<THREADS>(r, b0 < BINS - 1 && deep < 1e30f ? fmaxf(low, r.m32 - deep) : low, !few && flat > 0.f && flat < 1e30f ? r.m32 - flat : INFINITY, [&](float l, uint64_t p) {
           const int b = r.bin(l);
           return p >= from && (few ? b <= b0 : b == b0 && (!digits || p >> hi == known));
         });
@@ -695,14 +758,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     const uint64_t w = r.weight(l);
     return l >= low && (by_key || r.place(l, i) >= from) && w >= least ? w : 0;
   };
+  const bool simple = by_key && r.plain && least <= 1;
+  const float cut = fmaxf(low, r.least_l);
   auto kept4 = [&](const float4& v, int q) -> uint64_t {
+    if (simple) return r.weights(v, cut);
     if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= low)) return 0;
     return kept(v.x, q * 4) + kept(v.y, q * 4 + 1) + kept(v.z, q * 4 + 2) + kept(v.w, q * 4 + 3);
   };
-  constexpr int PIECE = 128;  // quads
   const int pieces = (r.share + 4 * PIECE - 1) / (4 * PIECE);
-  uint64_t* piece_sum = (uint64_t*)&s.bin;  // the bins are done with
-  static_assert(sizeof(s.bin) / 8 >= (1 << 20) / (4 * PIECE), "a sum for every piece of the longest share");
+  uint64_t* piece_sum = s.piece_sum;  // bins and list are done with
 #pragma unroll 1
   for (int p = warp; p < pieces; p += THREADS / 32) {
     float4 v[4];

@@ -795,7 +795,8 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
 }  // namespace
 
 int k_attn_paged_tiles(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  const bool one = (int64_t)a.max_new * (a.Hq / a.Hkv) <= BQ;  // one tile per sequence
+  // one tile per sequence, unless the two shares of so many rows would take more than 256 MB of scratch
+  const bool one = (int64_t)a.max_new * (a.Hq / a.Hkv) <= BQ && a.at.T * a.Hq * 2 * (a.D + 2) * 4 <= ((int64_t)256 << 20);
   if (a.D == 128) return one ? launch<2, true>(ctx, a) : launch<2, false>(ctx, a);
   return one ? launch<1, true>(ctx, a) : launch<1, false>(ctx, a);
 }

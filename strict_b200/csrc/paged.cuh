@@ -70,7 +70,7 @@ struct PagedWalk {
 };
 __device__ __forceinline__ PagedWalk paged_walk(const PagedView& v, int len, int lo_pos, int hi_pos, int window, int first, int kt) {
   PagedWalk w;
-  const int64_t room = (int64_t)v.ld << v.shift;
+  const int64_t room = min((int64_t)v.ld << v.shift, (int64_t)INT32_MAX - 1024);  // so that a tile's end is an int
   w.end = (int)(room < len ? room : len);
   w.end = max(0, min(w.end, hi_pos + 1));
   const int tiles = (w.end + kt - 1) / kt;

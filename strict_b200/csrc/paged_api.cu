@@ -13,6 +13,7 @@ namespace {
   if (!(ctx)) return sb_fail(STRICTB200_ERR_INVALID_ARG, "null context")
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
 
 // The checks that every operator over a paged cache makes, and its view of the cache.
 int paged_view(PagedView* v, const int32_t* table, const int32_t* lens, const int32_t* starts, int B, int64_t T, int n_pages, int page, int table_ld) {
@@ -20,6 +21,7 @@ int paged_view(PagedView* v, const int32_t* table, const int32_t* lens, const in
   SB_REQUIRE(n_pages > 0 && table_ld > 0, "bad shape: n_pages and table_ld must be positive");
   if (page < 16 || page > 256 || (page & (page - 1))) return sb_fail(STRICTB200_ERR_UNSUPPORTED, "pages hold 16, 32, 64, 128 or 256 positions");
   if (B && T) SB_REQUIRE(table && lens && starts, "null pointer");
+  SB_REQUIRE(aligned4(table) && aligned4(lens) && aligned4(starts), "table, lens and starts must be aligned to their type");
   int shift = 4;
   while ((1 << shift) < page) shift++;
   *v = PagedView{table, lens, starts, B, table_ld, n_pages, page, shift, T};
@@ -110,6 +112,8 @@ int strictb200_sample(strictb200_ctx* ctx, const void* logits, int dtype, int64_
   if (!M) return STRICTB200_OK;
   SB_REQUIRE(logits && u && out, "null pointer");
   SB_REQUIRE(((uintptr_t)logits & (dtype ? 3 : 1)) == 0, "logits must be aligned to their type");
+  SB_REQUIRE(aligned4(u) && aligned4(temperature) && aligned4(top_k) && aligned4(top_p) && aligned4(min_p) && aligned4(out) && aligned4(prob),
+             "arrays of a value per row must be aligned to their type");
   SB_ENTER(ctx);
   return k_draw(ctx, logits, dtype, M, N, ld, u, temperature, top_k, top_p, min_p, out, prob);
 }

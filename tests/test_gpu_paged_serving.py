@@ -266,3 +266,19 @@ def test_appends_of_many_tokens(ctx, Hq, Hkv, D, T):
     assert ((kk.double() - w[wrote][:, Hq:]).abs() <= bound[wrote][:, Hq:]).all() and torch.equal(vv, qkv.view(T, -1, D)[wrote][:, Hq + Hkv:])
     k[name[wrote], :, pos[wrote] % 64], v[name[wrote], :, pos[wrote] % 64] = kk, vv
     assert torch.equal(k, c.k) and torch.equal(v, c.v), "nothing else is written"
+
+
+def test_many_drafts(ctx):
+    """So many rows that two shares of each would take more scratch than they may."""
+    B, G = 1100, 16
+    rng = np.random.default_rng(3)
+    lens = [int(x) for x in rng.integers(2, 60, B)]
+    c = Cache(lens, [2] * B, 8, 128, 16, seed=3)
+    q = torch.randn(c.T, 8 * G, 128, generator=c.g, device="cuda").to(BF16)
+    out = c.attend(ctx, q)
+    few = list(range(0, B, 97)) + [B - 1]
+    for b in few:
+        rows = slice(c.starts[b], c.starts[b + 1])
+        want, size, scores = plain.attend(q[rows], c.k, c.v, c.table[b:b + 1], lens[b:b + 1], [0, 2], 0, 0, 128 ** -0.5, True)
+        bound = HALF * want.abs() + size * (2.0 ** -15 + 2 * scores * 130 * 2.0 ** -24 + 2 * 60 * 2.0 ** -24) + 1e-30
+        assert ((out[rows].double() - want).abs() <= bound * (1 + HALF)).all(), b

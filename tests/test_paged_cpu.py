@@ -95,3 +95,16 @@ def test_nothing_to_do_needs_nothing():
     copy([], [])
     copy([1], [2], pools=())
     sample(M=0, x=None, u=None, out=None)
+
+
+@pytest.mark.parametrize("name", ["table", "lens", "starts"])
+def test_index_arrays_that_are_not_aligned(name):
+    for call in (attn, rope):
+        with pytest.raises(ValueError, match="aligned"):
+            call(**{name: A + 2})
+
+
+@pytest.mark.parametrize("name", ["u", "t", "k", "p", "q", "out", "prob"])
+def test_row_arrays_that_are_not_aligned(name):
+    with pytest.raises(ValueError, match="aligned"):
+        sample(**{name: A + 1})

@@ -40,6 +40,7 @@ struct TilesArgs {
   int G, tw;       // heads per key/value head, tokens of a tile of 128 rows
   double inv_tb;   // 1 / tokens of a unit
   int one_round;   // a block for every unit
+  int direct;      // unit x is sequence x
   int* status;
 };
 
@@ -269,7 +270,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
         int tile;
         const int x = (int)(y / per);
         const bool one_round = t.one_round;
-        if (one_round ? u == 0 && place_unit(a.at, t.inv_tb, x, lane, &k.b, &tile)
+        if (t.direct) k.b = x, tile = 0;
+        if (t.direct ? x < a.at.B : one_round ? u == 0 && place_unit(a.at, t.inv_tb, x, lane, &k.b, &tile)
                       : a.at.B <= 32 ? find_unit<1>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile) : find_unit<4>(a.at, NQ * t.tw, t.inv_tb, x, lane, &k.b, &tile)) {
           k.part = (int)(y % per) / a.Hkv;
           k.hk = (int)(y % per) % a.Hkv;
@@ -778,6 +780,8 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   if (np > 1) SB_TRY(paged_join_scratch(ctx, a, np, &t.join));
   const int64_t blocks = std::min<int64_t>(tiles * a.Hkv * t.parts, ctx->sm_count);
   t.one_round = tiles * a.Hkv * t.parts <= ctx->sm_count;
+  // Sequences of one tile, more of them than the search keeps in registers: in their own order (1000 of at most 60 keys: 640 us searched for, 361 so; 256 of 1 to 2 thousand 474 and 357).
+  t.direct = !t.one_round && a.max_new <= tb && a.at.B > 128;
   CUtensorMap mq, mk, mv, mo;
   const int64_t rows = (int64_t)a.at.n_pages * a.Hkv * a.at.page;
   SB_TRY(map_tokens(&mq, a.q, a.at.T, a.Hq, a.D, t.G, t.tw));
@@ -795,8 +799,9 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
 }  // namespace
 
 int k_attn_paged_tiles(strictb200_ctx* ctx, const PagedAttnArgs& a) {
-  // one tile per sequence, unless the two shares of so many rows would take more than 256 MB of scratch
-  const bool one = (int64_t)a.max_new * (a.Hq / a.Hkv) <= BQ && a.at.T * a.Hq * 2 * (a.D + 2) * 4 <= ((int64_t)256 << 20);
+  // One tile where no sequence has more and the keys are many enough to pay for the join (20 rows: 16 sequences of 8192 keys 134 us with one tile and 161 with two, 256
+  // of 1 to 2 thousand 469 and 485, 500 of 200 to 600 702 and 613), and the two shares of all rows take at most 256 MB of scratch.
+  const bool one = (int64_t)a.max_new * (a.Hq / a.Hkv) <= BQ && paged_walk_tiles(a, BKV) >= 10 && a.at.T * a.Hq * 2 * (a.D + 2) * 4 <= ((int64_t)256 << 20);
   if (a.D == 128) return one ? launch<2, true>(ctx, a) : launch<2, false>(ctx, a);
   return one ? launch<1, true>(ctx, a) : launch<1, false>(ctx, a);
 }

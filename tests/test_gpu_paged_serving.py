@@ -189,9 +189,10 @@ def test_serving(ctx, Hq, Hkv, D, page, window, first):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("G,new", [(4, 2), (3, 3), (8, 2), (4, 4), (17, 1), (4, 5), (32, 1), (11, 3), (1, 16), (1, 17), (16, 8), (1, 128), (1, 129), (128, 1), (127, 2), (2, 64), (2, 65)])
 def test_where_kernels_change(ctx, D, G, new):
-    """Rows per sequence and key/value head around 8, 16, 128 and 256."""
+    """Rows per sequence and key/value head around 8, 16, 128 and 256, with few keys and with many."""
     lens = [new, new + 3, 130 + new, 700]
     Cache(lens, [new, new, new, max(1, new // 2)], 2, D, 16, seed=G).check(ctx, G)
+    Cache([1300, new + 1], [min(new, 9), min(new, 9)], 2, D, 16, seed=G).check(ctx, G)
 
 
 @pytest.mark.parametrize("B", [33, 150, 700])
@@ -202,6 +203,12 @@ def test_many_uneven_sequences(ctx, B, new):
     news = [min(n, int(rng.integers(0, new + 1))) for n in lens]
     news[B // 2], lens[B // 2] = new, max(new, lens[B // 2])
     Cache(lens, news, 2, 64, 16, seed=B, front=1, behind=2).check(ctx, 8)
+
+
+def test_many_sequences_with_many_keys(ctx):
+    """More than 128 sequences of one tile, the keys of each in two shares."""
+    lens = [1400 if b % 40 == 0 else 3 + b % 50 for b in range(170)]
+    Cache(lens, [3 if b % 7 else 0 for b in range(170)], 1, 128, 64, seed=1).check(ctx, 8)
 
 
 @pytest.mark.parametrize("new", [1, 3, 5])

@@ -18,7 +18,8 @@
 //   those in front of and in that bin go to the first block as above, if there are at most LIST        three meetings
 //   otherwise the place where the order is cut is found among those of the bin (in the first block if there are at most LIST, by bits of the place where
 //   more share the bin), and all blocks sum the kept weights and look for the token
-// Batches: two blocks per SM, so that one row's meetings are another's passes.
+// Many rows: a block per row, which keeps a part of it and reads the rest again from L2 in every pass; instruction issue bounds it (256 rows of 151936: 37 us
+// greedy, 75 with top_k 20, 105 unfiltered, 270 to 400 with a top_p of 0.9 over flat logits; one row 7.4, 13.4, 13.4, 42 to 57).
 #include <algorithm>
 
 #include "common.cuh"

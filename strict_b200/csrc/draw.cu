@@ -240,7 +240,6 @@ struct Crossing {
   uint64_t count;         // members of the bin
   uint64_t front;         // members of the bins in front
   uint64_t want;          // of the bin's own
-  bool whole;             // the bin is kept as a whole
 };
 template <int THREADS>
 __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want) {
@@ -317,13 +316,12 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
       s.pick[1] = c2[e];
       s.pick[2] = before_c;
       s.pick[3] = want - before;
-      s.pick[4] = sums ? c2[e] == 1 : here == want - before;
     }
     before_c += c2[e];
     before_s += w2[e];
   }
   __syncthreads();
-  return Crossing{(int)s.pick[0], s.pick[1], s.pick[2], s.pick[3], s.pick[4] != 0};
+  return Crossing{(int)s.pick[0], s.pick[1], s.pick[2], s.pick[3]};
 }
 
 template <int THREADS>
@@ -712,10 +710,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
       if (digits) {
         known = (hi < 52 ? known << (hi - lo) : 0) | (uint64_t)(mask - c.bin);
         hi = lo;
-        if (c.whole) {  // all that begin with these bits
-          from = max(from, known << hi);
-          break;
-        }
       } else {
         b0 = c.bin;
         few = c.front + c.count <= LIST;

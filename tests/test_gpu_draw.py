@@ -149,3 +149,21 @@ def test_recorded(ctx):
     ctx.synchronize()
     ctx.free_graph(ctx.last_graph)
     assert out.tolist() == [plain.draw(x[m].cpu().numpy(), float(u[m]), 1.0, 0, float(p[m]), 0.0)[0] for m in range(3)]
+
+
+@pytest.mark.parametrize("n", [1000, 20000, 60000])
+@pytest.mark.parametrize("at", [0.0, 1e6, -1e4])
+def test_cuts_at_the_end_of_many_equal_ones(ctx, n, at):
+    """A bin of more equal logits than a list holds is kept to its last, and a little further down a few more begin."""
+    rows = []
+    for few in (1, 2, 3):
+        x = torch.full((n,), at, dtype=torch.float32, device="cuda")
+        x[7], x[n // 2 : n // 2 + few], x[11] = at + 0.0625, at - 0.0625, at + 0.0625
+        rows += [x, x, x]
+    x = torch.stack(rows)
+    k = [v for few in (1, 2, 3) for v in (n - 1, n - few, n - few - 1)]
+    check(ctx, x, 0.999, temperature=0.7, top_k=np.array(k, np.int32))
+    check(ctx, x, 0.3, temperature=0.7, top_k=np.array(k, np.int32), top_p=0.5)
+    w = np.exp(-0.0625 / 0.7)  # what the largest and the many hold of the weight, and a little less
+    share = [(2 + (n - few - 2) * w - d) / (2 + (n - few - 2) * w + few * w * w) for few in (1, 2, 3) for d in (0.25, 0.75, 1.25)]
+    check(ctx, x, 0.999, temperature=0.7, top_p=np.array(share, np.float32))

@@ -19,7 +19,7 @@
 //   otherwise the place where the order is cut is found among those of the bin (in the first block if there are at most LIST, by bits of the place where
 //   more share the bin), and all blocks sum the kept weights and look for the token
 // Many rows: a block per row, which keeps a part of it and reads the rest again from L2 in every pass; instruction issue bounds it (256 rows of 151936: 37 us
-// greedy, 75 with top_k 20, 105 unfiltered, 270 to 400 with a top_p of 0.9 over flat logits; one row 7.4, 13.4, 13.4, 42 to 57).
+// greedy, 77 with top_k 20, 107 unfiltered, 270 to 400 with a top_p of 0.9 over flat logits; one row 7.4, 13.4, 13.4, 42 to 57).
 #include <algorithm>
 
 #include "common.cuh"
@@ -38,7 +38,7 @@ constexpr double ONE = 8796093022208.0;  // 2^43
 struct DrawArgs {
   const void* x;
   int64_t ld;
-  int N, f32;
+  int N, f32, M;
   const float *u, *temperature, *top_p, *min_p;
   const int32_t* top_k;
   int32_t* out;
@@ -470,6 +470,29 @@ __device__ __forceinline__ void end_row(const Row& r, const DrawArgs& a, int64_t
   }
 }
 
+// The row of this block, one to a block and at most a row per thread: first those whose top_p has no short list behind top_k, which take two to four times as
+// long as others (256 rows of mixed wishes: 219 us in the order of the rows, 171 so; 2 us where all are alike).
+template <int THREADS>
+__device__ __forceinline__ int long_ones_first(Shared& s, const DrawArgs& a) {
+  const int m = threadIdx.x, warp = m >> 5, lane = m & 31;
+  bool is_long = false;
+  if (m < a.M) {
+    const int k = a.top_k ? a.top_k[m] : 0;
+    is_long = a.top_p && a.top_p[m] < 1.f && (k <= 0 || 2 * k > GROUPS) && (!a.temperature || a.temperature[m] > 0.f);
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, is_long);
+  if (lane == 0) s.red[warp] = __popc(who);
+  const int all = __syncthreads_count(is_long);
+  int before = 0;
+  for (int i = 0; i < warp; i++) before += (int)s.red[i];
+  before += __popc(who & ((1u << lane) - 1));  // long ones in front of row m
+  if (m < a.M && (is_long ? before : all + m - before) == (int)blockIdx.x) s.there = m;
+  __syncthreads();
+  const int row = (int)s.there;
+  __syncthreads();
+  return row;
+}
+
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __grid_constant__ DrawArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -481,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   uint32_t rank, blocks;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
-  const int64_t row = blockIdx.x / blocks;
+  const int64_t row = THREADS == 1024 && blocks == 1 && a.M <= THREADS ? long_ones_first<THREADS>(s, a) : blockIdx.x / blocks;
   const int span = ((a.N + (int)blocks - 1) / (int)blocks + 7) / 8 * 8;
   Row r{s, near};
   r.x = (const char*)a.x + row * a.ld * (a.f32 ? 4 : 2);
@@ -833,7 +856,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
 
 int k_draw(strictb200_ctx* ctx, const void* x, int f32, int64_t M, int64_t N, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
            const float* top_p, const float* min_p, int32_t* out, float* prob) {
-  const DrawArgs a{x, ld, (int)N, f32, u, temperature, top_p, min_p, top_k, out, prob};
+  const DrawArgs a{x, ld, (int)N, f32, (int)std::min<int64_t>(M, INT32_MAX), u, temperature, top_p, min_p, top_k, out, prob};
   // Few rows: eight blocks of 512 threads for a long one, fewer where they hold it. Many rows: blocks of 1024 threads that have an SM each, as few to a row as keeps the SMs busy.
   int blocks = 1;
   while (blocks < MAX_CLUSTER && N > (int64_t)blocks * share_kept<512>()) blocks *= 2;

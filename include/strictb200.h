@@ -306,7 +306,7 @@ int strictb200_attn_decode_noalloc(strictb200_ctx* ctx, const uint16_t* d_q, con
 
 /* Per-head RMS norm (both gains NULL: none), rotation of the pairs (i, i + D/2) by the angle position * theta^(-2i/D), queries to d_q_out
  * [T,Hq,D], keys and values into the pages: strictb200_rope_qknorm_kvappend for a paged cache. d_qkv is [T, (Hq + 2 Hkv) * D]. Angles are reduced in
- * 64 bits: any position an int32 holds. Rows, gains and pages 16-byte aligned. */
+ * 64 bits: any position an int32 holds. Rows, gains and pages 16-byte aligned; d_q_out does not overlap d_qkv. */
 int strictb200_rope_qknorm_paged(strictb200_ctx* ctx, const uint16_t* d_qkv, const int32_t* d_table, const int32_t* d_lens, const int32_t* d_starts, int B,
                                  int64_t T, int Hq, int Hkv, int D, const float* d_qgain, const float* d_kgain, float eps, float theta, int n_pages,
                                  int page, int table_ld, uint16_t* d_q_out, uint16_t* d_kpages, uint16_t* d_vpages);

@@ -38,7 +38,8 @@ constexpr double ONE = 8796093022208.0;  // 2^43
 struct DrawArgs {
   const void* x;
   int64_t ld;
-  int N, f32, M;
+  int N, f32;
+  int M;  // rows, where their order may change
   const float *u, *temperature, *top_p, *min_p;
   const int32_t* top_k;
   int32_t* out;
@@ -554,6 +555,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
   for (int i = 0; i < (THREADS / 32); i++) best = s.red[i] > best ? s.red[i] : best;
+  const float heat = a.temperature ? a.temperature[row] : 1.f;  // read by all blocks before one of them may write a result
   if (threadIdx.x == 0) s.best = best;
   r.meet();
   if (r.blocks > 1) {
@@ -564,7 +566,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     for (int b = 0; b < MAX_CLUSTER; b++) best = v[b] > best ? v[b] : best;
   }
   const bool none = best >> 20 <= KEY_NONE;
-  const float heat = a.temperature ? a.temperature[row] : 1.f;
   if (none || !(heat > 0.f)) {
     if (rank == 0 && threadIdx.x == 0) {
       a.out[row] = none ? -1 : 0xFFFFF - (int)(best & 0xFFFFF);
@@ -856,7 +857,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
 
 int k_draw(strictb200_ctx* ctx, const void* x, int f32, int64_t M, int64_t N, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
            const float* top_p, const float* min_p, int32_t* out, float* prob) {
-  const DrawArgs a{x, ld, (int)N, f32, (int)std::min<int64_t>(M, INT32_MAX), u, temperature, top_p, min_p, top_k, out, prob};
+  // Blocks look at other rows' wishes for their order, unless those are written over by the results.
+  auto over = [&](const void* result, const void* wish) {
+    const uintptr_t r = (uintptr_t)result, w = (uintptr_t)wish, bytes = (uintptr_t)M * 4;
+    return result && wish && r < w + bytes && w < r + bytes;
+  };
+  bool in_order = false;
+  for (const void* wish : {(const void*)temperature, (const void*)top_k, (const void*)top_p}) in_order |= over(out, wish) || over(prob, wish);
+  const DrawArgs a{x, ld, (int)N, f32, in_order ? INT32_MAX : (int)M, u, temperature, top_p, min_p, top_k, out, prob};
   // Few rows: eight blocks of 512 threads for a long one, fewer where they hold it. Many rows: blocks of 1024 threads that have an SM each, as few to a row as keeps the SMs busy.
   int blocks = 1;
   while (blocks < MAX_CLUSTER && N > (int64_t)blocks * share_kept<512>()) blocks *= 2;

@@ -73,6 +73,8 @@ int strictb200_rope_qknorm_paged(strictb200_ctx* ctx, const uint16_t* qkv, const
   SB_REQUIRE(!qgain == !kgain, "gains for both queries and keys, or for neither");
   SB_REQUIRE(aligned16(qkv) && aligned16(q_out) && aligned16(kpages) && aligned16(vpages) && aligned16(qgain) && aligned16(kgain),
              "rows, gains and pages must be 16-byte aligned");
+  const uintptr_t in = (uintptr_t)qkv, to = (uintptr_t)q_out, in_bytes = (uintptr_t)T * (Hq + 2 * (uintptr_t)Hkv) * D * 2, to_bytes = (uintptr_t)T * Hq * D * 2;
+  SB_REQUIRE(to >= in + in_bytes || in >= to + to_bytes, "q_out overlaps qkv");  // a row's place in the one is another row's in the other
   a.qkv = (const bf16*)qkv; a.qgain = qgain; a.kgain = kgain; a.eps = eps; a.theta = theta; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
   a.q_out = (bf16*)q_out; a.k = (bf16*)kpages; a.v = (bf16*)vpages;
   SB_ENTER(ctx);

@@ -176,3 +176,20 @@ def test_many_rows_of_different_length(ctx, m):
     pick = lambda *v: np.array(rng.choice(v, m))  # noqa: E731
     check(ctx, logits(m, 20000, m), rng.random(m, np.float32), temperature=pick(0.0, 0.7, 1.0, 2.0).astype(np.float32), top_k=pick(0, 3, 300, 5000).astype(np.int32),
           top_p=pick(0.5, 0.9, 1.0).astype(np.float32), min_p=pick(0.0, 0.01).astype(np.float32))
+
+
+@pytest.mark.parametrize("m", [3, 400])
+def test_results_over_wishes(ctx, m):
+    """Tokens may be written over top_k, shares over top_p or the temperature: a row's wishes are read before its results are written."""
+    n = 20000
+    rng = np.random.default_rng(5)
+    x, u = logits(m, n, 5), torch.from_numpy(rng.random(m, np.float32)).cuda()
+    t, k, p = rng.choice([0.0, 1.0], m).astype(np.float32), rng.choice([0, 3, 300, 5000], m).astype(np.int32), rng.choice([0.5, 0.9, 1.0], m).astype(np.float32)
+    want = sample(ctx, x, u.cpu().numpy(), temperature=t, top_k=k, top_p=p)
+    for over_p in (True, False):
+        dt, dk, dp = (torch.from_numpy(v).cuda() for v in (t, k, p))
+        prob = dp if over_p else dt
+        torch.cuda.synchronize()
+        N.check(N.lib().strictb200_sample(ctx.h, x.data_ptr(), 1, m, n, n, u.data_ptr(), dt.data_ptr(), dk.data_ptr(), dp.data_ptr(), None, dk.data_ptr(), prob.data_ptr()))
+        ctx.synchronize()
+        assert np.array_equal(dk.cpu().numpy(), want[0]) and np.array_equal(prob.cpu().numpy(), want[1])

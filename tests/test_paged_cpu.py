@@ -108,3 +108,9 @@ def test_index_arrays_that_are_not_aligned(name):
 def test_row_arrays_that_are_not_aligned(name):
     with pytest.raises(ValueError, match="aligned"):
         sample(**{name: A + 1})
+
+
+@pytest.mark.parametrize("q", [A, A + 16, A + 2 * 12 * 128 * 2 - 16, A - 2 * 8 * 128 * 2 + 16])
+def test_append_refuses_queries_over_its_input(q):
+    with pytest.raises(ValueError, match="overlaps"):
+        rope(q=q)

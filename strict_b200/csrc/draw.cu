@@ -35,6 +35,19 @@ constexpr int share_kept() { return THREADS == 512 ? 19072 : 47488; }
 constexpr int MAX_CLUSTER = 8;
 constexpr double ONE = 8796093022208.0;  // 2^43
 
+}  // namespace
+
+// How far below the largest logit a row's logits may stay out of the bins where the order is cut at the weight `want` of `sum`. What is left out
+// together weighs sum - want at most: whole numbers none of which is above k = floor((sum - want) / N). That is what weights become that are below k + 1/2 before
+// they are rounded, so it is the distance of that weight, and a thousandth more, far above what a weight, this result and its difference from the largest logit
+// are off by. (From a k of 2^43 (1 - 4e-11) on a thousandth is less than that, but then `want` is below 2^43, which the largest logit has alone.)
+__host__ __device__ float sb_draw_reach(uint64_t sum, uint64_t want, int N, float heat, float top) {
+  const double bound = (double)((sum - want) / (uint64_t)N) + 0.5;
+  return (float)(heat * log(ONE / bound) * 1.001) + fabsf(top) * 1e-6f;
+}
+
+namespace {
+
 struct DrawArgs {
   const void* x;
   int64_t ld;
@@ -238,7 +251,7 @@ __device__ __forceinline__ void each(const Row& r, float low, F&& f) {
 // The bin where a running sum over the bins (sums: of weights, otherwise of counts) reaches `want`. The first block's list is empty afterwards, and its place free.
 struct Crossing {
   int bin;
-  uint64_t count;         // members of the bin
+  uint64_t count;         // members of the bin; 0: the sum of all bins is less, for all blocks alike, and the rest is undefined
   uint64_t front;         // members of the bins in front
   uint64_t want;          // of the bin's own
 };
@@ -308,6 +321,7 @@ __device__ __forceinline__ Crossing cross(const Row& r, bool sums, uint64_t want
   }
   uint64_t all, before_c = front_c + block_before64<THREADS>(c2[0] + c2[1], s.red, &all), before_s = 0;
   if (sums) before_s = front_s + block_before64<THREADS>(w2[0] + w2[1], s.red2, &all);
+  if (threadIdx.x == 0) s.pick[1] = 0;
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < 2; e++) {
@@ -667,12 +681,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         }
         r.meet();  // the word has been read
       }
-      // All weights up to (sum - want) / N together are at most sum - want: the cut is above them, and logits that far down (a thousandth further) stay out of the bins.
-      const double tail = (double)(sum - want) / a.N;
-      if (tail > 0) {
-        const float reach = (float)(heat * log(ONE / tail) * 1.001) + fabsf(r.m32) * 1e-6f;
-        if (reach < 1e30f) low = fmaxf(low, r.m32 - reach);
-      }
+      // logits that far down stay out of the bins: the cut is above them
+      const float reach = sb_draw_reach(sum, want, a.N, heat, r.m32);
+      if (reach < 1e30f) low = fmaxf(low, r.m32 - reach);
       // bins of what is left
       const float width = r.m32 - low;
       if (width < 32.f * heat) r.bin_scale = fminf((BINS - 1) / width, 1e30f);
@@ -730,6 +741,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
         if (lane < n) weigh(line[lane]);
       }
       const Crossing c = cross<THREADS>(r, sums, left);
+      if (c.count == 0) break;  // not reached: the bins hold `left`. Without it there is no cut.
       left = c.want;
       if (digits) {
         known = (hi < 52 ? known << (hi - lo) : 0) | (uint64_t)(mask - c.bin);

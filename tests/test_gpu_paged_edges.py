@@ -1,0 +1,62 @@
+"""The operators of a paged cache at the ends of what they take (plain forms: paged_plain.py)."""
+import numpy as np
+import pytest
+import torch
+
+from strict_b200 import native as N
+from test_gpu_draw import sample
+
+pytestmark = pytest.mark.gpu
+ONE = 2.0 ** 43
+
+
+def draw_whole(x, u, heat, top_k, top_p, min_p):
+    """Token and share of a row whose weights are whole numbers, 2^43 for the largest logit, in exact arithmetic."""
+    x = np.asarray(x, np.float32).astype(np.float64)
+    w = np.rint(np.exp((x - x.max()) / heat) * ONE).astype(np.uint64)
+    order = np.lexsort((np.arange(len(x)), -x))
+    keep = order[:top_k] if 0 < top_k < len(x) else order
+    sums = np.cumsum(w[keep])
+    if top_p < 1:
+        num, den = float(top_p).as_integer_ratio()
+        want = max(1, -(-int(sums[-1]) * num // den))
+        keep = keep[:int(np.searchsorted(sums, np.uint64(want), side="left")) + 1]
+    if min_p > 0:
+        keep = keep[w[keep] >= np.uint64(np.ceil(min(min_p, 1.0) * ONE))]
+    keep = np.sort(keep)
+    sums = np.cumsum(w[keep])
+    num, den = float(u).as_integer_ratio()
+    at = int(np.searchsorted(sums, np.uint64(int(sums[-1]) * num // den), side="right"))
+    return int(keep[at]), float(w[keep[at]]) / float(sums[-1])
+
+
+def check_whole(ctx, x, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    M = x.shape[0]
+    rows = [np.broadcast_to(np.asarray(v, t), (M,)) for v, t in ((u, np.float32), (heat, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+    got, prob = sample(ctx, x, rows[0], temperature=rows[1], top_k=rows[2], top_p=rows[3], min_p=rows[4])
+    host = x.float().cpu().numpy()
+    for m in range(M):
+        token, share = draw_whole(host[m], *[r[m].item() for r in rows])
+        # the quotient of two whole numbers, rounded to fp32 (by way of fp64)
+        assert got[m] == token and abs(float(prob[m]) - share) <= 2.0 ** -24 * (1 + 1e-6) * share, (m, got[m], token, prob[m], share)
+
+
+# Weights of the tail (6.6, 3.52, ..) are far enough from a half that every way to compute them rounds them alike.
+TAILS = [(151936, 6.6), (144000, 3.52), (50257, 10.8), (2 ** 20, 0.7), (20011, 26.3)]
+
+
+@pytest.mark.parametrize("peaks", [1, 3, 700])
+@pytest.mark.parametrize("n,weight", TAILS)
+@pytest.mark.parametrize("rows", [1, 5, 200])
+def test_top_p_next_to_one_over_a_flat_tail(ctx, n, weight, rows, peaks):
+    """Logits whose weights are rounded up to more than what top_p leaves out gives to each of them."""
+    if rows * n > 5_000_000:
+        rows = 3
+    for top, heat in ((0.0, 1.0), (28.5468, 0.7)):
+        x = torch.full((rows, n), float(np.float32(top + heat * np.log(weight / ONE))), device="cuda")
+        at = np.random.default_rng(n).choice(n, peaks, replace=False)
+        x[:, at] = top
+        u = np.linspace(0, 1 - 2.0 ** -24, rows).astype(np.float32)
+        for top_p in (1 - 2.0 ** -24, 1 - 2.0 ** -23, 0.9999999, 0.999999):
+            check_whole(ctx, x[:, :], u, heat, 0, top_p)
+        check_whole(ctx, x, u, heat, max(peaks + 1, n // 2), 1 - 2.0 ** -24)

@@ -186,7 +186,7 @@ __device__ bool find_unit(const PagedView& v, int tb, double inv_tb, int x, int 
   int rest = x - below;
   for (int b0 = 0; b0 < v.B; b0 += 32) {
     const UnitSeq u = seq(b0 + lane);
-    const int first = u.units - units_from(u, lo * BKV, inv_tb), c = u.units - first - units_from(u, hi * BKV, inv_tb);
+    const int first = u.units - units_from(u, lo * BKV, inv_tb), c = u.units - first - (hi > top / BKV ? 0 : units_from(u, hi * BKV, inv_tb));  // no unit ends there, and 128 hi may be 2^31
     int sum = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from strict_b200 import native as N
 from test_gpu_draw import sample
+from test_gpu_paged import Cache
 
 pytestmark = pytest.mark.gpu
 ONE = 2.0 ** 43
@@ -13,7 +13,9 @@ ONE = 2.0 ** 43
 def draw_whole(x, u, heat, top_k, top_p, min_p):
     """Token and share of a row whose weights are whole numbers, 2^43 for the largest logit, in exact arithmetic."""
     x = np.asarray(x, np.float32).astype(np.float64)
-    w = np.rint(np.exp((x - x.max()) / heat) * ONE).astype(np.uint64)
+    top = x.max()
+    w = np.where(x == top, ONE, 0.0) if top == np.inf else np.rint(np.exp((x - top) / heat) * ONE)  # beside infinity nothing weighs anything
+    w = w.astype(np.uint64)
     order = np.lexsort((np.arange(len(x)), -x))
     keep = order[:top_k] if 0 < top_k < len(x) else order
     sums = np.cumsum(w[keep])
@@ -30,7 +32,8 @@ def draw_whole(x, u, heat, top_k, top_p, min_p):
     return int(keep[at]), float(w[keep[at]]) / float(sums[-1])
 
 
-def check_whole(ctx, x, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0):
+def check_whole(ctx, x, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0, off=0.0):
+    """off: by how much a weight may differ, in units of the largest."""
     M = x.shape[0]
     rows = [np.broadcast_to(np.asarray(v, t), (M,)) for v, t in ((u, np.float32), (heat, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
     got, prob = sample(ctx, x, rows[0], temperature=rows[1], top_k=rows[2], top_p=rows[3], min_p=rows[4])
@@ -38,7 +41,7 @@ def check_whole(ctx, x, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0):
     for m in range(M):
         token, share = draw_whole(host[m], *[r[m].item() for r in rows])
         # the quotient of two whole numbers, rounded to fp32 (by way of fp64)
-        assert got[m] == token and abs(float(prob[m]) - share) <= 2.0 ** -24 * (1 + 1e-6) * share, (m, got[m], token, prob[m], share)
+        assert got[m] == token and abs(float(prob[m]) - share) <= 2.0 ** -24 * (1 + 1e-6) * share + x.shape[1] * off, (m, got[m], token, prob[m], share)
 
 
 # Weights of the tail (6.6, 3.52, ..) are far enough from a half that every way to compute them rounds them alike.
@@ -60,3 +63,24 @@ def test_top_p_next_to_one_over_a_flat_tail(ctx, n, weight, rows, peaks):
         for top_p in (1 - 2.0 ** -24, 1 - 2.0 ** -23, 0.9999999, 0.999999):
             check_whole(ctx, x[:, :], u, heat, 0, top_p)
         check_whole(ctx, x, u, heat, max(peaks + 1, n // 2), 1 - 2.0 ** -24)
+
+
+# ------------------------------------------------------------------ attention
+def attend_far(ctx, c, q, far, window=0, first=0, max_len=None):
+    """Sequence `far` is as long as an int32 says; what lies in the table is all that there is to see. Compared with a length just behind the table."""
+    c.d_lens[far] = 2 ** 31 - 1
+    out = c.attend(ctx, q, window, first, max_len=max_len)
+    c.lens[far] = c.ld * c.page + c.starts[far + 1] - c.starts[far]
+    c.compare(q, out, window, first)
+
+
+@pytest.mark.parametrize("new,G,far", [(1, 4, 0), (3, 4, 2), (12, 4, 0), (30, 4, 5), (100, 4, 0), (100, 4, 19), (150, 2, 7), (300, 1, 0)])
+@pytest.mark.parametrize("max_len", [None, 5000])
+def test_a_length_without_an_end(ctx, new, G, far, max_len):
+    """More units than SMs, so that each is searched for: the others' rows are there too."""
+    rng = np.random.default_rng(new)
+    lens = [int(x) + new for x in rng.integers(1, 500, 20)]
+    lens[far] = new + 700
+    c = Cache(lens, [new] * 20, 8, 64, 32, seed=new)
+    q = torch.randn(c.T, 8 * G, 64, generator=c.g, device="cuda").to(torch.bfloat16)
+    attend_far(ctx, c, q, far, max_len=max_len)

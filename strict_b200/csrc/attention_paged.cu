@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
       }
     }
     const float scale_log2 = a.scale * LOG2E;
-    const int lo_key = a.window ? lo_pos - a.window + 1 : 0;
+    const int lo_key = window_begin(lo_pos, a.window);
     const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
     uint32_t found = 0;
     bool ok = true;

@@ -60,7 +60,7 @@ __device__ __forceinline__ int share_count(int total, int part, int parts, int c
 // to r. Seldom, so slow. (A weight is positive; that it may have been rounded to zero does not matter to the sum: it is not finite either way.)
 static __device__ __noinline__ void add_poison(const PagedAttnArgs& a, const PagedWalk& w, int b, int hk, int part, int parts, int ct, int kt, int i0, int step, int n,
                                                int pos, int d0, int nd, float* r) {
-  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  const int lo = window_begin(pos, a.window);
   for (int i = i0; n > 0; n--, i += step) {
     const int k0 = w.tile(share_tile(i, part, parts, ct)) * kt;
     for (int j = k0; j < min(k0 + kt, min(w.end, pos + 1)); j++) {

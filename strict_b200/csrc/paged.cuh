@@ -60,6 +60,8 @@ __device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
   const int p = v.table[(int64_t)b * v.ld + n];
   return p >= 0 && p < v.n_pages ? p : -1;
 }
+// First position in the window of a row. Rows in front of their sequence (pos < 0) see nothing; counted from there, wide windows would pass 32 bits.
+__device__ __forceinline__ int window_begin(int pos, int window) { return window ? max(0, max(pos, 0) - window + 1) : 0; }
 // The key tiles (of `kt` positions) that rows at positions lo_pos .. hi_pos walk over: those of the first tokens, then those from the window on.
 struct PagedWalk {
   int first;  // tiles of the first tokens
@@ -74,7 +76,7 @@ __device__ __forceinline__ PagedWalk paged_walk(const PagedView& v, int len, int
   w.end = (int)(room < len ? room : len);
   w.end = max(0, min(w.end, hi_pos + 1));
   const int tiles = (w.end + kt - 1) / kt;
-  w.lo = window ? min(max(0, lo_pos - window + 1) / kt, tiles) : 0;
+  w.lo = min(window_begin(lo_pos, window) / kt, tiles);
   w.first = min((min(first, w.end) + kt - 1) / kt, w.lo);
   w.total = w.first + tiles - w.lo;
   return w;

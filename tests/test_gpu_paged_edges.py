@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+import paged_plain as plain
 from test_gpu_draw import sample
 from test_gpu_paged import Cache
 
@@ -84,3 +85,17 @@ def test_a_length_without_an_end(ctx, new, G, far, max_len):
     c = Cache(lens, [new] * 20, 8, 64, 32, seed=new)
     q = torch.randn(c.T, 8 * G, 64, generator=c.g, device="cuda").to(torch.bfloat16)
     attend_far(ctx, c, q, far, max_len=max_len)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 20, 2 ** 30 + 5])
+@pytest.mark.parametrize("lens,new", [([3, 40], [5, 9]), ([3, 40], [4, 1]), ([100, 500], [150, 30]), ([60, 3, 200], [70, 9, 200])])
+def test_windows_that_hide_nothing(ctx, window, lens, new):
+    """As wide as an int32 says, rows in front of their sequence among the new ones, and values that are not finite."""
+    for first in (0, 7, 2 ** 31 - 1):
+        c = Cache(lens, new, 2, 64, 16, seed=3)
+        q, out = c.check(ctx, 2, window, first)
+        assert torch.equal(out, c.attend(ctx, q))
+    c.v[int(c.table[0, 0]), :, 2, 5] = float("nan")
+    out = c.attend(ctx, q, window)
+    want = plain.attend(q, c.k, c.v, c.table, c.lens, c.starts, 0, 0, 64 ** -0.5)
+    assert torch.equal(out.isnan(), want.isnan())

@@ -627,7 +627,10 @@ size_t sb_argmax_scratch(int64_t M, int64_t N);  // bytes of chunk winners for t
 // draw.cu: a token per row under temperature, top-k, top-p and min-p (any of them null: without)
 int k_draw(strictb200_ctx*, const void* x, int f32, int64_t M, int64_t N, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
            const float* top_p, const float* min_p, int32_t* out, float* prob);
-__host__ __device__ float sb_draw_reach(uint64_t sum, uint64_t want, int N, float heat, float top);  // draw.cu
+// rules of draw.cu
+__host__ __device__ int sb_draw_top_k(int wish, int N);
+__host__ __device__ bool sb_draw_lists(int k);
+__host__ __device__ float sb_draw_reach(uint64_t sum, uint64_t want, int N, float heat, float top);
 int k_gather_rows(strictb200_ctx*, const void* src, const int32_t* rows, int64_t n_rows, int64_t row_bytes, void* dst);
 int k_add_i32(strictb200_ctx*, int32_t* x, const int32_t* inc, int32_t c, int64_t n);
 int k_f32_to_bf16(strictb200_ctx*, const float* x, int64_t n, bf16* y);

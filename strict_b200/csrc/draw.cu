@@ -37,6 +37,11 @@ constexpr double ONE = 8796093022208.0;  // 2^43
 
 }  // namespace
 
+// What a row's top_k cuts to: 0 where it is off, below 1 or from N on.
+__host__ __device__ int sb_draw_top_k(int wish, int N) { return wish > 0 && wish < N ? wish : 0; }
+// Whether the first k tokens are looked for in a list before there are bins: half as many as there are groups, so that seldom more come with them than it takes.
+__host__ __device__ bool sb_draw_lists(int k) { return k > 0 && k <= GROUPS / 2; }
+
 // How far below the largest logit a row's logits may stay out of the bins where the order is cut at the weight `want` of `sum`. What is left out
 // together weighs sum - want at most: whole numbers none of which is above k = floor((sum - want) / N). That is what weights become that are below k + 1/2 before
 // they are rounded, so it is the distance of that weight, and a thousandth more, far above what a weight, this result and its difference from the largest logit
@@ -492,8 +497,7 @@ __device__ __forceinline__ int long_ones_first(Shared& s, const DrawArgs& a) {
   const int m = threadIdx.x, warp = m >> 5, lane = m & 31;
   bool is_long = false;
   if (m < a.M) {
-    const int k = a.top_k ? a.top_k[m] : 0;
-    is_long = a.top_p && a.top_p[m] < 1.f && (k <= 0 || 2 * k > GROUPS) && (!a.temperature || a.temperature[m] > 0.f);
+    is_long = a.top_p && a.top_p[m] < 1.f && !sb_draw_lists(a.top_k ? sb_draw_top_k(a.top_k[m], a.N) : 0) && (!a.temperature || a.temperature[m] > 0.f);
   }
   const unsigned who = __ballot_sync(0xffffffffu, is_long);
   if (lane == 0) s.red[warp] = __popc(who);
@@ -599,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   r.plain = r.m32 < INFINITY && r.scale > 0 && r.zero_l >= LEAST && down >= 2912.0 && down <= 60000.0;
   r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
   if (r.m32 == INFINITY) r.m32 = -LEAST;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
-  const int k = a.top_k ? a.top_k[row] : 0;
+  const int k = a.top_k ? sb_draw_top_k(a.top_k[row], a.N) : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
   const uint64_t least = min_p > 0.f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * ONE) : 0;
   float u = a.u[row];
@@ -614,8 +618,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     by_count = !sums;
     float low = of_place(from);
     if (!sums) {
-      if (k <= 0 || k >= a.N) continue;
-      if (2 * k <= GROUPS) {
+      if (k == 0) continue;
+      if (sb_draw_lists(k)) {
         uint32_t own;
         gather<THREADS>(r, crest_bound<THREADS>(r, k, &own), INFINITY, [](float, uint64_t) { return true; });
         few = (r.blocks > 1 ? peer32(&s.n_list, 0) : s.n_list) <= LIST;
@@ -657,7 +661,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
       // the pass is saved.
       bool near_it = false;
       float bound = 0.f;
-      if (k <= 0 || 2 * k > GROUPS) {
+      if (!sb_draw_lists(k)) {
         uint32_t own;
         bound = fmaxf(low, crest_bound<THREADS>(r, GROUPS / 2, &own));
         const uint64_t crests = block_sum64<THREADS>(of_key(own) >= bound ? r.weight(of_key(own)) : 0, s.red);

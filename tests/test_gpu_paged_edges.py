@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import paged_plain as plain
-from test_gpu_draw import sample
+from test_gpu_draw import check, logits, sample
 from test_gpu_paged import Cache
 
 pytestmark = pytest.mark.gpu
@@ -64,6 +64,17 @@ def test_top_p_next_to_one_over_a_flat_tail(ctx, n, weight, rows, peaks):
         for top_p in (1 - 2.0 ** -24, 1 - 2.0 ** -23, 0.9999999, 0.999999):
             check_whole(ctx, x[:, :], u, heat, 0, top_p)
         check_whole(ctx, x, u, heat, max(peaks + 1, n // 2), 1 - 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rows", [5, 200])
+@pytest.mark.parametrize("top_k", [2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1, -2 ** 31])
+def test_top_k_beyond_every_row(ctx, rows, top_k):
+    """It is off, beside a top_p too, for few rows and for many."""
+    x, u = logits(rows, 20011, rows), np.random.default_rng(3).random(rows, np.float32)
+    for kw in (dict(top_p=0.9), dict(top_p=0.3, min_p=0.01), dict(top_p=0.95, temperature=3.0)):
+        got, want = sample(ctx, x, u, top_k=top_k, **kw), sample(ctx, x, u, **kw)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    check(ctx, x[:5], u[:5], top_k=top_k, top_p=0.9)
 
 
 # ------------------------------------------------------------------ attention

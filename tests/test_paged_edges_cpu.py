@@ -70,3 +70,13 @@ def test_bins_hold_what_top_p_wants_of_equal_logits(n):
 
 def test_an_infinite_heat_leaves_nothing_out():
     assert not reach(2 ** 43 * 10, 2 ** 43 * 3, 10, float("inf"), 1.0) < 1e30
+
+
+@pytest.mark.parametrize("wish,n,k,lists", [(0, 10, 0, False), (-1, 10, 0, False), (-2 ** 31, 10, 0, False), (1, 1, 0, False), (1, 2, 1, True), (9, 10, 9, True), (10, 10, 0, False),
+                                            (11, 10, 0, False), (256, 1000, 256, True), (257, 1000, 257, False), (256, 256, 0, False), (2 ** 20 - 1, 2 ** 20, 2 ** 20 - 1, False),
+                                            (2 ** 30, 2 ** 20, 0, False), (2 ** 30 + 1, 2 ** 20, 0, False), (2 ** 31 - 1, 2 ** 20, 0, False)])
+def test_top_k_of_every_size(wish, n, k, lists):
+    """Off below 1 and from the number of tokens on, however large; a list is tried for up to 256."""
+    cut, tried = N.lib()._Z13sb_draw_top_kii, N.lib()._Z13sb_draw_listsi
+    cut.restype, cut.argtypes, tried.restype, tried.argtypes = C.c_int, [C.c_int, C.c_int], C.c_bool, [C.c_int]
+    assert cut(wish, n) == k and tried(k) == lists

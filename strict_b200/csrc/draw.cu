@@ -71,10 +71,6 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ (~(uint32_t)((int32_t)k >> 31) | 0x80000000u)); }
 __device__ __forceinline__ float of_place(uint64_t p) { return of_key((uint32_t)(p >> 20)); }
-// A float's bits as a double's: exact for normal numbers, infinities become 2^128 (further than any number), subnormal ones others of no consequence.
-__device__ __forceinline__ double wide(uint32_t b) {
-  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29));
-}
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // of -inf
 constexpr float LEAST = -3.402823466e38f;  // of the logits that can be drawn
 
@@ -161,7 +157,7 @@ struct Row {
   // 2^43 exp((l - max) / T) rounded to a whole number. y = 64 log2(e) (l - max) / T = n + f with n whole and |f| <= 1/2: 2^(y / 64) is 2^(n / 64), from a table of
   // the 64 fractions, times the series of exp(f ln(2) / 64) to the fourth power (off by 4e-14 of the weight, a third of a unit at most). The sums that
   // round are additions of a power of two that leaves no bits behind the point. Straight-line, so that several go side by side.
-  // This is of a logit as a 64-bit number, with the bias of that addition; neither far away nor above the largest.
+  // This is of a logit as a 64-bit number, exactly (heats may be as small as the least numbers are), with the bias of that addition; neither far away nor above the largest.
   static constexpr uint64_t BIAS = 0x4330000000000000ull;
   __device__ __forceinline__ uint64_t weight_of(double x) const {
     const double d = x - m;
@@ -178,7 +174,7 @@ struct Row {
     return (uint64_t)__double_as_longlong(fma(p, __longlong_as_double(two), 4503599627370496.0));
   }
   __device__ __forceinline__ uint64_t weight(float l) const {  // of any logit
-    const uint64_t w = weight_of(wide(__float_as_uint(l))) - BIAS;
+    const uint64_t w = weight_of((double)fminf(l, -LEAST)) - BIAS;  // +inf as the largest number, which `m` is beside it
     return l >= least_l ? w : 0;
   }
   // The weights of four logits from `cut` on together, where `plain`: what is below counts as zero_l, whose weight is 0. (With a choice behind each weight, and
@@ -593,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
     return;
   }
   r.m32 = of_place(best);
-  r.m = wide(__float_as_uint(r.m32));
+  r.m = (double)fminf(r.m32, -LEAST);
   // beside +inf nothing has a weight
   r.scale = r.m32 == INFINITY ? 1e30 : 64 * 1.4426950408889634074 / heat;
   // 45 * 64 further down; to the next float above, since of the logits only floats are asked about

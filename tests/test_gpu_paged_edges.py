@@ -77,6 +77,24 @@ def test_top_k_beyond_every_row(ctx, rows, top_k):
     check(ctx, x[:5], u[:5], top_k=top_k, top_p=0.9)
 
 
+@pytest.mark.parametrize("heat", [1e-30, 1e-37, 1.2e-38, 1e-40, 1e-45])
+def test_heats_among_the_least_numbers(ctx, heat):
+    """Logits as near to one another as such heats are small: 0, subnormal numbers, the least normal ones."""
+    tiny = float(np.finfo(np.float32).tiny)
+    rows = []
+    for top in (0.0, -0.0, tiny, tiny / 8, -tiny / 4):
+        x = np.full(3000, -1.0, np.float32)
+        x[[5, 700, 2999]] = top
+        x[::7] = np.float32(top - heat)
+        x[[1, 9]] = np.float32(top - 3 * heat)
+        rows.append(x)
+    x = torch.from_numpy(np.stack(rows)).cuda()
+    for u in (0.0, 0.5, 0.99):
+        for kw in (dict(), dict(top_p=0.9), dict(top_p=0.999999, top_k=900), dict(min_p=0.1), dict(top_k=2)):
+            # running sums may meet their targets exactly, so by whole numbers: equal logits have equal ones, off by one at most
+            check_whole(ctx, x, u, heat, **kw, off=2.0 ** -43)
+
+
 # ------------------------------------------------------------------ attention
 def attend_far(ctx, c, q, far, window=0, first=0, max_len=None):
     """Sequence `far` is as long as an int32 says; what lies in the table is all that there is to see. Compared with a length just behind the table."""

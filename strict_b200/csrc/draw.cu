@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   r.zero_l = __double2float_rd(r.m - 2944.0 / r.scale);
   const double down = (r.m - (double)r.zero_l) * r.scale;  // what is left of it where floats lie far apart
   r.plain = r.m32 < INFINITY && r.scale > 0 && r.zero_l >= LEAST && down >= 2912.0 && down <= 60000.0;
-  r.bin_scale = fminf((BINS - 1) / (32.f * heat), 1e30f);
+  r.bin_scale = fmaxf(1e-36f, fminf((BINS - 1) / (32.f * heat), 1e30f));  // never 0: infinities are far from or in front of numbers at any heat
   if (r.m32 == INFINITY) r.m32 = -LEAST;  // bins below a largest logit of +inf: that one in the first, whatever is finite by its distance from the largest number
   const int k = a.top_k ? sb_draw_top_k(a.top_k[row], a.N) : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;

@@ -95,6 +95,23 @@ def test_heats_among_the_least_numbers(ctx, heat):
             check_whole(ctx, x, u, heat, **kw, off=2.0 ** -43)
 
 
+@pytest.mark.parametrize("heat", [1e36, 1e38, float("inf")])
+@pytest.mark.parametrize("rows", [2, 150])
+def test_heats_without_an_end(ctx, heat, rows):
+    """Everything weighs the same; beside infinities nothing else does."""
+    n = 20011
+    x = logits(rows, n, 3)
+    u = np.linspace(0, 1 - 2.0 ** -24, rows).astype(np.float32)
+    some = torch.randperm(n, generator=torch.Generator("cuda").manual_seed(1), device="cuda")[:1000]
+    for fill in (None, float("inf"), torch.finfo(torch.float32).max):
+        if fill is not None:
+            x[:, some] = fill
+        for kw in (dict(), dict(top_k=300), dict(top_k=999), dict(top_k=1000), dict(top_k=1001), dict(top_p=0.25), dict(top_k=700, top_p=0.5), dict(top_k=2000, top_p=0.9)):
+            if rows > 2 and len(kw) != 1:
+                continue
+            check_whole(ctx, x, u, heat, **kw, off=2.0 ** -43)  # weights below 2^-44 of the largest are 0, the others here are all the same
+
+
 # ------------------------------------------------------------------ attention
 def attend_far(ctx, c, q, far, window=0, first=0, max_len=None):
     """Sequence `far` is as long as an int32 says; what lies in the table is all that there is to see. Compared with a length just behind the table."""

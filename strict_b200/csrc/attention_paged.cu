@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
   const int last = a.at.starts[b + 1], len = a.at.lens[b];
   if (t0 < 0 || last > a.at.T || last <= t0) return;  // the same for every block of a cluster
   const int R = (int)min((int64_t)ROWS / G, last - t0) * G, lo_pos = len - last + (int)t0, hi_pos = lo_pos + R / G - 1;
-  const PagedWalk w = paged_walk(a.at, len, lo_pos, hi_pos, a.window, a.first, KT);
+  const int lo_key = window_begin(lo_pos, a.window);
+  const PagedWalk w = paged_walk(a.at, len, lo_key, hi_pos, a.first, KT);
   const int n = share_count(w.total, part, parts, ct);
   const uint32_t sK = smem_u32(smem), sV = sK + stages * TILE;
   auto row_head = [&](int row) { return (t0 + row / G) * a.Hq + hk * G + row % G; };  // place among all rows and heads
@@ -152,7 +153,6 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
       }
     }
     const float scale_log2 = a.scale * LOG2E;
-    const int lo_key = window_begin(lo_pos, a.window);
     const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
     uint32_t found = 0;
     bool ok = true;

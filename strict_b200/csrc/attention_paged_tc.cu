@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
           k.lo_pos = len - n_new + q0;
           k.lo_key = window_begin(k.lo_pos, a.window);
           k.n = sb < 0 || (int64_t)sb + n_new > a.at.T || q0 < 0 ? 0 : max(0, min(NQ * t.tw, n_new - q0));  // nothing where starts or lengths are none
-          k.w = paged_walk(a.at, len, k.lo_pos, k.lo_pos + k.n - 1, a.window, a.first, BKV);
+          k.w = paged_walk(a.at, len, k.lo_key, k.lo_pos + k.n - 1, a.first, BKV);
           k.ct = max(1, (k.w.total + t.parts - 1) / t.parts);
           k.nt = k.n ? share_count(k.w.total, k.part, t.parts, k.ct) : 0;
           if (ONE) {  // every other tile
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
       const bool any_live = __any_sync(0xffffffffu, live);  // a warp without rows only keeps step
       const int pos_a = k.lo_pos + (ONE ? 0 : w * t.tw), pos_b = k.lo_pos + min(k.n, (ONE ? 1 : 1 + w) * t.tw) - 1;  // positions of the stream's tokens
       const int pos = k.lo_pos + tok;
-      const int lo = window_begin(pos, a.window);
+      const int lo = a.window ? max(0, (int)((uint32_t)pos - a.window + 1)) : 0;  // a row in front of its sequence sees nothing, wherever this lies
       float m_run = -INFINITY, l_run = 0.f;
       for (int s = 0; s < nt; s++, steps++) {
         const uint32_t ph = (uint32_t)(steps & 1);

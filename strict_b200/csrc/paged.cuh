@@ -62,7 +62,8 @@ __device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
 }
 // First position in the window of a row. Rows in front of their sequence (pos < 0) see nothing; counted from there, wide windows would pass 32 bits.
 __device__ __forceinline__ int window_begin(int pos, int window) { return window ? max(0, max(pos, 0) - window + 1) : 0; }
-// The key tiles (of `kt` positions) that rows at positions lo_pos .. hi_pos walk over: those of the first tokens, then those from the window on.
+// The key tiles (of `kt` positions) that rows up to position hi_pos walk over, the window of whose first one begins at lo_key: those of the first tokens, then those from
+// the window on.
 struct PagedWalk {
   int first;  // tiles of the first tokens
   int lo;     // tile where the window begins
@@ -70,13 +71,13 @@ struct PagedWalk {
   int end;    // no row sees this position or a later one
   __device__ __forceinline__ int tile(int t) const { return t < first ? t : lo + t - first; }
 };
-__device__ __forceinline__ PagedWalk paged_walk(const PagedView& v, int len, int lo_pos, int hi_pos, int window, int first, int kt) {
+__device__ __forceinline__ PagedWalk paged_walk(const PagedView& v, int len, int lo_key, int hi_pos, int first, int kt) {
   PagedWalk w;
   const int64_t room = min((int64_t)v.ld << v.shift, (int64_t)INT32_MAX - 1024);  // so that a tile's end is an int
   w.end = (int)(room < len ? room : len);
   w.end = max(0, min(w.end, hi_pos + 1));
   const int tiles = (w.end + kt - 1) / kt;
-  w.lo = min(window_begin(lo_pos, window) / kt, tiles);
+  w.lo = min(lo_key / kt, tiles);
   w.first = min((min(first, w.end) + kt - 1) / kt, w.lo);
   w.total = w.first + tiles - w.lo;
   return w;

@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES];
   __shared__ uint32_t page_bits[MAX_STAGES];
-  __shared__ int poison;
+  __shared__ Poison poison;
   const int part = blockIdx.x, parts = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = a.Hq / a.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3, mi = lane >> 3, r8 = lane & 7;
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
       tc::mbar_init(smem_u32(&full[i]), 1);
       tc::mbar_init(smem_u32(&empty[i]), WARPS);
     }
-    poison = 0;
+    poison.n = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
     }
     const float scale_log2 = a.scale * LOG2E;
     const uint32_t sw = (uint32_t)r8 << 4;  // chunk c of row r lies at chunk c ^ (r & 7)
-    uint32_t found = 0;
     bool ok = true;
     int st = 0, step = part * ct, left = ct;  // place in the walk, tiles of the piece
     uint32_t ph = 0;
@@ -241,6 +240,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
 #pragma unroll
         for (int j = 0; j < 4; j++) ldsm_x4_t(tV + (j4 >> 2) * ATOM + ((mi >> 1) * 8 + r8) * 128 + (((j * 2 + (mi & 1)) << 4) ^ sw), vf[j]);
         if (!whole) {
+          uint32_t found = 0;
 #pragma unroll
           for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
               found |= not_finite(vf[j][x] & seen[x >> 1]);  // this thread's keys are j0 + 8 (x / 2) + 2 tig and the next one
               vf[j][x] = only_finite(vf[j][x]);
             }
+          if (__any_sync(0xffffffffu, found != 0) && lane == 0) note_poison(poison, i);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -263,7 +264,6 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
       if (++st == stages) st = 0, ph ^= 1;
     }
     if (!__all_sync(0xffffffffu, ok) && lane == 0) tc::set_status(status, 48);
-    if (found) poison = 1;
 #pragma unroll
     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
       }
   }
   __syncthreads();
-  const bool bad = poison;
+  const bool bad = poison.n > 0;
   for (int e = threadIdx.x; e < R * (HD / 4); e += BLOCK) {
     const int row = e / (HD / 4), d = e % (HD / 4) * 4;
     float M = -INFINITY, L = 0.f;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(160, few_fit<HD, NB>()) attn_paged_few_kernel(
     }
     if (bad && L != 0.f) {
       float r[4] = {O.x, O.y, O.z, O.w};
-      add_poison(a, w, b, hk, part, parts, ct, KT, 0, 1, n, lo_pos + row / G, d, 4, r);
+      add_poison(a, w, b, hk, part, parts, ct, KT, 16, lo_pos, hi_pos, poison, 0, 1, n, lo_pos + row / G, d, 4, r);
       O = make_float4(r[0], r[1], r[2], r[3]);
     }
     if (JOIN == JOIN_NONE) {

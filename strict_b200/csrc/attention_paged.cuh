@@ -54,23 +54,46 @@ __device__ __forceinline__ int share_count(int total, int part, int parts, int c
   return rounds * ct + min(max(rest - part * ct, 0), ct);
 }
 
-
 // What a weight of zero times a value that is not finite would do to a row that does not see it is avoided by zeros in place of such values in tiles that some
-// row does not see whole. Where there were any, a row that does see them gets them here: those of the n tiles i0, i0 + step .. of a block, dims d0 .. d0 + nd - 1, added
-// to r. Seldom, so slow. (A weight is positive; that it may have been rounded to zero does not matter to the sum: it is not finite either way.)
-static __device__ __noinline__ void add_poison(const PagedAttnArgs& a, const PagedWalk& w, int b, int hk, int part, int parts, int ct, int kt, int i0, int step, int n,
-                                               int pos, int d0, int nd, float* r) {
-  const int lo = window_begin(pos, a.window);
-  for (int i = i0; n > 0; n--, i += step) {
-    const int k0 = w.tile(share_tile(i, part, parts, ct)) * kt;
-    for (int j = k0; j < min(k0 + kt, min(w.end, pos + 1)); j++) {
-      if (j < lo && j >= a.first) continue;
-      const int page = paged_page(a.at, b, j >> a.at.shift);
-      if (page < 0) continue;
-      const bf16* v = a.v + ((page * (int64_t)a.Hkv + hk) * a.at.page + (j & (a.at.page - 1))) * a.D + d0;
-      for (int d = 0; d < nd; d++) {
-        const float x = __bfloat162float(v[d]);
-        if (!isfinite(x)) r[d] += x;
+// row does not see whole. Tiles of a block's share where that befell values that some row may see (the i-th ones, some of them more than once; more than
+// POISON_TILES: any of the share).
+constexpr int POISON_TILES = 24;
+struct Poison {
+  int n, tile[POISON_TILES];
+};
+__device__ __forceinline__ void note_poison(Poison& p, int i) {  // one lane of a warp
+  const int at = atomicAdd(&p.n, 1);
+  if (at < POISON_TILES) p.tile[at] = i;
+}
+// A row that does see such values gets them here: those of the n tiles i0, i0 + step .. of a block, dims d0 .. d0 + nd - 1 (nd % 4 == 0), added to r. Only groups of
+// `grain` keys are gone through that the rows lo_pos .. hi_pos do not see whole, as where the values were replaced: a walk over a whole long sequence would
+// hold up a call of 48 us for 1.4 ms at 16000 keys, and with it the other warps of a block that stays. Seldom, so slow. (A weight is positive; that it may have been rounded to zero does
+// not matter to the sum: it is not finite either way, and neither does a value that is added twice.)
+static __device__ __noinline__ void add_poison(const PagedAttnArgs& a, const PagedWalk& w, int b, int hk, int part, int parts, int ct, int kt, int grain, int lo_pos,
+                                               int hi_pos, const Poison& noted, int i0, int step, int n, int pos, int d0, int nd, float* r) {
+  const int lo = window_begin(pos, a.window), many = *(volatile const int*)&noted.n;
+  const bool any = many > POISON_TILES;
+  for (int x = 0; x < (any ? n : many); x++) {
+    const int i = any ? i0 + x * step : *(volatile const int*)&noted.tile[x];
+    if (i < i0 || (i - i0) % step || (i - i0) / step >= n) continue;  // another stream's
+    const int k0 = w.tile(share_tile(i, part, parts, ct)) * kt, end = min(k0 + kt, min(w.end, pos + 1));
+    for (int g0 = k0; g0 < end; g0 += grain) {
+      bool whole = sees_all(a, w.end, g0, grain, lo_pos, hi_pos);
+      for (int j = g0; whole && j < g0 + grain; j += a.at.page) whole = paged_page(a.at, b, j >> a.at.shift) >= 0;
+      if (whole) continue;
+      for (int j = g0; j < min(g0 + grain, end); j++) {
+        if (j < lo && j >= a.first) continue;
+        const int page = paged_page(a.at, b, j >> a.at.shift);
+        if (page < 0) continue;
+        const bf16* v = a.v + ((page * (int64_t)a.Hkv + hk) * a.at.page + (j & (a.at.page - 1))) * a.D + d0;
+        for (int d = 0; d < nd; d += 4) {
+          const uint2 y = *(const uint2*)(v + d);
+          if (!(not_finite(y.x) | not_finite(y.y))) continue;
+          for (int e = 0; e < 4; e++) {
+            const float z = __bfloat162float(v[d + e]);
+            if (!isfinite(z)) r[d + e] += z;
+          }
+        }
       }
     }
   }

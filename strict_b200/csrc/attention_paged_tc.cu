@@ -55,7 +55,6 @@ struct Unit {
   PagedWalk w;
   int ct;           // tiles of a part: what a unit sees is cut evenly (pieces cut by the longest sequence took 132 us where these take 84, uneven drafts)
   int nt, nt_w[2];  // key tiles of the unit and of each stream
-  int poison;       // values that are not finite were replaced
 };
 
 // What the issuing warp executes as a whole, one lane of it acting: operands that the compiler knows to be the same in all lanes need not be moved to
@@ -205,6 +204,11 @@ __device__ bool find_unit(const PagedView& v, int tb, double inv_tb, int x, int 
   return false;
 }
 
+// Of a row of a unit: 32 dims from d0 on. Everything else is looked up again here (as arguments they cost the softmax warps registers: 185 us a chunk instead of 177).
+__device__ __noinline__ void add_poison(const TilesArgs& t, const Unit& k, const Poison& noted, bool one, int w, int nt, int pos, int d0, float* r) {
+  add_poison(t.a, k.w, k.b, k.hk, k.part, t.parts, k.ct, BKV, BKV, k.lo_pos, k.lo_pos + k.n - 1, noted, one ? w : 0, one ? 2 : 1, nt, pos, d0, 32, r);
+}
+
 template <int QA, bool ONE>
 __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
@@ -216,6 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
   __shared__ __align__(8) uint64_t unit_full[2], unit_empty[2], q_full, q_empty, k_full[RING], k_empty[RING], v_full[RING], v_ready[RING], v_empty[RING], bar_s[2],
       bar_p[2][2], bar_o[2], o_free[2];
   __shared__ Unit units[2];
+  __shared__ Poison poison[2];  // of these units
   __shared__ uint32_t tmem_base_slot;
   __shared__ uint32_t page_bits[8];  // pages of a key tile that are there
   const PagedAttnArgs& a = t.a;
@@ -293,12 +298,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
             k.nt_w[1] = k.n > t.tw ? k.nt : 0;
             k.nt = max(k.nt_w[0], k.nt_w[1]);
           }
-          k.poison = 0;
         }
         if (u >= 2) good = warp_wait(smem_u32(&unit_empty[u & 1]), (uint32_t)(u >> 1 & 1) ^ 1);
         if (!good) break;
         if (lane == 0) {
           units[u & 1] = k;
+          poison[u & 1].n = 0;
           asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&unit_full[u & 1])) : "memory");
         }
         __syncwarp();
@@ -470,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
       int c = 0;
       bool good = true;
       for (int u = 0; good && next_unit(u); u++) {
-        Unit& k = units[u & 1];
+        const Unit& k = units[u & 1];
         const PagedWalk w = k.w;
         const int nt = k.nt, part = k.part, ct = k.ct, lo_pos = k.lo_pos, hi_pos = k.lo_pos + k.n - 1, lo_key = k.lo_key;
         for (int i = 0; i < nt; i++, c++) {
@@ -498,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
                 v[x] = make_uint4(only_finite(z.x), only_finite(z.y), only_finite(z.z), only_finite(z.w));
               }
             }
-            if (found) k.poison = 1;
+            if (__any_sync(0xffffffffu, found != 0) && lane == 0) note_poison(poison[u & 1], i);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
           asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&v_ready[st])) : "memory");
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
       const int np = ONE ? 2 * t.parts : t.parts, p = ONE ? 2 * part + w : part;
       const float inv = np > 1 ? 1.f : l_run == 0.f ? 0.f : 1.0f / l_run;
       if (np > 1 && live) t.join.ml[at * np + p] = make_float2(m_run, l_run);
-      const bool bad = nt > 0 && any_live && k.poison;
+      const bool bad = __any_sync(0xffffffffu, *(volatile int*)&poison[u & 1].n > 0) && nt > 0 && any_live;  // of the warp; later tiles of the other stream may still add to it
       if (bad) {
 #pragma unroll 1
         for (int c32 = 0; c32 < 2 * QA; c32++) {
@@ -641,7 +646,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_tiles_kernel(const __gr
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
-          if (live) add_poison(a, walk, k.b, k.hk, part, t.parts, ct, BKV, ONE ? w : 0, ONE ? 2 : 1, nt, pos, c32 * 32, 32, f);
+          if (live) add_poison(t, k, poison[u & 1], ONE, w, nt, pos, c32 * 32, f);
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 32; j++) r[j] = __float_as_uint(f[j]);

@@ -1,4 +1,6 @@
 """The operators of a paged cache at the ends of what they take (plain forms: paged_plain.py)."""
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -145,3 +147,56 @@ def test_windows_that_hide_nothing(ctx, window, lens, new):
     out = c.attend(ctx, q, window)
     want = plain.attend(q, c.k, c.v, c.table, c.lens, c.starts, 0, 0, 64 ** -0.5)
     assert torch.equal(out.isnan(), want.isnan())
+
+
+def milliseconds(ctx, call, n=5):
+    """The least of n calls, by the host's clock around calls that are waited for."""
+    best = 1e9
+    for _ in range(n):
+        ctx.synchronize()
+        t = time.perf_counter()
+        call()
+        ctx.synchronize()
+        best = min(best, (time.perf_counter() - t) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("new,D", [(1, 128), (6, 64), (25, 128), (200, 128)])
+def test_one_nan_does_not_hold_up_a_long_sequence(ctx, new, D):
+    """Values that are not finite, in tiles that some row does not see, are looked up again in those tiles only, however long the sequence is."""
+    lens = [16000 + new, 300 + new, 500 + new]
+    c = Cache(lens, [new] * 3, 2, D, 16, seed=new)
+    q = torch.randn(c.T, 8, D, generator=c.g, device="cuda").to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    call = lambda: c.attend(ctx, q, out=out)  # noqa: E731
+    call()
+    before, fine = milliseconds(ctx, call), out.clone()
+    c.v[int(c.table[0, (lens[0] - 1) // 16]), :, (lens[0] - 1) % 16, 9] = float("nan")  # the last position: only the last row sees it
+    c.v[int(c.table[0, 3]), :, 5, 11] = -float("inf")  # all rows see this one
+    after = milliseconds(ctx, call)
+    last = c.starts[1] - 1
+    assert out[last, :, 9].isnan().all() and not out[:c.starts[1], :, 11].isfinite().any()
+    same = torch.ones_like(q, dtype=torch.bool)
+    same[last, :, 9], same[:c.starts[1], :, 11] = False, False
+    assert torch.equal(out[same], fine[same])
+    assert after < 2 * before + 0.3, (before, after)
+
+
+@pytest.mark.parametrize("new,G,D", [(1, 4, 64), (5, 3, 128), (25, 4, 64), (90, 4, 128), (400, 2, 64)])
+@pytest.mark.parametrize("window,first", [(0, 0), (900, 300)])
+def test_values_that_are_not_finite_between_pages_that_are_missing(ctx, new, G, D, window, first):
+    """Many tiles that no row sees whole, each with such values in a dim of its own: more of them than a block takes down, and few."""
+    for every in (1, 9):
+        c = Cache([3000, 700], [new, new], 2, D, 16, seed=new + every)
+        q = torch.randn(c.T, 2 * G, D, generator=c.g, device="cuda").to(torch.bfloat16)
+        for b in (0, 1):
+            for i in range(0, c.lens[b] // 16 - 4, 5):
+                c.table[b, i + 1] = -1
+                if i // 5 % every == 0:
+                    c.v[int(c.table[b, i]), :, i % 16, i // 5 % D] = float("nan") if i % 2 else float("inf")
+            c.v[int(c.table[b, (c.lens[b] - 1) // 16]), :, (c.lens[b] - 1) % 16, D - 1] = float("nan")
+        out = c.attend(ctx, q, window, first)
+        want = plain.attend(q, c.k, c.v, c.table, c.lens, c.starts, window, first, D ** -0.5)
+        assert torch.equal(out.isfinite(), want.isfinite())
+        fine = want.isfinite()
+        assert ((out.double() - want).abs()[fine] < 2 * torch.finfo(torch.bfloat16).eps * want.abs()[fine] + 1e-3).all()  # roundings are test_chunks' business

@@ -315,7 +315,8 @@ int strictb200_rope_qknorm_paged(strictb200_ctx* ctx, const uint16_t* d_qkv, con
  * or j < first (the first tokens stay visible). What a row does not see does not reach it, whatever is there, and pages that no row
  * sees are not read. A row that sees no key with a score above -inf gets zeros; one that sees values that are not finite, values that are not finite. max_new: no sequence has more new tokens (of one
  * that has, further rows of out are undefined); max_len: how long the sequences are at most, for planning (longer ones are computed too). scale: positive.
- * Uses context scratch where keys are split. At most 128 query heads per key/value head. q, pages and out 16-byte aligned. */
+ * Uses context scratch where keys are split. At most 128 query heads per key/value head. q, pages and out 16-byte aligned. d_out may be d_q; otherwise it
+ * overlaps neither d_q nor the pages. */
 int strictb200_attn_paged(strictb200_ctx* ctx, const uint16_t* d_q, const uint16_t* d_kpages, const uint16_t* d_vpages, const int32_t* d_table,
                           const int32_t* d_lens, const int32_t* d_starts, int B, int64_t T, int max_new, int max_len, int Hq, int Hkv, int D, int n_pages,
                           int page, int table_ld, int window, int first, float scale, uint16_t* d_out);

@@ -14,6 +14,9 @@ namespace {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
+bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
 
 // The checks that every operator over a paged cache makes, and its view of the cache.
 int paged_view(PagedView* v, const int32_t* table, const int32_t* lens, const int32_t* starts, int B, int64_t T, int n_pages, int page, int table_ld) {
@@ -54,6 +57,9 @@ int strictb200_attn_paged(strictb200_ctx* ctx, const uint16_t* q, const uint16_t
   if (!B || !T) return STRICTB200_OK;
   SB_REQUIRE(q && kpages && vpages && out, "null pointer");
   SB_REQUIRE(aligned16(q) && aligned16(kpages) && aligned16(vpages) && aligned16(out), "q, pages and out must be 16-byte aligned");
+  const uint64_t rows = (uint64_t)T * Hq * D * 2, pages = (uint64_t)n_pages * Hkv * page * D * 2;
+  SB_REQUIRE(out == q || !overlap(out, rows, q, rows), "out overlaps q without being it");  // a row's place in the one is another row's in the other
+  SB_REQUIRE(!overlap(out, rows, kpages, pages) && !overlap(out, rows, vpages, pages), "out overlaps the pages");
   a.q = (const bf16*)q; a.k = (const bf16*)kpages; a.v = (const bf16*)vpages; a.out = (bf16*)out;
   a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.window = window; a.first = first; a.max_new = max_new; a.max_len = max_len; a.scale = scale;
   SB_ENTER(ctx);
@@ -73,8 +79,8 @@ int strictb200_rope_qknorm_paged(strictb200_ctx* ctx, const uint16_t* qkv, const
   SB_REQUIRE(!qgain == !kgain, "gains for both queries and keys, or for neither");
   SB_REQUIRE(aligned16(qkv) && aligned16(q_out) && aligned16(kpages) && aligned16(vpages) && aligned16(qgain) && aligned16(kgain),
              "rows, gains and pages must be 16-byte aligned");
-  const uintptr_t in = (uintptr_t)qkv, to = (uintptr_t)q_out, in_bytes = (uintptr_t)T * (Hq + 2 * (uintptr_t)Hkv) * D * 2, to_bytes = (uintptr_t)T * Hq * D * 2;
-  SB_REQUIRE(to >= in + in_bytes || in >= to + to_bytes, "q_out overlaps qkv");  // a row's place in the one is another row's in the other
+  const uint64_t in = (uint64_t)T * (Hq + 2 * (uint64_t)Hkv) * D * 2, rows = (uint64_t)T * Hq * D * 2;
+  SB_REQUIRE(!overlap(q_out, rows, qkv, in), "q_out overlaps qkv");  // a row's place in the one is another row's in the other
   a.qkv = (const bf16*)qkv; a.qgain = qgain; a.kgain = kgain; a.eps = eps; a.theta = theta; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
   a.q_out = (bf16*)q_out; a.k = (bf16*)kpages; a.v = (bf16*)vpages;
   SB_ENTER(ctx);

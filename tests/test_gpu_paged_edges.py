@@ -115,6 +115,19 @@ def test_heats_without_an_end(ctx, heat, rows):
 
 
 # ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("new,G,D", [(1, 4, 128), (4, 4, 64), (20, 4, 128), (200, 4, 64), (150, 5, 128)])
+@pytest.mark.parametrize("lens", [[7000, 300, 40], [260, 700] * 15])
+def test_rows_in_place_of_their_queries(ctx, new, G, D, lens):
+    """Every way the keys are cut and joined."""
+    c = Cache([max(n, new) for n in lens], [new] * len(lens), 2, D, 16, seed=new, front=1, behind=2)
+    q = torch.randn(c.T, 2 * G, D, generator=c.g, device="cuda").to(torch.bfloat16)
+    q[0], q[-2:] = 7.0, 7.0
+    want = c.attend(ctx, q)
+    for _ in range(3):
+        own = q.clone()
+        assert torch.equal(c.attend(ctx, own, out=own), want)
+
+
 def attend_far(ctx, c, q, far, window=0, first=0, max_len=None):
     """Sequence `far` is as long as an int32 says; what lies in the table is all that there is to see. Compared with a length just behind the table."""
     c.d_lens[far] = 2 ** 31 - 1

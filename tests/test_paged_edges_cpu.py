@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from strict_b200 import native as N
+from test_paged_cpu import A, attn
 
 ONE = 2.0 ** 43  # the weight of the largest logit
 
@@ -80,3 +81,20 @@ def test_top_k_of_every_size(wish, n, k, lists):
     cut, tried = N.lib()._Z13sb_draw_top_kii, N.lib()._Z13sb_draw_listsi
     cut.restype, cut.argtypes, tried.restype, tried.argtypes = C.c_int, [C.c_int, C.c_int], C.c_bool, [C.c_int]
     assert cut(wish, n) == k and tried(k) == lists
+
+
+FAR = A + 2 ** 40
+ROWS, PAGES = 2 * 8 * 128 * 2, 4 * 2 * 16 * 128 * 2  # bytes of the rows and of the pages of attn()'s arguments
+
+
+@pytest.mark.parametrize("out", [A + 16, A - 16, A + ROWS - 16, A - ROWS + 16])
+def test_attention_refuses_rows_over_other_rows_queries(out):
+    with pytest.raises(ValueError, match="out overlaps q"):
+        attn(k=FAR, v=FAR, out=out)
+
+
+@pytest.mark.parametrize("name", ["k", "v"])
+@pytest.mark.parametrize("out", [A, A + PAGES - 16, A - ROWS + 16])
+def test_attention_refuses_rows_over_pages(name, out):
+    with pytest.raises(ValueError, match="pages"):
+        attn(**{"q": FAR, "k": FAR, "v": FAR, name: A}, out=out)

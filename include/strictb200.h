@@ -338,7 +338,8 @@ int strictb200_argmax(strictb200_ctx* ctx, const float* d_x, int64_t M, int64_t 
  * d_temperature, d_top_k, d_top_p, d_min_p have a value per row and may be NULL. Temperature 0 or below (or NaN): the first of the order;
  * NULL: 1. top_k below 1 or from N on, top_p from 1 on (or NaN), min_p 0 or below (or NaN): without. top_p 0 or below keeps one token; min_p above 1 is 1.
  * NaN logits count as -inf, which is never drawn; a row without any other gives token -1 and share 0. Weights are held to 2^-42 of the largest, compared like that and
- * summed exactly, so that a result depends on nothing but the row's inputs. */
+ * summed exactly, so that a result depends on nothing but the row's inputs. d_out and d_prob may lie over arrays of a value per row (a row's values are read before its
+ * results are written), but overlap neither the logits nor one another. */
 int strictb200_sample(strictb200_ctx* ctx, const void* d_logits, int dtype, int64_t M, int64_t N, int64_t ld, const float* d_u, const float* d_temperature,
                       const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, int32_t* d_out, float* d_prob);
 

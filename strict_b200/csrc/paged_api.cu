@@ -122,6 +122,9 @@ int strictb200_sample(strictb200_ctx* ctx, const void* logits, int dtype, int64_
   SB_REQUIRE(((uintptr_t)logits & (dtype ? 3 : 1)) == 0, "logits must be aligned to their type");
   SB_REQUIRE(aligned4(u) && aligned4(temperature) && aligned4(top_k) && aligned4(top_p) && aligned4(min_p) && aligned4(out) && aligned4(prob),
              "arrays of a value per row must be aligned to their type");
+  const uint64_t row_bytes = (uint64_t)M * 4, bytes = ((uint64_t)(M - 1) * ld + N) * (dtype ? 4 : 2);
+  SB_REQUIRE(!overlap(out, row_bytes, logits, bytes) && !(prob && (overlap(prob, row_bytes, logits, bytes) || overlap(prob, row_bytes, out, row_bytes))),
+             "out and prob overlap neither the logits nor one another");
   SB_ENTER(ctx);
   return k_draw(ctx, logits, dtype, M, N, ld, u, temperature, top_k, top_p, min_p, out, prob);
 }

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import paged_plain as plain
+from strict_b200 import native as N
 from test_gpu_draw import check, logits, sample
 from test_gpu_paged import Cache
 
@@ -112,6 +113,21 @@ def test_heats_without_an_end(ctx, heat, rows):
             if rows > 2 and len(kw) != 1:
                 continue
             check_whole(ctx, x, u, heat, **kw, off=2.0 ** -43)  # weights below 2^-44 of the largest are 0, the others here are all the same
+
+
+@pytest.mark.parametrize("m", [3, 400])
+def test_results_over_what_a_row_reads_once(ctx, m):
+    """Tokens over the random numbers, shares over min_p."""
+    n = 20011
+    rng = np.random.default_rng(6)
+    x, u, least = logits(m, n, 6), rng.random(m, np.float32), rng.choice([0.0, 0.05, 0.3], m).astype(np.float32)
+    k, p = rng.choice([0, 3, 5000], m).astype(np.int32), rng.choice([0.5, 0.9, 1.0], m).astype(np.float32)
+    want = sample(ctx, x, u, top_k=k, top_p=p, min_p=least)
+    du, dk, dp, dq = (torch.from_numpy(v).cuda() for v in (u, k, p, least))
+    torch.cuda.synchronize()
+    N.check(N.lib().strictb200_sample(ctx.h, x.data_ptr(), 1, m, n, n, du.data_ptr(), None, dk.data_ptr(), dp.data_ptr(), dq.data_ptr(), du.data_ptr(), dq.data_ptr()))
+    ctx.synchronize()
+    assert np.array_equal(du.cpu().numpy().view(np.int32), want[0]) and np.array_equal(dq.cpu().numpy(), want[1])
 
 
 # ------------------------------------------------------------------ attention

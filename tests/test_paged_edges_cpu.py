@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from strict_b200 import native as N
-from test_paged_cpu import A, attn
+from test_paged_cpu import A, attn, sample
 
 ONE = 2.0 ** 43  # the weight of the largest logit
 
@@ -98,3 +98,11 @@ def test_attention_refuses_rows_over_other_rows_queries(out):
 def test_attention_refuses_rows_over_pages(name, out):
     with pytest.raises(ValueError, match="pages"):
         attn(**{"q": FAR, "k": FAR, "v": FAR, name: A}, out=out)
+
+
+@pytest.mark.parametrize("kw", [dict(out=A), dict(out=A + 4 * 249), dict(out=A - 4), dict(out=FAR, prob=A + 4 * 249), dict(out=FAR, prob=FAR), dict(out=FAR, prob=FAR + 4),
+                                dict(out=A + 2 * 248, dtype=0)], ids=str)
+def test_draws_refuse_results_over_logits(kw):
+    """Two rows of 100 logits, 150 apart."""
+    with pytest.raises(ValueError, match="overlap"):
+        sample(**{**dict(M=2, N=100, ld=150, u=FAR, t=FAR, k=FAR, p=FAR, q=FAR, prob=None), **kw})

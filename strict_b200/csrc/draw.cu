@@ -97,7 +97,7 @@ struct Shared {
   uint64_t part_sum[BINS / 2];
   uint64_t total_count, total_sum;
   uint64_t red[32], red2[32];
-  uint64_t pick[6];
+  uint64_t pick[4];
   uint64_t best, there, weights, word, drawn;  // what blocks tell one another: largest place, numbers, sums, a cut, the kept weights
   uint32_t n_list;
   long long fraction[64 * 8];  // bits of 2^(43 + i / 64), eight copies side by side: neighbouring lanes read other banks
@@ -125,7 +125,7 @@ struct Row {
   Shared& s;
   const float* near;  // the first `held` of this block's `share` of the logits
   const void* x;
-  int N, f32, vec, first, share, held;  // vec: rows begin at 16 bytes
+  int f32, vec, first, share, held;  // vec: rows begin at 16 bytes
   int blocks, rank, crests;  // crests: groups of this block's threads
   double m, scale;  // the largest logit, 64 log2(e) / temperature
   float m32, bin_scale, least_l, zero_l;  // least_l: from here on a weight is not 0 (2^-45 of the largest); zero_l: a little below
@@ -523,7 +523,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) draw_kernel(const __g
   const int span = ((a.N + (int)blocks - 1) / (int)blocks + 7) / 8 * 8;
   Row r{s, near};
   r.x = (const char*)a.x + row * a.ld * (a.f32 ? 4 : 2);
-  r.N = a.N;
   r.f32 = a.f32;
   r.blocks = (int)blocks;
   r.rank = (int)rank;

@@ -43,17 +43,6 @@ int k_rope_paged(strictb200_ctx*, const PagedRopeArgs& a);  // rope_paged.cu
 int k_pages_copy(strictb200_ctx*, void* const* pools, int n_pools, int64_t page_bytes, const int32_t* src, const int32_t* dst, int n);
 
 #ifdef __CUDACC__
-// Sequence of packed row t (0 <= t < T): the first b with t < starts[b + 1]; B where the row is in front of the first or behind the last
-// sequence. All lanes of a warp call it with the same t.
-__device__ __forceinline__ int paged_seq(const PagedView& v, int64_t t) {
-  const int lane = threadIdx.x & 31;
-  for (int b0 = 0; b0 < v.B; b0 += 32) {
-    const int b = b0 + lane;
-    const unsigned past = __ballot_sync(0xffffffffu, b < v.B && t < v.starts[min(b, v.B - 1) + 1]);
-    if (past) return t >= v.starts[0] ? b0 + __ffs(past) - 1 : v.B;
-  }
-  return v.B;
-}
 // Page of slot group `n` of sequence b, or -1 where the table names none.
 __device__ __forceinline__ int paged_page(const PagedView& v, int b, int n) {
   if ((unsigned)n >= (unsigned)v.ld) return -1;

@@ -34,7 +34,8 @@ __device__ __forceinline__ Eight eight(const float* p, int further) {
   return Eight{{{a.x, a.y}, {a.z, a.w}, {b.x, b.y}, {b.z, b.w}}};
 }
 
-// paged_seq and the row's position, all of it from one round of loads
+// Sequence of packed row t (0 <= t < T), the first b with t < starts[b + 1], and the row's position, all of it from one round of loads; B where the row is in
+// front of the first or behind the last sequence. All lanes of a warp call it with the same t.
 __device__ __forceinline__ int place(const PagedView& v, int64_t t, int* pos) {
   const int lane = threadIdx.x & 31, s0 = v.starts[0];
   for (int b0 = 0; b0 < v.B; b0 += 32) {

@@ -13,7 +13,8 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Bound by HBM: every key and value is read once (64 sequences of 1 to 16 thousand keys, 2.28 GB: 339 us, 6.7 TB/s). A block is one key/value head of one sequence and a share of its tiles of 64 keys. The last warp copies:
+// Bound by HBM: every key and value is read once (64 sequences of 1 to 16 thousand keys, 2.28 GB: 339 us, 6.7 TB/s; times in these files are
+// of calls in a row on the same data, 352 us with other data between them). A block is one key/value head of one sequence and a share of its tiles of 64 keys. The last warp copies:
 // its lanes look the pages up, well ahead, and request the tile by TMA (boxes of min(page, 64) keys x 64 dims, 128-byte swizzle) into a ring
 // of `stages`. The others have 16 keys of every tile and all 8 NB rows each, with a softmax of their own; the four shares of the keys are
 // joined at the end.

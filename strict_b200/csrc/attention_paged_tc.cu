@@ -768,7 +768,8 @@ int launch(strictb200_ctx* ctx, const PagedAttnArgs& a) {
   // Parts, by key tiles as the unit of time (2.6 us; 1.5 with one tile): rounds of units that are all as long, each with three tiles more for its start and
   // its end, and, where there are several sequences, lengths spread below max_len (mean 0.65): then the longest unit, or what the SMs have to do together.
   // A prompt's rows see half of it. The join costs 4 us and its bytes. (16 sequences of 1.5 to 8 thousand keys, five new tokens, eight heads:
-  // one part 121 us, two 84, four 96; one of 16 thousand, 512 new tokens: two 176, three 229, four 193.)
+  // one part 121 us, two 84, four 96; one of 16 thousand, 512 new tokens: two 176, three 229, four 193. Calls in a row on the same data; with other data in between two
+  // parts take 92 and 200.)
   const double units = (double)std::max<int64_t>((a.at.T + tb - 1) / tb, a.at.B) * a.Hkv, sms = ctx->sm_count;
   const double keys = (double)std::max<int64_t>(1, paged_walk_tiles(a, BKV)), seen = keys * (1 - 0.5 * std::min(1.0, (double)a.max_new / std::max(1, a.max_len)));
   const int outs = ONE ? 2 : 1;

@@ -18,8 +18,10 @@
 //   those in front of and in that bin go to the first block as above, if there are at most LIST        three meetings
 //   otherwise the place where the order is cut is found among those of the bin (in the first block if there are at most LIST, by bits of the place where
 //   more share the bin), and all blocks sum the kept weights and look for the token
-// Many rows: a block per row, which keeps a part of it and reads the rest again from L2 in every pass; instruction issue bounds it (256 rows of 151936: 37 us
-// greedy, 77 with top_k 20, 107 unfiltered, 270 to 400 with a top_p of 0.9 over flat logits; one row 7.4, 13.4, 13.4, 42 to 57).
+// Many rows: a block per row, which keeps a part of it and reads the rest again from L2 in every pass; the instructions of an SM's row bound it (256 rows of 151936: 37 us
+// greedy, 77 with top_k 20, 107 unfiltered, 270 to 400 with a top_p of 0.9 over flat logits; one row 7.4, 13.4, 13.4, 42 to 57). A row with a top_p that no short list holds
+// takes 160 us on its SM, 75 or 148 of them as long as one, and with mixed wishes (170 us) such a row is the launch: most other SMs are done before it.
+// Times here and below: calls in a row on the same logits.
 #include <algorithm>
 
 #include "common.cuh"
